@@ -42,7 +42,8 @@ typedef enum {
   VS_F16 = 1,  ///< IEEE binary16 stored as uint16
   VS_I16 = 2,
   VS_I32 = 3,
-  VS_U8 = 4
+  VS_U8 = 4,
+  VS_BF16 = 5  ///< bfloat16 stored as uint16 (sequence operators)
 } vs_dtype;
 
 /* ---------------------------------------------------------------- runtime */
@@ -335,6 +336,43 @@ vs_status vs_detect_peaks_batched(const float *x, size_t n, int64_t x_stride, si
                                   int type, void *pos_dev, int pos64, float *val_dev,
                                   size_t capacity, unsigned long long *row_start_dev,
                                   vs_stream_t stream);
+
+/* --------------------------------------------------- sequence operators */
+/// Gated linear recurrence over [batch][t][d] arrays (dtype VS_F32, VS_F16 or
+/// VS_BF16; channels contiguous, the other strides in elements and free):
+///   i = 1 / (1 + exp(gate)), h_t = h_{t-1} + i_t (x_t - h_{t-1}), y_t = h_t.
+/// state: h_0, fp32 [batch][d] (NULL: zeros).  lengths: int32 (lengths64 = 0)
+/// or int64 [batch] on the device (NULL: t for all), clamped to 0..t; steps
+/// from lengths[b] on are padding: they are not read, y is 0 there and the
+/// state passes through.  y is [batch][t][d], final_state fp32 [batch][d].
+/// starts: NULL, or fp32 [batch][vs_gated_recurrence_tiles(t)][d], which the
+/// backward pass reads.  workspace: device memory of
+/// vs_gated_recurrence_workspace(batch, t, d) bytes (the same for both
+/// directions), or NULL for the library's pool.
+vs_status vs_gated_recurrence(int dtype, const void *x, int64_t x_batch, int64_t x_time,
+                              const void *gate, int64_t gate_batch, int64_t gate_time,
+                              const float *state, const void *lengths, int lengths64,
+                              int64_t batch, int64_t t, int64_t d, void *y, float *final_state,
+                              float *starts, void *workspace, size_t workspace_bytes,
+                              vs_stream_t stream);
+int64_t vs_gated_recurrence_tiles(int64_t t);
+size_t vs_gated_recurrence_workspace(int64_t batch, int64_t t, int64_t d);
+/// Gradients of vs_gated_recurrence: dx and dgate [batch][t][d] (0 in the
+/// padding), dstate fp32 [batch][d] (or NULL), from dy (strides dy_batch,
+/// dy_time; NULL: zeros) and dfinal fp32 [batch][d] (NULL: zeros).  starts is
+/// what the forward call with the same lengths wrote.
+vs_status vs_gated_recurrence_backward(int dtype, const void *x, int64_t x_batch, int64_t x_time,
+                                       const void *gate, int64_t gate_batch, int64_t gate_time,
+                                       const void *lengths, int lengths64, const float *starts,
+                                       const void *dy, int64_t dy_batch, int64_t dy_time,
+                                       const float *dfinal, int64_t batch, int64_t t, int64_t d,
+                                       void *dx, void *dgate, float *dstate, void *workspace,
+                                       size_t workspace_bytes, vs_stream_t stream);
+/// One step for [batch][d] rows (strides x_batch, gate_batch): state (fp32,
+/// [batch][d]) is updated in place, y [batch][d] is the new state.
+vs_status vs_gated_recurrence_step(int dtype, const void *x, int64_t x_batch, const void *gate,
+                                   int64_t gate_batch, float *state, int64_t batch, int64_t d,
+                                   void *y, vs_stream_t stream);
 
 SIMD_API_END
 

@@ -103,6 +103,13 @@ _SIGNATURES = {
     "vs_dwt_multilevel": (_i, [_i, _i, _i, _i, _vp, _i64, _vp, _i, _vp]),
     "vs_wavelet_filter": (_i, [_i, _i, _vp]),
     "vs_detect_peaks": (_i, [_vp, _sz, _i, _vp, _vp, _sz, _vp, _vp]),
+    "vs_gated_recurrence": (_i, [_i, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i, _i64, _i64, _i64,
+                                 _vp, _vp, _vp, _vp, _sz, _vp]),
+    "vs_gated_recurrence_tiles": (_i64, [_i64]),
+    "vs_gated_recurrence_workspace": (_sz, [_i64, _i64, _i64]),
+    "vs_gated_recurrence_backward": (_i, [_i, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i, _vp, _vp, _i64,
+                                          _i64, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "vs_gated_recurrence_step": (_i, [_i, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _vp, _vp]),
     # multi-GPU layer (include/simd/dist.h)
     "vs_dist_create": (_i, [_i, _vp, _i, ctypes.POINTER(_vp)]),
     "vs_dist_destroy": (_i, [_vp]),

@@ -17,6 +17,26 @@ def stream_of(t: torch.Tensor) -> ctypes.c_void_p:
     return ctypes.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
 
 
+def raw_stream(t: torch.Tensor) -> int:
+    """Handle of t's device's current stream."""
+    return torch._C._cuda_getCurrentRawStream(t.device.index)
+
+
+def plain_call(*tensors) -> bool:
+    """True when a call needs none of the dispatcher's services: ordinary tensors, no gradient to
+    record, nothing tracing.  The implementation is then called directly, which takes several
+    microseconds of host time off the calls of a decoding loop."""
+    if torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack() \
+            or torch._C._functorch.peek_interpreter_stack() is not None:
+        return False
+    grad = torch.is_grad_enabled()
+    for t in tensors:
+        if t is not None and (type(t) not in (torch.Tensor, torch.nn.Parameter)
+                              or (grad and t.requires_grad)):
+            return False
+    return True
+
+
 @contextlib.contextmanager
 def on_device(t: torch.Tensor):
     """Make t's GPU the current HIP device for the native launch."""

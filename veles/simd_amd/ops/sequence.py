@@ -1,0 +1,267 @@
+"""Operators of sequence models: the gated linear recurrence (forward, gradient, single-token step).
+
+The counterparts of conv1d for filters whose coefficient changes from sample to sample.  GPU
+tensors run the native HIP kernels; CPU tensors run the definition step by step in float64.
+"""
+from __future__ import annotations
+
+import torch
+
+from .. import _lib
+from ._util import on_device, plain_call, ptr, raw_stream, require_gpu_tensor
+
+DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 5}
+
+
+def _opt(t):
+    return None if t is None else ptr(t)
+
+
+def _rows_last(t: torch.Tensor) -> torch.Tensor:
+    """t with neighbouring elements in its last dimension (a copy only where they are not)."""
+    return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
+
+
+def _same_device(name, first, **others):
+    for n, t in others.items():
+        if t is not None and t.device != first.device:
+            raise ValueError(f"{name}: {n} is on {t.device}, x on {first.device}")
+
+
+# ------------------------------------------------------- gated recurrence
+def _check_recurrence(name, x, gate, state, lengths):
+    if x.dtype not in DTYPES:
+        raise TypeError(f"{name}: x is {x.dtype}; float32, float16 or bfloat16 expected")
+    if gate.dtype != x.dtype:
+        raise TypeError(f"{name}: gate is {gate.dtype}, x {x.dtype}")
+    if x.dim() != 3 or gate.shape != x.shape:
+        raise ValueError(f"{name}: x and gate are [batch, time, channels]; got {tuple(x.shape)} and "
+                         f"{tuple(gate.shape)}")
+    if state is not None:
+        if state.dtype != torch.float32:
+            raise TypeError(f"{name}: the state is float32; got {state.dtype}")
+        if tuple(state.shape) != (x.shape[0], x.shape[2]):
+            raise ValueError(f"{name}: state {tuple(state.shape)}, [batch, channels] = "
+                             f"{(x.shape[0], x.shape[2])} expected")
+    if lengths is not None:
+        if lengths.dtype not in (torch.int32, torch.int64):
+            raise TypeError(f"{name}: lengths are int32 or int64; got {lengths.dtype}")
+        if tuple(lengths.shape) != (x.shape[0],):
+            raise ValueError(f"{name}: lengths {tuple(lengths.shape)}, one per sequence "
+                             f"({x.shape[0]}) expected")
+    _same_device(name, x, gate=gate, state=state, lengths=lengths)
+
+
+def _tiles(t: int) -> int:
+    return int(_lib.lib().vs_gated_recurrence_tiles(t))
+
+
+def _recurrence_workspace(x):
+    size = int(_lib.lib().vs_gated_recurrence_workspace(*x.shape))
+    return torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
+
+
+def _valid_steps(x, lengths):
+    n = torch.full((x.shape[0],), x.shape[1]) if lengths is None else lengths.clamp(0, x.shape[1])
+    return torch.arange(x.shape[1])[:, None] < n[None, :]      # [time, batch]
+
+
+def _recurrence_cpu(x, gate, state, lengths, save):
+    b, t, d = x.shape
+    on = _valid_steps(x, lengths)
+    h = torch.zeros(b, d, dtype=torch.float64) if state is None else state.double()
+    xd, i = x.double(), torch.sigmoid(-gate.double())
+    y = torch.zeros(b, t, d, dtype=torch.float64)
+    for s in range(t):
+        h = torch.where(on[s][:, None], h + i[:, s] * (xd[:, s] - h), h)
+        y[:, s] = torch.where(on[s][:, None], h, 0.0)
+    # the CPU backward starts from the initial state: one tile
+    starts = (torch.zeros(b, d) if state is None else state)[:, None].clone() if save else x.new_empty(
+        0, dtype=torch.float32)
+    return y.to(x.dtype), h.float(), starts
+
+
+def _recurrence_impl(x, gate, state, lengths, save):
+    _check_recurrence("veles::gated_recurrence", x, gate, state, lengths)
+    if not x.is_cuda:
+        return _recurrence_cpu(x, gate, state, lengths, save)
+    require_gpu_tensor(x, "veles::gated_recurrence")
+    b, t, d = x.shape
+    x, gate = _rows_last(x), _rows_last(gate)
+    state = None if state is None else state.contiguous()
+    lengths = None if lengths is None else lengths.contiguous()
+    y = torch.empty((b, t, d), dtype=x.dtype, device=x.device)
+    final = torch.empty((b, d), dtype=torch.float32, device=x.device)
+    starts = torch.empty((b, _tiles(t), d) if save else (0,), dtype=torch.float32, device=x.device)
+    ws = _recurrence_workspace(x)
+    with on_device(x):
+        _lib.call("vs_gated_recurrence", DTYPES[x.dtype], ptr(x), x.stride(0), x.stride(1), ptr(gate),
+                  gate.stride(0), gate.stride(1), _opt(state), _opt(lengths),
+                  int(lengths is not None and lengths.dtype == torch.int64), b, t, d, ptr(y), ptr(final),
+                  ptr(starts) if save else None, _opt(ws), 0 if ws is None else ws.numel(), raw_stream(x))
+    return y, final, starts
+
+
+def _recurrence_backward_cpu(x, gate, lengths, starts, dy, dfinal):
+    b, t, d = x.shape
+    on = _valid_steps(x, lengths)
+    xd, i = x.double(), torch.sigmoid(-gate.double())
+    h = starts[:, 0].double()
+    before = torch.zeros(b, t, d, dtype=torch.float64)
+    for s in range(t):
+        before[:, s] = h
+        h = torch.where(on[s][:, None], h + i[:, s] * (xd[:, s] - h), h)
+    m = torch.zeros(b, d, dtype=torch.float64) if dfinal is None else dfinal.double()
+    dx, dg = torch.zeros(b, t, d, dtype=torch.float64), torch.zeros(b, t, d, dtype=torch.float64)
+    for s in range(t - 1, -1, -1):
+        k = on[s][:, None]
+        lam = m if dy is None else m + dy[:, s].double()
+        dx[:, s] = torch.where(k, i[:, s] * lam, 0.0)
+        dg[:, s] = torch.where(k, i[:, s] * (1 - i[:, s]) * lam * (before[:, s] - xd[:, s]), 0.0)
+        m = torch.where(k, (1 - i[:, s]) * lam, m)
+    return dx.to(x.dtype), dg.to(x.dtype), m.float()
+
+
+def _recurrence_backward_impl(x, gate, lengths, starts, dy, dfinal):
+    name = "veles::gated_recurrence_backward"
+    _check_recurrence(name, x, gate, dfinal, lengths)
+    if dy is not None and (dy.shape != x.shape or dy.dtype != x.dtype):
+        raise ValueError(f"{name}: dy is {dy.dtype} {tuple(dy.shape)}, {x.dtype} {tuple(x.shape)} expected")
+    if starts.dtype != torch.float32:
+        raise TypeError(f"{name}: the saved states are float32; got {starts.dtype}")
+    _same_device(name, x, starts=starts, dy=dy)
+    b, t, d = x.shape
+    want = (b, _tiles(t) if x.is_cuda else 1, d)
+    if tuple(starts.shape) != want:
+        raise ValueError(f"{name}: saved states {tuple(starts.shape)}, {want} expected")
+    if not x.is_cuda:
+        return _recurrence_backward_cpu(x, gate, lengths, starts, dy, dfinal)
+    require_gpu_tensor(x, name)
+    x, gate = _rows_last(x), _rows_last(gate)
+    dy = None if dy is None else _rows_last(dy)
+    dfinal = None if dfinal is None else dfinal.contiguous()
+    lengths = None if lengths is None else lengths.contiguous()
+    starts = starts.contiguous()
+    dx = torch.empty((b, t, d), dtype=x.dtype, device=x.device)
+    dg = torch.empty_like(dx)
+    dstate = torch.empty((b, d), dtype=torch.float32, device=x.device)
+    ws = _recurrence_workspace(x)
+    with on_device(x):
+        _lib.call("vs_gated_recurrence_backward", DTYPES[x.dtype], ptr(x), x.stride(0), x.stride(1),
+                  ptr(gate), gate.stride(0), gate.stride(1), _opt(lengths),
+                  int(lengths is not None and lengths.dtype == torch.int64), ptr(starts), _opt(dy),
+                  0 if dy is None else dy.stride(0), 0 if dy is None else dy.stride(1), _opt(dfinal), b, t, d,
+                  ptr(dx), ptr(dg), ptr(dstate), _opt(ws), 0 if ws is None else ws.numel(), raw_stream(x))
+    return dx, dg, dstate
+
+
+def _recurrence_fake(x, gate, state, lengths, save):
+    _check_recurrence("veles::gated_recurrence", x, gate, state, lengths)
+    b, t, d = x.shape
+    starts = (b, _tiles(t) if x.is_cuda else 1, d) if save else (0,)
+    return (x.new_empty((b, t, d)), x.new_empty((b, d), dtype=torch.float32),
+            x.new_empty(starts, dtype=torch.float32))
+
+
+def _recurrence_setup(ctx, inputs, output):
+    x, gate, state, lengths, save = inputs
+    if not save:
+        raise RuntimeError("veles::gated_recurrence: gradients need the saved states (save=True)")
+    ctx.set_materialize_grads(False)
+    ctx.mark_non_differentiable(output[2])
+    ctx.save_for_backward(x, gate, lengths, output[2])
+
+
+def _recurrence_grad(ctx, dy, dfinal, _):
+    x, gate, lengths, starts = ctx.saved_tensors
+    if dy is None and dfinal is None:
+        return None, None, None, None, None
+    dx, dg, dstate = torch.ops.veles.gated_recurrence_backward(x, gate, lengths, starts, dy, dfinal)
+    need = ctx.needs_input_grad
+    return dx if need[0] else None, dg if need[1] else None, dstate if need[2] else None, None, None
+
+
+def _no_second_derivative(name):
+    def setup(ctx, inputs, output):
+        pass
+
+    def grad(ctx, *_):
+        raise NotImplementedError(f"{name} has no derivative of its own (second derivatives)")
+    torch.library.register_autograd(name, grad, setup_context=setup)
+
+
+torch.library.define("veles::gated_recurrence",
+                     "(Tensor x, Tensor gate, Tensor? state, Tensor? lengths, bool save) -> (Tensor, Tensor, Tensor)")
+torch.library.impl("veles::gated_recurrence", "default", _recurrence_impl)
+torch.library.register_fake("veles::gated_recurrence", _recurrence_fake)
+torch.library.register_autograd("veles::gated_recurrence", _recurrence_grad, setup_context=_recurrence_setup)
+torch.library.define("veles::gated_recurrence_backward",
+                     "(Tensor x, Tensor gate, Tensor? lengths, Tensor starts, Tensor? dy, Tensor? dfinal) -> "
+                     "(Tensor, Tensor, Tensor)")
+torch.library.impl("veles::gated_recurrence_backward", "default", _recurrence_backward_impl)
+torch.library.register_fake(
+    "veles::gated_recurrence_backward",
+    lambda x, gate, lengths, starts, dy, dfinal: (
+        x.new_empty(x.shape), x.new_empty(x.shape),
+        x.new_empty((x.shape[0], x.shape[2]), dtype=torch.float32)))
+_no_second_derivative("veles::gated_recurrence_backward")
+
+
+def gated_recurrence(x: torch.Tensor, gate: torch.Tensor, state: torch.Tensor | None = None,
+                     lengths: torch.Tensor | None = None):
+    """Gated linear recurrence along time, (y, final_state):
+
+        i_t = sigmoid(-gate_t),  h_t = h_{t-1} + i_t (x_t - h_{t-1}),  y_t = h_t
+
+    x, gate: [batch, time, channels], float32, float16 or bfloat16, any batch and time strides.
+    state: h_0, float32 [batch, channels] (zeros if None); final_state is the float32 state after
+    the last step, so a sequence can be continued by another call or by gated_recurrence_step.
+    lengths: int32 / int64 [batch] on x's device: steps from lengths[b] on are padding (not read,
+    y = 0, the state passes through; values outside 0..time are clamped).
+    The state is held in float32.  Differentiable in x, gate and state; in the padding the
+    gradients are 0 and dy is not read.  Where the update meets an infinite state or value inside
+    a sequence it follows the formula above (inf - inf is NaN)."""
+    if plain_call(x, gate, state, lengths):
+        return _recurrence_impl(x, gate, state, lengths, False)[:2]
+    save = torch.is_grad_enabled() and any(
+        v is not None and v.requires_grad for v in (x, gate, state))
+    y, final, _ = torch.ops.veles.gated_recurrence(x, gate, state, lengths, save)
+    return y, final
+
+
+def _step_impl(x, gate, state):
+    name = "veles::gated_recurrence_step"
+    if x.dim() != 2:
+        raise ValueError(f"{name}: x and gate are [batch, channels]; got {tuple(x.shape)}")
+    if gate.dim() != 2:
+        raise ValueError(f"{name}: x and gate are [batch, channels]; got {tuple(gate.shape)}")
+    _check_recurrence(name, x[:, None], gate[:, None], state, None)
+    if not state.is_contiguous():
+        raise ValueError(f"{name}: the state is updated in place and has to be contiguous")
+    if not x.is_cuda:
+        state += torch.sigmoid(-gate.double()) * (x.double() - state)
+        return state.to(x.dtype, copy=True)
+    require_gpu_tensor(x, name)
+    x, gate = _rows_last(x), _rows_last(gate)
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    with on_device(x):
+        _lib.call("vs_gated_recurrence_step", DTYPES[x.dtype], ptr(x), x.stride(0), ptr(gate), gate.stride(0),
+                  ptr(state), x.shape[0], x.shape[1], ptr(y), raw_stream(x))
+    return y
+
+
+torch.library.define("veles::gated_recurrence_step", "(Tensor x, Tensor gate, Tensor(a!) state) -> Tensor")
+torch.library.impl("veles::gated_recurrence_step", "default", _step_impl)
+torch.library.register_fake("veles::gated_recurrence_step", lambda x, gate, state: x.new_empty(x.shape))
+
+
+def gated_recurrence_step(x: torch.Tensor, gate: torch.Tensor, state: torch.Tensor) -> torch.Tensor:
+    """One step of gated_recurrence for a batch of sequences: x, gate [batch, channels]; state
+    (float32 [batch, channels], contiguous) is updated in place and returned as y in x's type.
+    For generation: it records no gradient."""
+    if plain_call(x, gate, state):
+        return _step_impl(x, gate, state)
+    if torch.is_grad_enabled() and (x.requires_grad or gate.requires_grad or state.requires_grad):
+        raise RuntimeError("gated_recurrence_step records no gradient: call it under torch.no_grad(), or use "
+                           "gated_recurrence")
+    return torch.ops.veles.gated_recurrence_step(x, gate, state)
