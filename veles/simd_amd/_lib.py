@@ -110,6 +110,7 @@ _SIGNATURES = {
     "vs_gated_recurrence_backward": (_i, [_i, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i, _vp, _vp, _i64,
                                           _i64, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _sz, _vp]),
     "vs_gated_recurrence_step": (_i, [_i, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _vp, _vp]),
+    "vs_matvec_int4": (_i, [_i, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _vp]),
     # multi-GPU layer (include/simd/dist.h)
     "vs_dist_create": (_i, [_i, _vp, _i, ctypes.POINTER(_vp)]),
     "vs_dist_destroy": (_i, [_vp]),

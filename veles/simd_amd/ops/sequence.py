@@ -265,3 +265,114 @@ def gated_recurrence_step(x: torch.Tensor, gate: torch.Tensor, state: torch.Tens
         raise RuntimeError("gated_recurrence_step records no gradient: call it under torch.no_grad(), or use "
                            "gated_recurrence")
     return torch.ops.veles.gated_recurrence_step(x, gate, state)
+
+
+# -------------------------------------------------------- 4-bit products
+def _check_group(name, group_size):
+    if group_size not in (32, 64) and (group_size <= 0 or group_size % 128):
+        raise ValueError(f"{name}: group size {group_size}; 32, 64 or a multiple of 128 expected")
+
+
+def _check_matvec(name, x, qweight, scales, zeros, group_size):
+    if x.dtype not in (torch.bfloat16, torch.float16):
+        raise TypeError(f"{name}: x is {x.dtype}; float16 or bfloat16 expected")
+    if x.dim() < 1 or qweight.dim() != 2 or qweight.dtype != torch.uint8:
+        raise ValueError(f"{name}: x [..., k] and uint8 qweight [n, (k + 1) // 2] expected")
+    _check_group(name, group_size)
+    n, k = qweight.shape[0], x.shape[-1]
+    if qweight.shape[1] != (k + 1) // 2:
+        raise ValueError(f"{name}: qweight {tuple(qweight.shape)} does not fit x with {k} columns")
+    groups = (n, -(-k // group_size))
+    if scales.dtype != x.dtype:
+        raise TypeError(f"{name}: scales are {scales.dtype}, x {x.dtype}")
+    if tuple(scales.shape) != groups:
+        raise ValueError(f"{name}: scales {tuple(scales.shape)}, {groups} expected")
+    if zeros is not None and (zeros.dtype != torch.uint8 or tuple(zeros.shape) != groups):
+        raise ValueError(f"{name}: zeros {zeros.dtype} {tuple(zeros.shape)}, uint8 {groups} expected")
+    if n > 1 and k > 2 and qweight.stride(1) != 1:
+        raise ValueError(f"{name}: the bytes of a row of qweight have to be neighbours")
+    _same_device(name, x, qweight=qweight, scales=scales, zeros=zeros)
+
+
+def _matvec_impl(x, qweight, scales, zeros, group_size):
+    name = "veles::matvec_int4"
+    _check_matvec(name, x, qweight, scales, zeros, group_size)
+    n, k = qweight.shape[0], x.shape[-1]
+    if not x.is_cuda:
+        q = torch.stack([qweight & 15, qweight >> 4], -1).flatten(1)[:, :k].double()
+        at = torch.arange(k) // group_size
+        z = 8.0 if zeros is None else zeros.double()[:, at]
+        return (x.double() @ ((q - z) * scales.double()[:, at]).t()).to(x.dtype)
+    require_gpu_tensor(x, name)
+    rows = x if x.dim() == 2 else x.reshape(-1, k) if k else x.new_empty((x[..., 0:0].numel(), 0))
+    rows = _rows_last(rows)
+    y = torch.empty((*x.shape[:-1], n), dtype=x.dtype, device=x.device)
+    scales = scales.contiguous()
+    zeros = None if zeros is None else zeros.contiguous()
+    with on_device(x):
+        _lib.call("vs_matvec_int4", DTYPES[x.dtype], ptr(rows), rows.stride(0), ptr(qweight), qweight.stride(0),
+                  ptr(scales), _opt(zeros), group_size, y.numel() // max(n, 1), n, k, ptr(y), raw_stream(x))
+    return y
+
+
+def _matvec_fake(x, qweight, scales, zeros, group_size):
+    _check_matvec("veles::matvec_int4", x, qweight, scales, zeros, group_size)
+    return x.new_empty((*x.shape[:-1], qweight.shape[0]))
+
+
+torch.library.define("veles::matvec_int4",
+                     "(Tensor x, Tensor qweight, Tensor scales, Tensor? zeros, int group_size) -> Tensor")
+torch.library.impl("veles::matvec_int4", "default", _matvec_impl)
+torch.library.register_fake("veles::matvec_int4", _matvec_fake)
+
+
+def matvec_int4(x: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor,
+                zeros: torch.Tensor | None = None, group_size: int = 128) -> torch.Tensor:
+    """x @ W.T for few rows x [..., k] (float16 or bfloat16) and a weight kept in 4 bits:
+
+        W[n, j] = (q[n, j] - zeros[n, j // group_size]) * scales[n, j // group_size]
+
+    qweight: uint8 [n, (k + 1) // 2], two numbers 0..15 to a byte, the even column in the low half.
+    scales: x's type, [n, ceil(k / group_size)]; zeros: uint8 of that shape (8 everywhere if None).
+    group_size: 32, 64 or a multiple of 128; the last group may end early.  Weights are exact and sums
+    are float32; the result is rounded once, to x's type.  An infinite x gives NaN (the zero point is
+    taken off the sum).  For generation: it records no gradient; more than 16 rows read the weights
+    once for every 16.  quantize_int4 makes the operands."""
+    if plain_call(x, qweight, scales, zeros):
+        return _matvec_impl(x, qweight, scales, zeros, group_size)
+    if torch.is_grad_enabled() and (x.requires_grad or scales.requires_grad):
+        raise RuntimeError("matvec_int4 records no gradient: call it under torch.no_grad()")
+    return torch.ops.veles.matvec_int4(x, qweight, scales, zeros, group_size)
+
+
+def quantize_int4(weight: torch.Tensor, group_size: int = 128, symmetric: bool = False,
+                  dtype: torch.dtype | None = None):
+    """(qweight, scales, zeros) of a weight [n, k] for matvec_int4, to be made once and kept.  Every
+    group's range, zero included, is cut into 15 steps (symmetric: +-7 steps around 8, zeros None).
+    dtype: of the scales, the type that x will have (weight's, or bfloat16 for a float32 weight)."""
+    _check_group("quantize_int4", group_size)
+    if weight.dim() != 2 or not weight.is_floating_point():
+        raise ValueError(f"quantize_int4: a floating weight [n, k] expected; got {weight.dtype} {tuple(weight.shape)}")
+    dtype = dtype or (weight.dtype if weight.dtype in (torch.float16, torch.bfloat16) else torch.bfloat16)
+    if dtype not in (torch.float16, torch.bfloat16):
+        raise TypeError(f"quantize_int4: scales of {dtype}; float16 or bfloat16 expected")
+    w = weight.detach().float()
+    if not torch.isfinite(w).all():
+        raise ValueError("quantize_int4: the weight has values that are not finite")
+    n, k = w.shape
+    groups = -(-k // group_size)
+    w = torch.nn.functional.pad(w, (0, groups * group_size - k)).view(n, groups, group_size)
+    if symmetric:
+        step = w.abs().amax(-1) / 7 if groups else w.new_zeros(n, 0)
+    else:
+        lo, hi = (w.amin(-1).clamp(max=0), w.amax(-1).clamp(min=0)) if groups else (w.new_zeros(n, 0),) * 2
+        step = (hi - lo) / 15
+    scales = step.to(dtype)
+    if not torch.isfinite(scales).all():
+        raise ValueError(f"quantize_int4: a group's step does not fit {dtype}")
+    step = scales.float()
+    step = torch.where(step > 0, step, 1.0)
+    zeros = torch.full_like(step, 8.0) if symmetric else torch.round(-lo / step).clamp(0, 15)
+    q = torch.clamp(torch.round(w / step[..., None]) + zeros[..., None], 0, 15).to(torch.uint8)
+    q = torch.nn.functional.pad(q.view(n, -1)[:, :k], (0, k % 2))
+    return q[:, 0::2] | (q[:, 1::2] << 4), scales, None if symmetric else zeros.to(torch.uint8)
