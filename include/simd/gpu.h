@@ -382,6 +382,28 @@ vs_status vs_gated_recurrence_step(int dtype, const void *x, int64_t x_batch, co
 vs_status vs_matvec_int4(int dtype, const void *x, int64_t ldx, const uint8_t *qweight,
                          int64_t ldq, const void *scales, const uint8_t *zeros, int64_t group,
                          int64_t m, int64_t n, int64_t k, void *y, vs_stream_t stream);
+/// Gated linear layer (dtype VS_F16 or VS_BF16, fp32 sums):
+///   h = act(x w_gate^T) * (x w_up^T)
+/// x [m][k], w_gate and w_up [f][k] with row strides ldx, ld_gate, ld_up in
+/// elements; h [m][f] contiguous.  pre: NULL, or fp32 [m][f][2], the pairs
+/// (x w_gate^T, x w_up^T) that the backward pass reads.  workspace: device
+/// memory of vs_gated_linear_workspace(m, f, k) bytes, or NULL for the library's
+/// pool; it is used where rows are not 16-byte aligned.
+typedef enum { VS_ACT_SILU = 0, VS_ACT_GELU = 1, VS_ACT_RELU = 2, VS_ACT_SIGMOID = 3 } vs_activation;
+vs_status vs_gated_linear(int dtype, int act, const void *x, int64_t ldx, const void *w_gate,
+                          int64_t ld_gate, const void *w_up, int64_t ld_up, int64_t m, int64_t f,
+                          int64_t k, void *h, float *pre, void *workspace, size_t workspace_bytes,
+                          vs_stream_t stream);
+size_t vs_gated_linear_workspace(int64_t m, int64_t f, int64_t k);
+/// Gradients of vs_gated_linear from dh [m][f] (row stride ld_dh) and pre:
+/// dx [m][k] and dw [2 f][k] (w_gate's rows, then w_up's); NULL skips one.
+vs_status vs_gated_linear_backward(int dtype, int act, const void *x, int64_t ldx,
+                                   const void *w_gate, int64_t ld_gate, const void *w_up,
+                                   int64_t ld_up, const float *pre, const void *dh, int64_t ld_dh,
+                                   int64_t m, int64_t f, int64_t k, void *dx, void *dw,
+                                   void *workspace, size_t workspace_bytes, vs_stream_t stream);
+size_t vs_gated_linear_backward_workspace(int64_t m, int64_t f, int64_t k, int want_dx,
+                                          int want_dw);
 
 SIMD_API_END
 

@@ -1,0 +1,313 @@
+"""Gated linear layer (ops.gated_linear) against the definition in float64, and a block of all sequence operators.
+
+Tolerances.  u = 2^-24, e = eps / 2 of the 16-bit type.  A product of k terms is added in float32: any order rounds partial
+sums of at most S = sum |a| |b|, so it is off by at most k u S (worst case; the exact products of 16-bit numbers fit
+float32).  The activation adds 8 u of itself and passes its argument's error on with a slope of at most 1.13 (gelu; silu
+1.1); h is rounded once.  In the backward pass dg = dh u act'(g) is off by its inputs' errors (slopes of act' are at most
+1, 1.6 for gelu is generous), 16 u of itself for the functions, and one rounding e to the 16-bit type, and so is du; the
+products then carry these errors times the other operand, their own k u S, and one rounding."""
+import pytest
+import torch
+
+from veles.simd_amd import _lib, ops
+from veles.simd_amd.utils import CapturedCall
+
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+U = 2.0 ** -24
+ACTS = ["silu", "gelu", "relu", "sigmoid"]
+
+
+def _inputs(m, k, f, dtype, dev, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(m, k, generator=g).to(dtype).to(dev)
+    wg, wu = ((torch.randn(f, k, generator=g) * max(k, 1) ** -0.5).to(dtype).to(dev) for _ in range(2))
+    dh = torch.randn(m, f, generator=g).to(dtype).to(dev)
+    return x, wg, wu, dh
+
+
+def _act(name, g):
+    """act(g) and its slope."""
+    s = 1.0 / (1.0 + torch.exp(-g))
+    if name == "silu":
+        return g * s, s + g * s * (1 - s)
+    if name == "gelu":
+        phi = 0.5 * torch.special.erfc(-g * 0.5 ** 0.5)
+        return g * phi, phi + g * torch.exp(-0.5 * g * g) / (2 * torch.pi) ** 0.5
+    if name == "relu":
+        return g.clamp(min=0), (g > 0).double()
+    return s, s * (1 - s)
+
+
+def _oracle(x, wg, wu, dh, act):
+    e = torch.finfo(x.dtype).eps / 2
+    tiny = torch.finfo(x.dtype).smallest_normal
+    x, wg, wu, dh = (v.detach().double().cpu() for v in (x, wg, wu, dh))
+    m, k = x.shape
+    f = wg.shape[0]
+    g, u = x @ wg.t(), x @ wu.t()
+    eg, eu = k * U * (x.abs() @ wg.abs().t()), k * U * (x.abs() @ wu.abs().t())
+    a, slope = _act(act, g)
+    ea = 1.2 * eg + 8 * U * a.abs()
+    eslope = (1.6 * eg if act != "relu" else (g.abs() <= eg).double()) + 16 * U
+    h, eh = a * u, ea * u.abs() + a.abs() * eu
+    dg, du = dh * u * slope, dh * a
+    edg = dh.abs() * (eu * slope.abs() + u.abs() * eslope) + 4 * U * dg.abs()
+    edu = dh.abs() * ea + 4 * U * du.abs()
+    edg, edu = edg + e * (dg.abs() + edg) + tiny, edu + e * (du.abs() + edu) + tiny
+    d, ed, w = torch.cat([dg, du], 1), torch.cat([edg, edu], 1), torch.cat([wg, wu])
+    dx, edx = d @ w, ed @ w.abs() + 2 * f * U * ((d.abs() + ed) @ w.abs())
+    dw, edw = d.t() @ x, ed.t() @ x.abs() + m * U * ((d.abs() + ed).t() @ x.abs())
+    return dict(h=(h, eh), dx=(dx, edx), dw_gate=(dw[:f], edw[:f]), dw_up=(dw[f:], edw[f:]))
+
+
+def _close(name, got, want):
+    ref, bound = want
+    got_d = got.detach().double().cpu().reshape(ref.shape)
+    tol = bound + torch.finfo(got.dtype).eps / 2 * (ref.abs() + bound) + torch.finfo(got.dtype).smallest_normal
+    bad = ~((got_d - ref).abs() <= tol)
+    assert not bad.any(), (name, int(bad.sum()), ((got_d - ref).abs() / tol).max().item())
+
+
+def _all(x, wg, wu, dh, act, want=None):
+    leaves = [v.detach().requires_grad_() for v in (x, wg, wu)]
+    h = ops.gated_linear(*leaves, act)
+    grads = torch.autograd.grad(h, leaves, dh)
+    want = want or _oracle(x.reshape(-1, x.shape[-1]), wg, wu, dh.reshape(-1, dh.shape[-1]), act)
+    for name, got in zip(("h", "dx", "dw_gate", "dw_up"), (h, *grads)):
+        assert got.dtype == x.dtype
+        _close(name, got, want[name])
+    with torch.no_grad():
+        assert torch.equal(ops.gated_linear(x, wg, wu, act), h)
+    return (h.detach(), *grads)
+
+
+SHAPES = [(1, 1, 1), (1, 64, 16), (3, 70, 33), (16, 128, 40), (17, 33, 100), (40, 200, 31), (64, 129, 65), (65, 64, 64),
+          (130, 72, 200), (129, 75, 131), (300, 136, 260)]
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_forward_and_gradients(dev, dtype, shape):
+    for act in ("silu", "gelu"):
+        _all(*_inputs(*shape, dtype, dev, seed=sum(shape)), act)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("m", [5, 100])
+def test_activations(dev, act, m):
+    x, wg, wu, dh = _inputs(m, 64, 48, torch.bfloat16, dev, seed=2)
+    _all(x * 4, wg, wu, dh, act)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(4096, 200, 2100), (4100, 1000, 2056), (2100, 2048, 5000), (70, 4096, 3000),
+                                   (60, 1027, 4099)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_large_tiles(shape, dtype):
+    """Shapes whose forward or backward products take the large tiles, ragged in every dimension."""
+    _all(*_inputs(*shape, dtype, "cuda", seed=3), "silu")
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("m", [6, 90])
+def test_shapes_strides_and_alignment(dev, m):
+    """Leading dimensions, odd offsets, transposed storage and broadcast rows give the values of a copy."""
+    x, wg, wu, dh = _inputs(m, 64, 40, torch.bfloat16, dev, seed=4)
+    ref = _all(x, wg, wu, dh, "silu")
+    three = _all(x.view(2, m // 2, 64), wg, wu, dh.view(2, m // 2, 40), "silu")
+    for a, b in zip(three, ref):
+        assert torch.equal(a.reshape(b.shape), b)
+
+    def shifted(v, off):
+        wide = torch.full((v.shape[0], v.shape[1] + 9), float("nan"), dtype=v.dtype, device=dev)
+        wide[:, off:off + v.shape[1]] = v
+        return wide[:, off:off + v.shape[1]]
+    for change in (lambda v: shifted(v, 1), lambda v: shifted(v, 8), lambda v: v.t().contiguous().t()):
+        _all(change(x), change(wg), change(wu), change(dh), "silu")
+    one = x[:1].expand(m, 64)
+    _all(one, wg, wu, dh[:, :1].expand(m, 40), "silu")
+    _all(x, wg[:1].expand(40, 64), wu, dh, "silu")
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_shared_weight_and_partial_gradients(dev):
+    """One tensor as both weights gets the sum of both gradients; gradients that nobody asks for are not made."""
+    x, w, _, dh = _inputs(33, 64, 24, torch.bfloat16, dev, seed=5)
+    want = _oracle(x, w, w, dh, "silu")
+    leaf = w.detach().requires_grad_()
+    h = ops.gated_linear(x, leaf, leaf)
+    got, = torch.autograd.grad(h, leaf, dh)
+    e = torch.finfo(w.dtype).eps
+    both = (want["dw_gate"][0] + want["dw_up"][0],
+            want["dw_gate"][1] + want["dw_up"][1] + e * (want["dw_gate"][0].abs() + want["dw_up"][0].abs()))
+    _close("dw", got, both)
+    for k in range(3):
+        args = [x, w, w.clone()]
+        args[k] = args[k].detach().requires_grad_()
+        got, = torch.autograd.grad(ops.gated_linear(*args), args[k], dh)
+        _close("part", got, want[("dx", "dw_gate", "dw_up")[k]])
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_formula_gradient_agrees_with_differences(dev):
+    """Central differences of the float64 definition against the gradients (which carry 16-bit roundings)."""
+    x, wg, wu, dh = _inputs(3, 5, 4, torch.float16, dev, seed=6)
+    base = [v.double().cpu() for v in (x, wg, wu)]
+    d = dh.double().cpu()
+    for act in ("silu", "gelu", "sigmoid"):
+        def loss(xv, gv, uv):
+            return (_act(act, xv @ gv.t())[0] * (xv @ uv.t()) * d).sum()
+        want = _oracle(x, wg, wu, dh, act)
+        leaves = [v.detach().requires_grad_() for v in (x, wg, wu)]
+        grads = torch.autograd.grad(ops.gated_linear(*leaves, act), leaves, dh)
+        for k, name in enumerate(("dx", "dw_gate", "dw_up")):
+            diff = torch.zeros_like(base[k])
+            for at in range(base[k].numel()):
+                vals = []
+                for sign in (1, -1):
+                    moved = [v.clone() for v in base]
+                    moved[k].view(-1)[at] += sign * 1e-5
+                    vals.append(loss(*moved))
+                diff.view(-1)[at] = (vals[0] - vals[1]) / 2e-5
+            _close(name, grads[k], (diff, want[name][1] + 1e-7))
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("m,k,f", [(0, 8, 8), (3, 0, 8), (3, 8, 0), (100, 0, 8), (100, 8, 0)])
+def test_empty(dev, m, k, f):
+    x, wg, wu, dh = _inputs(m, k, f, torch.bfloat16, dev)
+    leaves = [v.detach().requires_grad_() for v in (x, wg, wu)]
+    h = ops.gated_linear(*leaves)
+    assert h.shape == (m, f) and (h == 0).all()
+    for g, leaf in zip(torch.autograd.grad(h, leaves, dh), leaves):
+        assert g.shape == leaf.shape and (g == 0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [4, 200])
+def test_not_finite_rows_stay_in_their_rows(m):
+    x, wg, wu, dh = _inputs(m, 72, 64, torch.bfloat16, "cuda", seed=7)
+    ref = ops.gated_linear(x, wg, wu)
+    x2 = x.clone()
+    x2[1] = float("nan")
+    x2[2, 5] = float("inf")
+    got = ops.gated_linear(x2, wg, wu)
+    keep = torch.ones(m, dtype=torch.bool)
+    keep[1:3] = False
+    assert torch.equal(got[keep], ref[keep]) and torch.isnan(got[1]).all() and not torch.isfinite(got[2]).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,k", [(8, 96), (200, 96), (200, 75)])
+def test_streams_captures_and_repeats(m, k):
+    args = _inputs(m, k, 80, torch.bfloat16, "cuda", seed=8)
+
+    def train(x, wg, wu, dh):
+        leaves = [v.detach().requires_grad_() for v in (x, wg, wu)]
+        h = ops.gated_linear(*leaves)
+        return (h.detach(), *torch.autograd.grad(h, leaves, dh))
+    ref = train(*args)
+    caps = [CapturedCall(train, *args) for _ in range(2)]
+    for seed in range(3):
+        other = _inputs(m, k, 80, torch.bfloat16, "cuda", seed=30 + seed)
+        got = [[v.clone() for v in c(*other)] for c in caps]
+        want = train(*other)
+        for a, b, c in zip(*got, want):
+            assert torch.equal(a, c) and torch.equal(b, c)
+        torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        a = train(*args)
+    b = train(*args)
+    torch.cuda.current_stream().wait_stream(side)
+    for u, v, w in zip(a, b, ref):
+        assert torch.equal(u, w) and torch.equal(v, w)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_refusals(dev):
+    x, wg, wu, dh = _inputs(3, 16, 8, torch.bfloat16, dev)
+    bad = [(ValueError, (x, wg, wu, "tanh")), (TypeError, (x.float(), wg.float(), wu.float())), (TypeError, (x, wg, wu.half())),
+           (ValueError, (x[:, :8], wg, wu)), (ValueError, (x, wg[:4], wu)), (ValueError, (x, wg[0], wu[0]))]
+    for err, args in bad:
+        with pytest.raises(err):
+            ops.gated_linear(*args)
+    if dev == "cuda":
+        with pytest.raises(ValueError, match="is on"):
+            ops.gated_linear(x, wg, wu.cpu())
+    xr = x.clone().requires_grad_()
+    g, = torch.autograd.grad(ops.gated_linear(xr, wg, wu).sum(), xr, create_graph=True)
+    if g.requires_grad:
+        with pytest.raises(NotImplementedError, match="second"):
+            g.float().sum().backward()
+
+
+def test_native_refusals():
+    lib = _lib.lib()
+    p = torch.zeros(8).data_ptr()
+
+    def call(dtype=5, act=0, x=p, ldx=64, ldw=64, m=1, f=1, k=64, ws=None, size=0):
+        return lib.vs_gated_linear(dtype, act, x, ldx, p, ldw, p, ldw, m, f, k, p, None, ws, size, None)
+    for kw in (dict(dtype=0), dict(act=4), dict(act=-1), dict(m=-1), dict(f=-1), dict(k=-1), dict(x=None),
+               dict(m=2, ldx=63), dict(f=2, ldw=63), dict(m=1 << 31), dict(f=1 << 21), dict(k=1 << 21),
+               dict(ldx=1 << 21)):
+        assert call(**kw) == 1 and b"gated_linear" in lib.vs_last_error()
+    assert call(m=100, f=100, k=65, ldx=65, ldw=65, ws=p, size=16) == 1 and b"workspace" in lib.vs_last_error()
+    assert lib.vs_gated_linear_backward(5, 0, p, 8, p, 8, p, 8, None, p, 8, 1, 1, 8, p, p, None, 0, None) == 1
+    assert lib.vs_gated_linear_workspace(-1, 1, 1) == 0
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_opcheck(dev):
+    x, wg, wu, _ = _inputs(5, 24, 16, torch.bfloat16, dev)
+    for args in ((x, wg, wu, "gelu", False), (x.clone().requires_grad_(), wg.clone().requires_grad_(), wu, "silu", True)):
+        torch.library.opcheck(torch.ops.veles.gated_linear.default, args)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_block_trains_prefills_and_generates(dev):
+    """The operators as a model uses them: value and gate projections, the recurrence, a gated feed-forward; its gradients
+    against float64, then a ragged prefill followed by single tokens with 4-bit output weights, which has to agree with the
+    same positions of a whole run (both paths round to bf16 at the same places: 4 roundings of 2^-8 of the largest value)."""
+    b, t, d, f = 3, 20, 64, 96
+    gen = torch.Generator().manual_seed(12)
+    x = torch.randn(b, t, d, generator=gen).bfloat16().to(dev)
+    ws = [(torch.randn(*s, generator=gen) * s[1] ** -0.5).bfloat16().to(dev)
+          for s in ((d, d), (d, d), (f, d), (f, d), (d, f))]
+    wv, wa, wg, wu, wo = ws
+    down = ops.quantize_int4(wo, 32)
+
+    def mix(x, wv, wa):
+        return ops.gemm_bf16(x.reshape(-1, d), wv, False, True).bfloat16().view(x.shape), \
+            (ops.gemm_bf16(x.reshape(-1, d), wa, False, True) + 1.5).bfloat16().view(x.shape)
+    v, a = mix(x, wv, wa)
+    leaves = [q.detach().requires_grad_() for q in (v, a, wg, wu)]
+    y, final = ops.gated_recurrence(leaves[0], leaves[1])
+    h = ops.gated_linear(y, leaves[2], leaves[3])
+    up = torch.randn(b, t, f, generator=gen).bfloat16().to(dev)
+    grads = torch.autograd.grad(h, leaves, up)
+    ref = [q.detach().double().cpu().requires_grad_() for q in leaves]
+    hr, rows = torch.zeros(b, d, dtype=torch.float64), []
+    for s in range(t):
+        i = torch.sigmoid(-ref[1][:, s])
+        hr = hr + i * (ref[0][:, s] - hr)
+        rows.append(hr)
+    yr = torch.stack(rows, 1)
+    gr, ur = yr @ ref[2].t(), yr @ ref[3].t()
+    want = torch.autograd.grad(gr * torch.sigmoid(gr) * ur, ref, up.double().cpu())
+    # y, dg / du, dy and the result are each rounded to bf16 on the way: 4 half steps of the norm
+    for got, w in zip(grads, want):
+        assert (got.double().cpu() - w).norm() <= 4 * 2.0 ** -8 * w.norm()
+
+    with torch.no_grad():
+        whole = ops.matvec_int4(ops.gated_linear(ops.gated_recurrence(v, a)[0], wg, wu), *down, 32)
+        lengths = torch.tensor([12, 5, 1], device=dev)
+        _, state = ops.gated_recurrence(v[:, :12], a[:, :12], None, lengths)
+        for s in range(6):
+            at = (torch.arange(b, device=dev), lengths + s)
+            tok = ops.gated_recurrence_step(v[at], a[at], state)
+            out = ops.matvec_int4(ops.gated_linear(tok, wg, wu), *down, 32)
+            assert (out.float() - whole[at].float()).abs().max() <= 4 * 2.0 ** -8 * whole.float().abs().max()

@@ -11,8 +11,8 @@ from .elementwise import (add, affine, binary, complex_conjugate,  # noqa: F401
                           complex_multiply, convert, cos, exp, log, math,
                           minmax, mul, normalize2d, pow, saxpy, sin, sincos, sqrt, sub,
                           sum_all)
-from .sequence import (gated_recurrence, gated_recurrence_step, matvec_int4,  # noqa: F401
-                       quantize_int4)
+from .sequence import (gated_linear, gated_recurrence, gated_recurrence_step,  # noqa: F401
+                       matvec_int4, quantize_int4)
 from .signal import (Conv1dPlan, conv1d, conv1d_algorithm, correlate, detect_peaks,  # noqa: F401
                      detect_peaks_batched, dwt, fft, irfft, rfft, swt, swt_level, wavedec,
                      wavelet_filter)
@@ -23,5 +23,5 @@ __all__ = [
     "sin", "cos", "log", "exp", "sum_all", "minmax", "normalize2d", "conv1d",
     "correlate", "conv1d_algorithm", "Conv1dPlan", "fft", "rfft", "irfft", "dwt", "swt",
     "wavedec", "wavelet_filter", "detect_peaks", "detect_peaks_batched", "swt_level",
-    "gated_recurrence", "gated_recurrence_step", "matvec_int4", "quantize_int4",
+    "gated_recurrence", "gated_recurrence_step", "matvec_int4", "quantize_int4", "gated_linear",
 ]

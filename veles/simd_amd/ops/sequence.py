@@ -1,7 +1,7 @@
-"""Operators of sequence models: the gated linear recurrence (forward, gradient, single-token step).
+"""Operators of sequence models: the gated linear recurrence (a conv1d whose filter changes from sample to
+sample), the gated linear layer, and products of few rows with 4-bit weights.
 
-The counterparts of conv1d for filters whose coefficient changes from sample to sample.  GPU
-tensors run the native HIP kernels; CPU tensors run the definition step by step in float64.
+GPU tensors run the native HIP kernels; CPU tensors run the definitions in float64.  Arguments are checked on both.
 """
 from __future__ import annotations
 
@@ -304,14 +304,13 @@ def _matvec_impl(x, qweight, scales, zeros, group_size):
         z = 8.0 if zeros is None else zeros.double()[:, at]
         return (x.double() @ ((q - z) * scales.double()[:, at]).t()).to(x.dtype)
     require_gpu_tensor(x, name)
-    rows = x if x.dim() == 2 else x.reshape(-1, k) if k else x.new_empty((x[..., 0:0].numel(), 0))
-    rows = _rows_last(rows)
+    rows = _as_rows(x)
     y = torch.empty((*x.shape[:-1], n), dtype=x.dtype, device=x.device)
     scales = scales.contiguous()
     zeros = None if zeros is None else zeros.contiguous()
     with on_device(x):
         _lib.call("vs_matvec_int4", DTYPES[x.dtype], ptr(rows), rows.stride(0), ptr(qweight), qweight.stride(0),
-                  ptr(scales), _opt(zeros), group_size, y.numel() // max(n, 1), n, k, ptr(y), raw_stream(x))
+                  ptr(scales), _opt(zeros), group_size, rows.shape[0], n, k, ptr(y), raw_stream(x))
     return y
 
 
@@ -376,3 +375,172 @@ def quantize_int4(weight: torch.Tensor, group_size: int = 128, symmetric: bool =
     q = torch.clamp(torch.round(w / step[..., None]) + zeros[..., None], 0, 15).to(torch.uint8)
     q = torch.nn.functional.pad(q.view(n, -1)[:, :k], (0, k % 2))
     return q[:, 0::2] | (q[:, 1::2] << 4), scales, None if symmetric else zeros.to(torch.uint8)
+
+
+# ---------------------------------------------------- gated linear layer
+ACTIVATIONS = {"silu": 0, "gelu": 1, "relu": 2, "sigmoid": 3}
+
+
+def _check_gated(name, x, w_gate, w_up, activation):
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"{name}: activation {activation!r}; one of {sorted(ACTIVATIONS)} expected")
+    if x.dtype not in (torch.bfloat16, torch.float16):
+        raise TypeError(f"{name}: x is {x.dtype}; float16 or bfloat16 expected")
+    if w_gate.dtype != x.dtype or w_up.dtype != x.dtype:
+        raise TypeError(f"{name}: weights are {w_gate.dtype} and {w_up.dtype}, x {x.dtype}")
+    if x.dim() < 1 or w_gate.dim() != 2 or w_up.shape != w_gate.shape or w_gate.shape[1] != x.shape[-1]:
+        raise ValueError(f"{name}: x [..., k] and two weights [features, k] expected; got {tuple(x.shape)}, "
+                         f"{tuple(w_gate.shape)}, {tuple(w_up.shape)}")
+    _same_device(name, x, w_gate=w_gate, w_up=w_up)
+
+
+def _as_rows(x: torch.Tensor) -> torch.Tensor:
+    """x [..., k] as [rows, k] with neighbouring k (a copy only where the layout asks for one)."""
+    if x.dim() != 2:
+        rows = 1
+        for n in x.shape[:-1]:
+            rows *= n
+        x = x.reshape(rows, x.shape[-1])
+    return _rows_last(x)
+
+
+def _weight_rows(w: torch.Tensor) -> torch.Tensor:
+    w = _rows_last(w)
+    return w if w.shape[0] <= 1 or w.stride(0) >= w.shape[1] else w.contiguous()
+
+
+def _act_cpu(kind, g):
+    if kind == "silu":
+        return g * torch.sigmoid(g)
+    if kind == "gelu":
+        return 0.5 * g * (1.0 + torch.erf(g * 0.5 ** 0.5))
+    return torch.relu(g) if kind == "relu" else torch.sigmoid(g)
+
+
+def _slope_cpu(kind, g):
+    s = torch.sigmoid(g)
+    if kind == "silu":
+        return s * (1.0 + g * (1.0 - s))
+    if kind == "gelu":
+        return 0.5 * (1.0 + torch.erf(g * 0.5 ** 0.5)) + g * torch.exp(-0.5 * g * g) * (0.5 / torch.pi) ** 0.5
+    return (g > 0).to(g.dtype) if kind == "relu" else s * (1.0 - s)
+
+
+def _gated_impl(x, w_gate, w_up, activation, save):
+    name = "veles::gated_linear"
+    _check_gated(name, x, w_gate, w_up, activation)
+    f, k = w_gate.shape
+    rows = _as_rows(x)
+    m = rows.shape[0]
+    if not x.is_cuda:
+        g, u = rows.double() @ w_gate.double().t(), rows.double() @ w_up.double().t()
+        h = (_act_cpu(activation, g) * u).to(x.dtype).view(*x.shape[:-1], f)
+        return h, (torch.stack([g, u], -1).float() if save else x.new_empty(0, dtype=torch.float32))
+    require_gpu_tensor(x, name)
+    w_gate, w_up = _weight_rows(w_gate), _weight_rows(w_up)
+    h = torch.empty((*x.shape[:-1], f), dtype=x.dtype, device=x.device)
+    pre = torch.empty((m, f, 2) if save else (0,), dtype=torch.float32, device=x.device)
+    size = int(_lib.lib().vs_gated_linear_workspace(m, f, k))
+    ws = torch.empty(size, dtype=torch.uint8, device=x.device) if size and not _aligned(rows, w_gate, w_up) else None
+    with on_device(x):
+        _lib.call("vs_gated_linear", DTYPES[x.dtype], ACTIVATIONS[activation], ptr(rows), rows.stride(0), ptr(w_gate),
+                  w_gate.stride(0), ptr(w_up), w_up.stride(0), m, f, k, ptr(h), ptr(pre) if save else None, _opt(ws),
+                  0 if ws is None else size, raw_stream(x))
+    return h, pre
+
+
+def _aligned(*tensors) -> bool:
+    """Rows of whole 16-byte pieces: the kernel reads them where they are."""
+    return all(t.shape[-1] % 8 == 0 and t.stride(0) % 8 == 0 and t.data_ptr() % 16 == 0 for t in tensors)
+
+
+def _gated_backward_impl(x, w_gate, w_up, pre, dh, activation, want_dx, want_dw):
+    name = "veles::gated_linear_backward"
+    _check_gated(name, x, w_gate, w_up, activation)
+    f, k = w_gate.shape
+    rows, dhr = _as_rows(x), _as_rows(dh)
+    m = rows.shape[0]
+    if dh.dtype != x.dtype or tuple(dh.shape) != (*x.shape[:-1], f):
+        raise ValueError(f"{name}: dh is {dh.dtype} {tuple(dh.shape)}, {x.dtype} {(*x.shape[:-1], f)} expected")
+    if pre.dtype != torch.float32 or tuple(pre.shape) != (m, f, 2):
+        raise ValueError(f"{name}: pre-activations {pre.dtype} {tuple(pre.shape)}, float32 {(m, f, 2)} expected")
+    _same_device(name, x, pre=pre, dh=dh)
+    if not x.is_cuda:
+        g, u, d = pre[..., 0].double(), pre[..., 1].double(), dhr.double()
+        dg, du = d * u * _slope_cpu(activation, g), d * _act_cpu(activation, g)
+        dx = (dg @ w_gate.double() + du @ w_up.double()).to(x.dtype).view(x.shape) if want_dx else x.new_empty(0)
+        dw = torch.cat([dg.t() @ rows.double(), du.t() @ rows.double()]).to(x.dtype) if want_dw else x.new_empty(0)
+        return dx, dw
+    require_gpu_tensor(x, name)
+    w_gate, w_up, pre = _weight_rows(w_gate), _weight_rows(w_up), pre.contiguous()
+    dx = torch.empty(x.shape if want_dx else (0,), dtype=x.dtype, device=x.device)
+    dw = torch.empty((2 * f, k) if want_dw else (0,), dtype=x.dtype, device=x.device)
+    size = int(_lib.lib().vs_gated_linear_backward_workspace(m, f, k, int(want_dx), int(want_dw)))
+    ws = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
+    with on_device(x):
+        _lib.call("vs_gated_linear_backward", DTYPES[x.dtype], ACTIVATIONS[activation], ptr(rows), rows.stride(0),
+                  ptr(w_gate), w_gate.stride(0), ptr(w_up), w_up.stride(0), ptr(pre), ptr(dhr), dhr.stride(0), m, f, k,
+                  ptr(dx) if want_dx else None, ptr(dw) if want_dw else None, _opt(ws), size, raw_stream(x))
+    return dx, dw
+
+
+def _gated_fake(x, w_gate, w_up, activation, save):
+    _check_gated("veles::gated_linear", x, w_gate, w_up, activation)
+    m, f = 1, w_gate.shape[0]
+    for n in x.shape[:-1]:
+        m = m * n
+    return x.new_empty((*x.shape[:-1], f)), x.new_empty((m, f, 2) if save else (0,), dtype=torch.float32)
+
+
+def _gated_setup(ctx, inputs, output):
+    x, w_gate, w_up, activation, save = inputs
+    if not save:
+        raise RuntimeError("veles::gated_linear: gradients need the pre-activations (save=True)")
+    ctx.set_materialize_grads(False)
+    ctx.mark_non_differentiable(output[1])
+    ctx.save_for_backward(x, w_gate, w_up, output[1])
+    ctx.activation = activation
+
+
+def _gated_grad(ctx, dh, _):
+    if dh is None:
+        return None, None, None, None, None
+    x, w_gate, w_up, pre = ctx.saved_tensors
+    need = ctx.needs_input_grad
+    dx, dw = torch.ops.veles.gated_linear_backward(x, w_gate, w_up, pre, dh, ctx.activation, need[0],
+                                                   need[1] or need[2])
+    f = w_gate.shape[0]
+    return dx if need[0] else None, dw[:f] if need[1] else None, dw[f:] if need[2] else None, None, None
+
+
+torch.library.define("veles::gated_linear",
+                     "(Tensor x, Tensor w_gate, Tensor w_up, str activation, bool save) -> (Tensor, Tensor)")
+torch.library.impl("veles::gated_linear", "default", _gated_impl)
+torch.library.register_fake("veles::gated_linear", _gated_fake)
+torch.library.register_autograd("veles::gated_linear", _gated_grad, setup_context=_gated_setup)
+torch.library.define("veles::gated_linear_backward",
+                     "(Tensor x, Tensor w_gate, Tensor w_up, Tensor pre, Tensor dh, str activation, bool want_dx, "
+                     "bool want_dw) -> (Tensor, Tensor)")
+torch.library.impl("veles::gated_linear_backward", "default", _gated_backward_impl)
+torch.library.register_fake(
+    "veles::gated_linear_backward",
+    lambda x, w_gate, w_up, pre, dh, activation, want_dx, want_dw: (
+        x.new_empty(x.shape if want_dx else (0,)),
+        x.new_empty((2 * w_gate.shape[0], w_gate.shape[1]) if want_dw else (0,))))
+_no_second_derivative("veles::gated_linear_backward")
+
+
+def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor,
+                 activation: str = "silu") -> torch.Tensor:
+    """act(x @ w_gate.T) * (x @ w_up.T): both products, the activation and the product of the two in one
+    kernel, the first half of a gated feed-forward block.
+
+    x: [..., k], weights [features, k], all float16 or all bfloat16; activation: silu, gelu (by the error
+    function), relu or sigmoid.  Sums, activation and product are float32 and rounded once.  Differentiable
+    in x and the weights; the float32 pairs (x @ w_gate.T, x @ w_up.T), 8 bytes per output, are kept for the
+    backward pass, and the gradients of the two products are rounded to x's type before they are
+    multiplied.  Up to 64 rows (generation) stream the weights once at memory speed."""
+    if plain_call(x, w_gate, w_up):
+        return _gated_impl(x, w_gate, w_up, activation, False)[0]
+    save = torch.is_grad_enabled() and (x.requires_grad or w_gate.requires_grad or w_up.requires_grad)
+    return torch.ops.veles.gated_linear(x, w_gate, w_up, activation, save)[0]
