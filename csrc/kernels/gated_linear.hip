@@ -41,10 +41,11 @@ namespace {
 typedef float floatx4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) void lds_void;
 
 template <class N>
-__device__ __forceinline__ floatx4 mma(const uint4 &a, const uint4 &b, floatx4 c) {
+__device__ __forceinline__ floatx4 mma(const u32x4 &a, const u32x4 &b, floatx4 c) {
   if constexpr (std::is_same_v<N, num::BF16>)
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
                                                    __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
@@ -93,19 +94,21 @@ struct Args {
   int act;
 };
 
-// BM x BN tile of products, WM x WN waves.  GATED: the BN product columns are BN / 2 outputs.
-template <int BM_, int BN_, int WM_, int WN_, bool GATED_>
+// A tile of 2 (rows) x 4 (columns) waves, each with 2 x 2 quadrants of 16 XH x 16 YH products.
+// GATED: the column quadrants are Wg and Wu of the same outputs.
+template <int XH_, int YH_, bool GATED_>
 struct Cfg {
-  static constexpr int BM = BM_, BN = BN_, BK = 64, WM = WM_, WN = WN_;
+  static constexpr int XH = XH_, YH = YH_, BK = 64;
   static constexpr bool GATED = GATED_;
-  static constexpr int BO = GATED ? BN / 2 : BN;  // output columns
-  static constexpr int kWaves = WM * WN, kThreads = 64 * kWaves;
-  static constexpr int XM = BM / WM / 16, XN = BN / WN / 16;
-  static constexpr int RB = 2 * BK;               // bytes of an image row
-  static constexpr int kImgA = BM * RB, kImgB = BN * RB, kStage = kImgA + kImgB;
-  static constexpr int PA = kImgA / 1024 / kWaves, PB = kImgB / 1024 / kWaves;
-  static constexpr int kLds = 2 * kStage;
-  static_assert(BN / WN == 64, "a wave owns 64 product columns");
+  static constexpr int BM = 64 * XH, BN = 128 * YH;    // products
+  static constexpr int BO = GATED ? BN / 2 : BN;       // output columns
+  static constexpr int kThreads = 512;
+  static constexpr int RB = 2 * BK;                    // bytes of an image row
+  static constexpr int kHalfA = BM / 2 * RB, kHalfB = BN / 2 * RB;
+  static constexpr int kBuf = 2 * (kHalfA + kHalfB);   // A0 A1 B0 B1
+  static constexpr int PA = kHalfA / 8192, PB = kHalfB / 8192;  // 1 KiB pieces per wave
+  static constexpr int kLds = 2 * kBuf;
+  static_assert(kHalfA % 8192 == 0 && kHalfB % 8192 == 0, "whole pieces for every wave");
 };
 
 constexpr uint32_t kOut = 0x80000000u;  // past every descriptor's range: reads zeros
@@ -131,141 +134,266 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_of(const uint16_t *p, int
       0x00020000);
 }
 
+// Fragment reads are inline asm: the compiler would wait for every DMA in flight before a read of
+// LDS that it sees.  `settle` is the wait, and the registers pass through it, so no product can
+// move above it.
+template <int OFF>
+__device__ __forceinline__ void read_frag(u32x4 &f, uint32_t at) {
+  asm volatile("ds_read_b128 %0, %1 offset:%2" : "=v"(f) : "v"(at), "i"(OFF) : "memory");
+}
+template <int XH>
+__device__ __forceinline__ void settle(u32x4 (&f)[XH][2]) {
+  if constexpr (XH == 4)
+    asm volatile("s_waitcnt lgkmcnt(0)"
+                 : "+v"(f[0][0]), "+v"(f[1][0]), "+v"(f[2][0]), "+v"(f[3][0]), "+v"(f[0][1]),
+                   "+v"(f[1][1]), "+v"(f[2][1]), "+v"(f[3][1])::"memory");
+  else if constexpr (XH == 2)
+    asm volatile("s_waitcnt lgkmcnt(0)"
+                 : "+v"(f[0][0]), "+v"(f[1][0]), "+v"(f[0][1]), "+v"(f[1][1])::"memory");
+  else
+    asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(f[0][0]), "+v"(f[0][1])::"memory");
+}
+template <int N>
+__device__ __forceinline__ void wait_vmcnt() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void meet() {
+  __builtin_amdgcn_sched_barrier(0);
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+// The k loop.  A k tile of 64 is taken in four phases, one quadrant of every wave's products
+// each.  With first / second the column halves 0 / 1 in even tiles and 1 / 0 in odd ones:
+//
+//   phase  reads into registers     multiplies          starts the DMA of (two tiles ahead)
+//   0      A0                       A0 x first          first
+//   1      second                   A0 x second         A0
+//   2      A1                       A1 x second         second
+//   3      first of the next tile   A1 x first          A1
+//
+// (the next tile's first half is this tile's second index, whose registers are free by then).
+// A phase is: start the reads and the DMA, wait for the reads, barrier, products, barrier.  Waves
+// 4-7 are one barrier behind waves 0-3, so of the two waves on a SIMD one multiplies while the
+// other reads and issues.  The halves h_0, h_1, ... in this order are read in phase j - 1 and
+// started in phase j - 8, right after the phase that read what they overwrite: a wave's reads
+// have arrived before its first barrier of a phase, and no wave is further than that barrier
+// behind a wave that starts the next phase.  Before that barrier a wave also waits until its
+// pieces of the half that the next phase reads have landed; six halves stay in flight.  Tiles
+// past the end of k are started out of range (zeros), so the counts hold to the end.
 template <class N, class C>
-__global__ __launch_bounds__(C::kThreads) void tile_kernel(Args p) {
+__global__ __launch_bounds__(512) void tile_kernel(Args p) {
   extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
-  constexpr int XM = C::XM, XN = C::XN;
+  constexpr int XH = C::XH, YH = C::YH;
   const unsigned tiles_m = (p.m + C::BM - 1) / C::BM, tiles_n = (p.n + C::BO - 1) / C::BO;
   unsigned tm, tn;
   dev::grouped_tile(dev::xcd_remap(blockIdx.x, tiles_m * tiles_n), tiles_m, tiles_n, tm, tn);
   const int m0 = tm * C::BM, n0 = tn * C::BO;
   const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int wm = wid / C::WN, wn = wid % C::WN;
+  const int wm = wid / 4, wn = wid % 4;
   const int l16 = lane & 15, lq = lane >> 4;
 
   const __amdgpu_buffer_rsrc_t ra = rows_of(p.a, p.lda, m0, p.m, C::BM, p.k);
   const __amdgpu_buffer_rsrc_t rb0 = rows_of(p.b[0], p.ldb[0], n0, p.n, C::BO, p.k);
   const __amdgpu_buffer_rsrc_t rb1 =
       C::GATED ? rows_of(p.b[1], p.ldb[1], n0, p.n, C::BO, p.k) : rb0;
-  // piece i of this wave: image rows 8 (i of the wave's pieces) + lane / 8, chunk lane % 8
-  uint32_t offa[C::PA], offb[C::PB];
-  int ka, kb[C::PB];
-  {
-    const int r8 = lane / 8, pc = lane % 8;
+  // Image row r of A half h is row 32 XH (r / 16 XH) + 16 XH h + r % 16 XH of the tile; of B half
+  // h it is the same with YH and four waves (GATED: row r of operand h).  Piece i of a wave: image rows
+  // 8 (P wid + i) + lane / 8, chunk lane % 8.
+  uint32_t offa[2][C::PA], offb[2][C::PB];
+  int ka[C::PA], kb[C::PB];
 #pragma unroll
-    for (int i = 0; i < C::PA; i++) {
-      const int row = (wid * C::PA + i) * 8 + r8;
-      offa[i] = static_cast<uint32_t>((row * p.lda + 8 * swz(row, pc)) * 2);
-    }
+  for (int i = 0; i < C::PA; i++) {
+    const int r = (wid * C::PA + i) * 8 + lane / 8;
+    ka[i] = 8 * swz(r, lane % 8);
 #pragma unroll
-    for (int i = 0; i < C::PB; i++) {
-      const int row = (wid * C::PB + i) * 8 + r8;  // image row
-      // GATED: 64 image rows are 32 of Wg, then the same 32 of Wu
-      const int src = C::GATED ? row / 64 * 32 + row % 32 : row;
-      const bool up = C::GATED && (row & 32);
-      offb[i] = static_cast<uint32_t>((src * p.ldb[up ? 1 : 0] + 8 * swz(row, pc)) * 2);
-      kb[i] = 8 * swz(row, pc);
+    for (int h = 0; h < 2; h++) {
+      const int row = r / (16 * XH) * (32 * XH) + 16 * XH * h + r % (16 * XH);
+      offa[h][i] = static_cast<uint32_t>((row * p.lda + ka[i]) * 2);
     }
-    ka = pc;
   }
-  const auto stage = [&](int buf, int k0) {
-    uint8_t *base = lds + buf * C::kStage;
-    const bool whole = k0 + C::BK <= p.k;
 #pragma unroll
-    for (int i = 0; i < C::PA; i++) {
-      const int j = wid * C::PA + i, row = j * 8 + lane / 8;
-      const uint32_t off = whole || k0 + 8 * swz(row, ka) < p.k ? offa[i] : kOut;
-      dma16(ra, base + j * 1024, off, 2 * k0);
+  for (int i = 0; i < C::PB; i++) {
+    const int r = (wid * C::PB + i) * 8 + lane / 8;
+    kb[i] = 8 * swz(r, lane % 8);
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      const int row = C::GATED ? r : r / (16 * YH) * (32 * YH) + 16 * YH * h + r % (16 * YH);
+      offb[h][i] = static_cast<uint32_t>((row * p.ldb[C::GATED ? h : 0] + kb[i]) * 2);
     }
+  }
+  const auto start_a = [&](auto half, auto buf, int tile) {
+    constexpr int h = decltype(half)::value;
+    uint8_t *dst = lds + decltype(buf)::value * C::kBuf + h * C::kHalfA + wid * (C::PA * 1024);
+    const int k0 = tile * C::BK;
 #pragma unroll
-    for (int i = 0; i < C::PB; i++) {
-      const int j = wid * C::PB + i;
-      const uint32_t off = whole || k0 + kb[i] < p.k ? offb[i] : kOut;
-      const bool up = C::GATED && (j & 4);  // 8 rows a piece: rows 32..63 of each 64 are Wu's
-      dma16(up ? rb1 : rb0, base + C::kImgA + j * 1024, off, 2 * k0);
-    }
+    for (int i = 0; i < C::PA; i++)
+      dma16(ra, dst + i * 1024, ka[i] < p.k - k0 ? offa[h][i] : kOut, 2 * k0);
   };
-  const auto frag = [&](const uint8_t *img, int row, int c) {
-    return *reinterpret_cast<const uint4 *>(img + row * C::RB + swz(row, c) * 16);
+  const auto start_b = [&](auto half, auto buf, int tile) {
+    constexpr int h = decltype(half)::value;
+    uint8_t *dst = lds + decltype(buf)::value * C::kBuf + 2 * C::kHalfA + h * C::kHalfB +
+                   wid * (C::PB * 1024);
+    const int k0 = tile * C::BK;
+#pragma unroll
+    for (int i = 0; i < C::PB; i++)
+      dma16(h ? rb1 : rb0, dst + i * 1024, kb[i] < p.k - k0 ? offb[h][i] : kOut, 2 * k0);
   };
-
-  floatx4 acc[XM][XN];
+  // LDS addresses of this lane's fragments [buffer][32-deep step]
+  uint32_t ata[2][2], atb[2][2];
+  {
+    const uint32_t base = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_void *)lds));
+    const int arow = wm * (16 * XH) + l16, brow = wn * (16 * YH) + l16;
 #pragma unroll
-  for (int x = 0; x < XM; x++)
+    for (int b = 0; b < 2; b++)
 #pragma unroll
-    for (int y = 0; y < XN; y++) acc[x][y] = floatx4{0.f, 0.f, 0.f, 0.f};
-  const int arow = wm * (C::BM / C::WM) + l16, brow = wn * 64 + l16;
-  const int nk = (p.k + C::BK - 1) / C::BK;
-  const bool late = C::kWaves == 8 && wid >= 4;
-  if (nk > 0) stage(0, 0);
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  __syncthreads();
-  for (int kt = 0; kt < nk; kt++) {
-    const int cur = kt & 1;
-    const uint8_t *ia = lds + cur * C::kStage, *ib = ia + C::kImgA;
-    if (!late && kt + 1 < nk) stage(cur ^ 1, (kt + 1) * C::BK);
+      for (int ks = 0; ks < 2; ks++) {
+        ata[b][ks] = base + b * C::kBuf + arow * C::RB + 16 * swz(arow, 4 * ks + lq);
+        atb[b][ks] = base + b * C::kBuf + 2 * C::kHalfA + brow * C::RB + 16 * swz(brow, 4 * ks + lq);
+      }
+  }
+  u32x4 fa[XH][2], fb[2][YH][2];
+  const auto read_a = [&](auto half, auto buf) {
+    constexpr int O = decltype(half)::value * C::kHalfA, b = decltype(buf)::value;
 #pragma unroll
     for (int ks = 0; ks < 2; ks++) {
-      uint4 fa[XM], fb[XN];
-#pragma unroll
-      for (int x = 0; x < XM; x++) fa[x] = frag(ia, arow + 16 * x, 4 * ks + lq);
-#pragma unroll
-      for (int y = 0; y < XN; y++) fb[y] = frag(ib, brow + 16 * y, 4 * ks + lq);
-#pragma unroll
-      for (int x = 0; x < XM; x++) {
-        if (ks == 0 && x == XM / 2 && late && kt + 1 < nk) stage(cur ^ 1, (kt + 1) * C::BK);
-#pragma unroll
-        for (int y = 0; y < XN; y++) acc[x][y] = mma<N>(fa[x], fb[y], acc[x][y]);
-      }
+      read_frag<O>(fa[0][ks], ata[b][ks]);
+      if constexpr (XH > 1) read_frag<O + 2048>(fa[1][ks], ata[b][ks]);
+      if constexpr (XH > 2) read_frag<O + 4096>(fa[2][ks], ata[b][ks]);
+      if constexpr (XH > 2) read_frag<O + 6144>(fa[3][ks], ata[b][ks]);
     }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
+  };
+  const auto read_b = [&](auto half, auto buf) {
+    constexpr int h = decltype(half)::value, O = h * C::kHalfB, b = decltype(buf)::value;
+#pragma unroll
+    for (int ks = 0; ks < 2; ks++) {
+      read_frag<O>(fb[h][0][ks], atb[b][ks]);
+      if constexpr (YH > 1) read_frag<O + 2048>(fb[h][1][ks], atb[b][ks]);
+    }
+  };
+  floatx4 acc[2][XH][2][YH];
+#pragma unroll
+  for (int i = 0; i < 2; i++)
+#pragma unroll
+    for (int x = 0; x < XH; x++)
+#pragma unroll
+      for (int j = 0; j < 2; j++)
+#pragma unroll
+        for (int y = 0; y < YH; y++) acc[i][x][j][y] = floatx4{0.f, 0.f, 0.f, 0.f};
+  const auto multiply = [&](auto ih, auto jh) {
+    constexpr int i = decltype(ih)::value, j = decltype(jh)::value;
+    __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+    for (int ks = 0; ks < 2; ks++)
+#pragma unroll
+      for (int x = 0; x < XH; x++)
+#pragma unroll
+        for (int y = 0; y < YH; y++)
+          acc[i][x][j][y] = mma<N>(fa[x][ks], fb[j][y][ks], acc[i][x][j][y]);
+    __builtin_amdgcn_s_setprio(0);
+  };
+  constexpr std::integral_constant<int, 0> c0{};
+  constexpr std::integral_constant<int, 1> c1{};
+  constexpr int kFlight = 3 * (C::PA + C::PB);
+  const auto phases = [&](auto first, auto second, auto buf, auto other, int t) {
+    constexpr int F = decltype(first)::value, S = decltype(second)::value;
+    read_a(c0, buf);
+    start_b(first, buf, t + 2);
+    wait_vmcnt<kFlight>();
+    settle<XH>(fa);
+    meet();
+    multiply(c0, first);
+    meet();
+    read_b(second, buf);
+    start_a(c0, buf, t + 2);
+    wait_vmcnt<kFlight>();
+    settle<YH>(fb[S]);
+    meet();
+    multiply(c0, second);
+    meet();
+    read_a(c1, buf);
+    start_b(second, buf, t + 2);
+    wait_vmcnt<kFlight>();
+    settle<XH>(fa);
+    meet();
+    multiply(c1, second);
+    meet();
+    read_b(second, other);  // the next tile's first half
+    start_a(c1, buf, t + 2);
+    wait_vmcnt<kFlight>();
+    settle<YH>(fb[S]);
+    meet();
+    multiply(c1, first);
+    meet();
+    (void)F;
+  };
+  start_b(c0, c0, 0);
+  start_a(c0, c0, 0);
+  start_b(c1, c0, 0);
+  start_a(c1, c0, 0);
+  start_b(c1, c1, 1);
+  start_a(c0, c1, 1);
+  start_b(c0, c1, 1);
+  start_a(c1, c1, 1);
+  wait_vmcnt<kFlight>();
+  meet();
+  read_b(c0, c0);
+  settle<YH>(fb[0]);
+  meet();
+  if (wid >= 4) meet();
+  const int nk = (p.k + C::BK - 1) / C::BK;
+  for (int t = 0; t < nk; t += 2) {
+    phases(c0, c1, c0, c1, t);
+    phases(c1, c0, c1, c0, t + 1);
   }
+  if (wid < 4) meet();
+  wait_vmcnt<0>();
+  __syncthreads();
 
   // Results leave through LDS: a 16 x 16 block leaves lane l with rows 4 (l / 16) + r of column
-  // l % 16; from LDS a row of the tile is stored 16 bytes a lane.
-  constexpr int YO = C::GATED ? XN / 2 : XN;  // 16-column blocks of outputs per wave
-  constexpr int LD = C::BO + 8;               // elements of an LDS row
-  constexpr int kRound = C::BM * LD * 2 > C::kLds ? 2 : 1;
-  constexpr int XR = XM / kRound;
+  // l % 16; from LDS a row of the tile is stored 16 bytes a lane.  One row half at a time.
+  constexpr int LD = C::BO + 8;  // elements of an LDS row
+  static_assert(C::BM / 2 * LD * 2 <= C::kLds, "half a tile of results fits the stages");
   uint16_t *img = reinterpret_cast<uint16_t *>(lds);
   const bool vec = p.n % 8 == 0 && (reinterpret_cast<uintptr_t>(p.c) & 15) == 0;
 #pragma unroll
-  for (int round = 0; round < kRound; round++) {
-    if (round) __syncthreads();
+  for (int i = 0; i < 2; i++) {
+    if (i) __syncthreads();
 #pragma unroll
-    for (int x = 0; x < XR; x++)
+    for (int x = 0; x < XH; x++)
 #pragma unroll
-      for (int y = 0; y < YO; y++)
+      for (int j = 0; j < (C::GATED ? 1 : 2); j++)
 #pragma unroll
-        for (int r = 0; r < 4; r++) {
-          const int xx = round * XR + x;
-          const int lr = (wm * XR + x) * 16 + 4 * lq + r, lc = (wn * YO + y) * 16 + l16;
-          float v;
-          if constexpr (C::GATED) {
-            const float g = acc[xx][y][r], u = acc[xx][y + YO][r];
-            v = act(p.act, g) * u;
-            const int row = m0 + wm * (C::BM / C::WM) + xx * 16 + 4 * lq + r, col = n0 + lc;
-            if (p.pre && row < p.m && col < p.n)
-              p.pre[static_cast<int64_t>(row) * p.n + col] = make_float2(g, u);
-          } else {
-            v = acc[xx][y][r];
+        for (int y = 0; y < YH; y++)
+#pragma unroll
+          for (int r = 0; r < 4; r++) {
+            const int lr = (wm * XH + x) * 16 + 4 * lq + r;
+            const int lc = C::GATED ? (wn * YH + y) * 16 + l16 : ((wn * 2 + j) * YH + y) * 16 + l16;
+            float v;
+            if constexpr (C::GATED) {
+              const float g = acc[i][x][0][y][r], u = acc[i][x][1][y][r];
+              v = act(p.act, g) * u;
+              const int row = m0 + wm * (32 * XH) + (i * XH + x) * 16 + 4 * lq + r, col = n0 + lc;
+              if (p.pre && row < p.m && col < p.n)
+                p.pre[static_cast<int64_t>(row) * p.n + col] = make_float2(g, u);
+            } else {
+              v = acc[i][x][j][y][r];
+            }
+            img[lr * LD + lc] = N::save(v);
           }
-          img[lr * LD + lc] = N::save(v);
-        }
     __syncthreads();
     constexpr int CH = C::BO / 8;  // 16-byte chunks of a row
-    for (int i = threadIdx.x; i < C::BM / kRound * CH; i += C::kThreads) {
-      const int lr = i / CH, lc = i % CH * 8;
-      const int row = m0 + lr / (XR * 16) * (C::BM / C::WM) + round * XR * 16 + lr % (XR * 16);
+    for (int e = threadIdx.x; e < C::BM / 2 * CH; e += C::kThreads) {
+      const int lr = e / CH, lc = e % CH * 8;
+      const int row = m0 + lr / (16 * XH) * (32 * XH) + i * (16 * XH) + lr % (16 * XH);
       const int col = n0 + lc;
       if (row >= p.m || col >= p.n) continue;
       uint16_t *dst = p.c + static_cast<int64_t>(row) * p.n + col;
       if (vec) {
         *reinterpret_cast<uint4 *>(dst) = *reinterpret_cast<const uint4 *>(img + lr * LD + lc);
       } else {
-        for (int e = 0; e < 8; e++)
-          if (col + e < p.n) dst[e] = img[lr * LD + lc + e];
+        for (int q = 0; q < 8; q++)
+          if (col + q < p.n) dst[q] = img[lr * LD + lc + q];
       }
     }
   }
@@ -293,14 +421,14 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_kernel(Args p) {
   const int steps = (p.k + 63) / 64, per = (steps + kFewWaves - 1) / kFewWaves;
   const int first = wave * per, last = first + per < steps ? first + per : steps;
   const auto load = [&](const uint16_t *row, int k0) {
-    uint4 v = {0, 0, 0, 0};
+    u32x4 v = {0, 0, 0, 0};
     if (k0 + 8 <= p.k) {
       __builtin_memcpy(&v, row + k0, 16);
     } else {
       uint32_t e[4] = {0, 0, 0, 0};
       for (int i = 0; i < 8; i++)
         if (k0 + i < p.k) e[i / 2] |= static_cast<uint32_t>(row[k0 + i]) << (16 * (i & 1));
-      v = uint4{e[0], e[1], e[2], e[3]};
+      v = u32x4{e[0], e[1], e[2], e[3]};
     }
     return v;
   };
@@ -309,7 +437,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_kernel(Args p) {
   for (int i = 0; i < 2; i++)
 #pragma unroll
     for (int t = 0; t < RT; t++) acc[i][t] = floatx4{0.f, 0.f, 0.f, 0.f};
-  uint4 wv[2][2], nw[2][2];
+  u32x4 wv[2][2], nw[2][2];
   if (first < last)
     for (int h = 0; h < 2; h++)
       for (int i = 0; i < 2; i++) wv[h][i] = load(w[i], first * 64 + 32 * h + 8 * lq);
@@ -323,7 +451,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_kernel(Args p) {
     for (int h = 0; h < 2; h++)
 #pragma unroll
       for (int t = 0; t < RT; t++) {
-        const uint4 xv = load(xr[t], st * 64 + 32 * h + 8 * lq);
+        const u32x4 xv = load(xr[t], st * 64 + 32 * h + 8 * lq);
 #pragma unroll
         for (int i = 0; i < 2; i++) acc[i][t] = mma<N>(xv, wv[h][i], acc[i][t]);
       }
@@ -499,8 +627,8 @@ template <class N, bool GATED>
 vs_status product(const Args &p, hipStream_t s) {
   const int bo = GATED ? 128 : 256;
   const int64_t large = static_cast<int64_t>((p.m + 255) / 256) * ((p.n + bo - 1) / bo);
-  if (large >= 256) return launch_tile<N, Cfg<256, 256, 2, 4, GATED>>(p, s);
-  return launch_tile<N, Cfg<128, 128, 2, 2, GATED>>(p, s);
+  if (large >= 256) return launch_tile<N, Cfg<4, 2, GATED>>(p, s);
+  return launch_tile<N, Cfg<2, 1, GATED>>(p, s);
 }
 
 // Bump allocator over the caller's workspace or the library's pool.
