@@ -28,6 +28,7 @@
 #include <algorithm>
 #include <cstdint>
 #include <type_traits>
+#include <utility>
 
 #include "csrc/kernels/device.h"
 #include "csrc/kernels/number.h"
@@ -41,6 +42,7 @@ namespace {
 typedef float floatx4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) void lds_void;
 
@@ -92,6 +94,12 @@ struct Args {
   uint16_t *c;            // [m][n], row stride n
   float2 *pre;            // [m][n] (g, u), or null
   int act;
+};
+
+// One or two products in a launch: tiles [0, first) belong to q[0], the rest to q[1].
+struct Work {
+  Args q[2];
+  unsigned first, tiles;
 };
 
 // A tile of 2 (rows) x 4 (columns) waves, each with 2 x 2 quadrants of 16 XH x 16 YH products.
@@ -181,22 +189,31 @@ __device__ __forceinline__ void meet() {
 // behind a wave that starts the next phase.  Before that barrier a wave also waits until its
 // pieces of the half that the next phase reads have landed; six halves stay in flight.  Tiles
 // past the end of k are started out of range (zeros), so the counts hold to the end.
+//
+// A workgroup takes tiles blockIdx.x, + gridDim.x, ...; the next tile's first eight halves are
+// started before the results of the last one are stored.
 template <class N, class C>
-__global__ __launch_bounds__(512) void tile_kernel(Args p) {
+__global__ __launch_bounds__(512) void tile_kernel(Work work) {
   extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
   constexpr int XH = C::XH, YH = C::YH;
+  const Args &p = work.q[blockIdx.x < work.first ? 0 : 1];
+  const unsigned begin = blockIdx.x < work.first ? 0 : work.first;
   const unsigned tiles_m = (p.m + C::BM - 1) / C::BM, tiles_n = (p.n + C::BO - 1) / C::BO;
-  unsigned tm, tn;
-  dev::grouped_tile(dev::xcd_remap(blockIdx.x, tiles_m * tiles_n), tiles_m, tiles_n, tm, tn);
-  const int m0 = tm * C::BM, n0 = tn * C::BO;
   const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wid / 4, wn = wid % 4;
   const int l16 = lane & 15, lq = lane >> 4;
 
-  const __amdgpu_buffer_rsrc_t ra = rows_of(p.a, p.lda, m0, p.m, C::BM, p.k);
-  const __amdgpu_buffer_rsrc_t rb0 = rows_of(p.b[0], p.ldb[0], n0, p.n, C::BO, p.k);
-  const __amdgpu_buffer_rsrc_t rb1 =
-      C::GATED ? rows_of(p.b[1], p.ldb[1], n0, p.n, C::BO, p.k) : rb0;
+  int m0, n0;
+  __amdgpu_buffer_rsrc_t ra, rb0, rb1;
+  const auto place = [&](unsigned tile) {
+    unsigned tm, tn;
+    dev::grouped_tile(dev::xcd_remap(tile - begin, tiles_m * tiles_n), tiles_m, tiles_n, tm, tn);
+    m0 = tm * C::BM;
+    n0 = tn * C::BO;
+    ra = rows_of(p.a, p.lda, m0, p.m, C::BM, p.k);
+    rb0 = rows_of(p.b[0], p.ldb[0], n0, p.n, C::BO, p.k);
+    rb1 = C::GATED ? rows_of(p.b[1], p.ldb[1], n0, p.n, C::BO, p.k) : rb0;
+  };
   // Image row r of A half h is row 32 XH (r / 16 XH) + 16 XH h + r % 16 XH of the tile; of B half
   // h it is the same with YH and four waves (GATED: row r of operand h).  Piece i of a wave: image rows
   // 8 (P wid + i) + lane / 8, chunk lane % 8.
@@ -271,15 +288,9 @@ __global__ __launch_bounds__(512) void tile_kernel(Args p) {
       if constexpr (YH > 1) read_frag<O + 2048>(fb[h][1][ks], atb[b][ks]);
     }
   };
+  // Weights are the matrix instruction's first operand, so a lane ends with four neighbouring
+  // columns (4 lq + r of the 16) of one row (l16) of the result.
   floatx4 acc[2][XH][2][YH];
-#pragma unroll
-  for (int i = 0; i < 2; i++)
-#pragma unroll
-    for (int x = 0; x < XH; x++)
-#pragma unroll
-      for (int j = 0; j < 2; j++)
-#pragma unroll
-        for (int y = 0; y < YH; y++) acc[i][x][j][y] = floatx4{0.f, 0.f, 0.f, 0.f};
   const auto multiply = [&](auto ih, auto jh) {
     constexpr int i = decltype(ih)::value, j = decltype(jh)::value;
     __builtin_amdgcn_s_setprio(1);
@@ -289,14 +300,14 @@ __global__ __launch_bounds__(512) void tile_kernel(Args p) {
       for (int x = 0; x < XH; x++)
 #pragma unroll
         for (int y = 0; y < YH; y++)
-          acc[i][x][j][y] = mma<N>(fa[x][ks], fb[j][y][ks], acc[i][x][j][y]);
+          acc[i][x][j][y] = mma<N>(fb[j][y][ks], fa[x][ks], acc[i][x][j][y]);
     __builtin_amdgcn_s_setprio(0);
   };
   constexpr std::integral_constant<int, 0> c0{};
   constexpr std::integral_constant<int, 1> c1{};
   constexpr int kFlight = 3 * (C::PA + C::PB);
   const auto phases = [&](auto first, auto second, auto buf, auto other, int t) {
-    constexpr int F = decltype(first)::value, S = decltype(second)::value;
+    constexpr int S = decltype(second)::value;
     read_a(c0, buf);
     start_b(first, buf, t + 2);
     wait_vmcnt<kFlight>();
@@ -325,77 +336,109 @@ __global__ __launch_bounds__(512) void tile_kernel(Args p) {
     meet();
     multiply(c1, first);
     meet();
-    (void)F;
   };
-  start_b(c0, c0, 0);
-  start_a(c0, c0, 0);
-  start_b(c1, c0, 0);
-  start_a(c1, c0, 0);
-  start_b(c1, c1, 1);
-  start_a(c0, c1, 1);
-  start_b(c0, c1, 1);
-  start_a(c1, c1, 1);
-  wait_vmcnt<kFlight>();
-  meet();
-  read_b(c0, c0);
-  settle<YH>(fb[0]);
-  meet();
-  if (wid >= 4) meet();
+  const auto start_tile = [&] {
+    start_b(c0, c0, 0);
+    start_a(c0, c0, 0);
+    start_b(c1, c0, 0);
+    start_a(c1, c0, 0);
+    start_b(c1, c1, 1);
+    start_a(c0, c1, 1);
+    start_b(c0, c1, 1);
+    start_a(c1, c1, 1);
+  };
   const int nk = (p.k + C::BK - 1) / C::BK;
-  for (int t = 0; t < nk; t += 2) {
-    phases(c0, c1, c0, c1, t);
-    phases(c1, c0, c1, c0, t + 1);
-  }
-  if (wid < 4) meet();
-  wait_vmcnt<0>();
-  __syncthreads();
+  place(blockIdx.x);
+  start_tile();
+  for (unsigned tile = blockIdx.x;;) {
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+#pragma unroll
+      for (int x = 0; x < XH; x++)
+#pragma unroll
+        for (int j = 0; j < 2; j++)
+#pragma unroll
+          for (int y = 0; y < YH; y++) acc[i][x][j][y] = floatx4{0.f, 0.f, 0.f, 0.f};
+    wait_vmcnt<kFlight>();
+    meet();
+    read_b(c0, c0);
+    settle<YH>(fb[0]);
+    meet();
+    if (wid >= 4) meet();
+    for (int t = 0; t < nk; t += 2) {
+      phases(c0, c1, c0, c1, t);
+      phases(c1, c0, c1, c0, t + 1);
+    }
+    if (wid < 4) meet();
+    wait_vmcnt<0>();  // the pieces started past the end of k have written their zeros
+    meet();
+    const int rm = m0 + wm * (32 * XH) + l16, rn = n0 + wn * (C::GATED ? 16 * YH : 32 * YH);
+    tile += gridDim.x;
+    if (tile < work.tiles) {
+      place(tile);
+      start_tile();
+    }
 
-  // Results leave through LDS: a 16 x 16 block leaves lane l with rows 4 (l / 16) + r of column
-  // l % 16; from LDS a row of the tile is stored 16 bytes a lane.  One row half at a time.
-  constexpr int LD = C::BO + 8;  // elements of an LDS row
-  static_assert(C::BM / 2 * LD * 2 <= C::kLds, "half a tile of results fits the stages");
-  uint16_t *img = reinterpret_cast<uint16_t *>(lds);
-  const bool vec = p.n % 8 == 0 && (reinterpret_cast<uintptr_t>(p.c) & 15) == 0;
+    // Results: rows of 16-bit values, two neighbouring 16-column blocks exchanged between odd and
+    // even lane groups where there are two, so a lane stores 16 bytes.
+    constexpr int NB = C::GATED ? YH : 2 * YH;
+    const bool vec = p.n % 8 == 0 && (reinterpret_cast<uintptr_t>(p.c) & 15) == 0;
 #pragma unroll
-  for (int i = 0; i < 2; i++) {
-    if (i) __syncthreads();
+    for (int i = 0; i < 2; i++)
 #pragma unroll
-    for (int x = 0; x < XH; x++)
+      for (int x = 0; x < XH; x++) {
+        const int row = rm + (i * XH + x) * 16;
+        uint32_t w[NB][2];
 #pragma unroll
-      for (int j = 0; j < (C::GATED ? 1 : 2); j++)
-#pragma unroll
-        for (int y = 0; y < YH; y++)
+        for (int b = 0; b < NB; b++) {
+          float v[4];
 #pragma unroll
           for (int r = 0; r < 4; r++) {
-            const int lr = (wm * XH + x) * 16 + 4 * lq + r;
-            const int lc = C::GATED ? (wn * YH + y) * 16 + l16 : ((wn * 2 + j) * YH + y) * 16 + l16;
-            float v;
-            if constexpr (C::GATED) {
-              const float g = acc[i][x][0][y][r], u = acc[i][x][1][y][r];
-              v = act(p.act, g) * u;
-              const int row = m0 + wm * (32 * XH) + (i * XH + x) * 16 + 4 * lq + r, col = n0 + lc;
-              if (p.pre && row < p.m && col < p.n)
-                p.pre[static_cast<int64_t>(row) * p.n + col] = make_float2(g, u);
-            } else {
-              v = acc[i][x][j][y][r];
-            }
-            img[lr * LD + lc] = N::save(v);
+            if constexpr (C::GATED) v[r] = act(p.act, acc[i][x][0][b][r]) * acc[i][x][1][b][r];
+            else v[r] = acc[i][x][b / YH][b % YH][r];
           }
-    __syncthreads();
-    constexpr int CH = C::BO / 8;  // 16-byte chunks of a row
-    for (int e = threadIdx.x; e < C::BM / 2 * CH; e += C::kThreads) {
-      const int lr = e / CH, lc = e % CH * 8;
-      const int row = m0 + lr / (16 * XH) * (32 * XH) + i * (16 * XH) + lr % (16 * XH);
-      const int col = n0 + lc;
-      if (row >= p.m || col >= p.n) continue;
-      uint16_t *dst = p.c + static_cast<int64_t>(row) * p.n + col;
-      if (vec) {
-        *reinterpret_cast<uint4 *>(dst) = *reinterpret_cast<const uint4 *>(img + lr * LD + lc);
-      } else {
-        for (int q = 0; q < 8; q++)
-          if (col + q < p.n) dst[q] = img[lr * LD + lc + q];
+          w[b][0] = N::save(v[0]) | static_cast<uint32_t>(N::save(v[1])) << 16;
+          w[b][1] = N::save(v[2]) | static_cast<uint32_t>(N::save(v[3])) << 16;
+          if constexpr (C::GATED)
+            if (p.pre && row < p.m) {
+              const int col = rn + 16 * b + 4 * lq;
+              float2 *dst = p.pre + static_cast<int64_t>(row) * p.n + col;
+#pragma unroll
+              for (int r = 0; r < 4; r += 2) {
+                const float4 gu = {acc[i][x][0][b][r], acc[i][x][1][b][r], acc[i][x][0][b][r + 1],
+                                   acc[i][x][1][b][r + 1]};
+                if (col + r + 1 < p.n) __builtin_memcpy(dst + r, &gu, 16);
+                else if (col + r < p.n) dst[r] = make_float2(gu.x, gu.y);
+              }
+            }
+        }
+        if (row >= p.m) continue;
+        uint16_t *out = p.c + static_cast<int64_t>(row) * p.n;
+        if (vec && NB % 2 == 0) {
+#if defined(__HIP_DEVICE_COMPILE__)
+#pragma unroll
+          for (int b = 0; b + 1 < NB; b += 2) {
+            const u32x2 lo = __builtin_amdgcn_permlane16_swap(w[b][0], w[b + 1][0], false, false);
+            const u32x2 hi = __builtin_amdgcn_permlane16_swap(w[b][1], w[b + 1][1], false, false);
+            const int col = rn + 16 * (b + (lq & 1)) + 8 * (lq >> 1);
+            if (col < p.n) *reinterpret_cast<uint4 *>(out + col) = uint4{lo.x, hi.x, lo.y, hi.y};
+          }
+#endif
+        } else {
+#pragma unroll
+          for (int b = 0; b < NB; b++) {
+            const int col = rn + 16 * b + 4 * lq;
+            if (vec) {
+              if (col < p.n) *reinterpret_cast<uint2 *>(out + col) = uint2{w[b][0], w[b][1]};
+            } else {
+#pragma unroll
+              for (int r = 0; r < 4; r++)
+                if (col + r < p.n) out[col + r] = static_cast<uint16_t>(w[b][r / 2] >> (16 * (r & 1)));
+            }
+          }
+        }
       }
-    }
+    if (tile >= work.tiles) return;
   }
 }
 
@@ -544,44 +587,63 @@ __global__ __launch_bounds__(256) void transpose_kernel(const uint16_t *__restri
 }
 
 // (dh, g, u) -> dg, du as rows [m][2 fp] (dg, then du) and transposed [2 f][mp]; zeros in the
-// padding of both.  Either output may be null.
+// padding of both.  Either output may be null.  64 x 64 tiles: a wave reads two rows of 64 pairs
+// (16 bytes, two columns, a lane), the results meet in LDS and leave 16 bytes a lane both ways.
 template <class N>
 __global__ __launch_bounds__(256) void slope_kernel(const uint16_t *__restrict__ dh, int64_t ld,
                                                     const float2 *__restrict__ pre, int kind, int m,
                                                     int f, int fp, int mp, int tiles_c,
                                                     uint16_t *__restrict__ rows,
                                                     uint16_t *__restrict__ cols) {
-  __shared__ uint16_t tile[2][64][66];
+  constexpr int LD = 72;  // elements of an LDS row: 16-byte aligned
+  __shared__ __attribute__((aligned(16))) uint16_t tile[2][64][LD];
   const int c0 = static_cast<int>(blockIdx.x % tiles_c) * 64;
   const int r0 = static_cast<int>(blockIdx.x / tiles_c) * 64;
-  const int a = threadIdx.x >> 3, b = (threadIdx.x & 7) * 8;
+  {
+    const int r1 = threadIdx.x / 32, c = (threadIdx.x % 32) * 2;
+    float4 gu[8];
+    uint32_t d[8];
 #pragma unroll
-  for (int i = 0; i < 2; i++) {
-    const int r = r0 + a + 32 * i;
-    uint32_t eg[4] = {0, 0, 0, 0}, eu[4] = {0, 0, 0, 0};
-#pragma unroll
-    for (int j = 0; j < 8; j++) {
-      const int c = c0 + b + j;
-      uint16_t dg = 0, du = 0;
-      if (r < m && c < f) {
-        const float d = N::load(dh[r * ld + c]);
-        const float2 gu = pre[static_cast<int64_t>(r) * f + c];
-        dg = N::save(d * gu.y * act_slope(kind, gu.x));
-        du = N::save(d * act(kind, gu.x));
+    for (int i = 0; i < 8; i++) {
+      const int r = r0 + r1 + 8 * i;
+      gu[i] = float4{0.f, 0.f, 0.f, 0.f};
+      d[i] = 0;
+      if (r >= m || c0 + c >= f) continue;
+      const float2 *p = pre + static_cast<int64_t>(r) * f + c0 + c;
+      const uint16_t *q = dh + r * ld + c0 + c;
+      if (c0 + c + 2 <= f) {
+        __builtin_memcpy(&gu[i], p, 16);
+        __builtin_memcpy(&d[i], q, 4);
+      } else {
+        gu[i].x = p->x;
+        gu[i].y = p->y;
+        d[i] = *q;
       }
-      eg[j / 2] |= static_cast<uint32_t>(dg) << (16 * (j & 1));
-      eu[j / 2] |= static_cast<uint32_t>(du) << (16 * (j & 1));
-      tile[0][a + 32 * i][b + j] = dg;
-      tile[1][a + 32 * i][b + j] = du;
     }
-    if (rows && r < m && c0 + b < fp) {
-      uint16_t *dst = rows + static_cast<int64_t>(r) * (2 * fp) + c0 + b;
-      *reinterpret_cast<uint4 *>(dst) = uint4{eg[0], eg[1], eg[2], eg[3]};
-      *reinterpret_cast<uint4 *>(dst + fp) = uint4{eu[0], eu[1], eu[2], eu[3]};
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      const float d0 = N::load(static_cast<uint16_t>(d[i])), d1 = N::load(static_cast<uint16_t>(d[i] >> 16));
+      const uint32_t dg = N::save(d0 * gu[i].y * act_slope(kind, gu[i].x)) |
+                          static_cast<uint32_t>(N::save(d1 * gu[i].w * act_slope(kind, gu[i].z))) << 16;
+      const uint32_t du = N::save(d0 * act(kind, gu[i].x)) |
+                          static_cast<uint32_t>(N::save(d1 * act(kind, gu[i].z))) << 16;
+      // a pair past the end of its row or of the rows is 0 by d = 0
+      *reinterpret_cast<uint32_t *>(&tile[0][r1 + 8 * i][c]) = dg;
+      *reinterpret_cast<uint32_t *>(&tile[1][r1 + 8 * i][c]) = du;
     }
   }
-  if (!cols) return;
   __syncthreads();
+  const int a = threadIdx.x >> 3, b = (threadIdx.x & 7) * 8;
+  if (rows && c0 + b < fp)
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      const int lr = a + 32 * i;
+      if (r0 + lr >= m) continue;
+      uint16_t *dst = rows + static_cast<int64_t>(r0 + lr) * (2 * fp) + c0 + b;
+      *reinterpret_cast<uint4 *>(dst) = *reinterpret_cast<const uint4 *>(&tile[0][lr][b]);
+      *reinterpret_cast<uint4 *>(dst + fp) = *reinterpret_cast<const uint4 *>(&tile[1][lr][b]);
+    }
+  if (!cols) return;
 #pragma unroll
   for (int k = 0; k < 2; k++)
 #pragma unroll
@@ -608,27 +670,43 @@ bool direct(const void *p, int64_t ld, int64_t k) {
   return k % 8 == 0 && ld % 8 == 0 && reinterpret_cast<uintptr_t>(p) % 16 == 0;
 }
 
+template <class C>
+int64_t tiles_of(const Args &p) {
+  return static_cast<int64_t>((p.m + C::BM - 1) / C::BM) * ((p.n + C::BO - 1) / C::BO);
+}
+
 template <class N, class C>
-vs_status launch_tile(const Args &p, hipStream_t s) {
+vs_status launch_tile(const Args *q, int count, hipStream_t s) {
   static const hipError_t attr =
       hipFuncSetAttribute(reinterpret_cast<const void *>(&tile_kernel<N, C>),
                           hipFuncAttributeMaxDynamicSharedMemorySize, C::kLds);
   VS_HIP(attr);
-  const int64_t tiles = static_cast<int64_t>((p.m + C::BM - 1) / C::BM) * ((p.n + C::BO - 1) / C::BO);
+  Work w{};
+  int64_t tiles = 0;
+  for (int i = 0; i < count; i++) {
+    w.q[i] = q[i];
+    tiles += tiles_of<C>(q[i]);
+    if (i == 0) w.first = static_cast<unsigned>(tiles);
+  }
   VS_REQUIRE(tiles < (1ll << 23), "gated_linear: too many output tiles");
-  hipLaunchKernelGGL((tile_kernel<N, C>), dim3(static_cast<unsigned>(tiles)), dim3(C::kThreads),
-                     C::kLds, s, p);
+  w.tiles = static_cast<unsigned>(tiles);
+  // one product: as many workgroups as fit the chip walk its tiles; two: a workgroup per tile,
+  // the longer product's first, so whichever CU is free takes the next
+  const int64_t fit = static_cast<int64_t>(device_cu_count()) * (160 * 1024 / C::kLds);
+  const unsigned grid = static_cast<unsigned>(count == 1 ? std::min(tiles, fit) : tiles);
+  hipLaunchKernelGGL((tile_kernel<N, C>), dim3(grid), dim3(C::kThreads), C::kLds, s, w);
   VS_HIP(hipGetLastError());
   return VS_OK;
 }
 
 // Large tiles once they give every CU one, else 128 x 128.
 template <class N, bool GATED>
-vs_status product(const Args &p, hipStream_t s) {
-  const int bo = GATED ? 128 : 256;
-  const int64_t large = static_cast<int64_t>((p.m + 255) / 256) * ((p.n + bo - 1) / bo);
-  if (large >= 256) return launch_tile<N, Cfg<4, 2, GATED>>(p, s);
-  return launch_tile<N, Cfg<2, 1, GATED>>(p, s);
+vs_status product(const Args *q, int count, hipStream_t s) {
+  using Large = Cfg<4, 2, GATED>;
+  int64_t large = 0;
+  for (int i = 0; i < count; i++) large += tiles_of<Large>(q[i]);
+  if (large >= 256) return launch_tile<N, Large>(q, count, s);
+  return launch_tile<N, Cfg<2, 1, GATED>>(q, count, s);
 }
 
 // Bump allocator over the caller's workspace or the library's pool.
@@ -733,7 +811,7 @@ vs_status forward(Args p, void *workspace, size_t bytes, hipStream_t s) {
       p.ldb[i] = kp;
     }
   p.k = kp;
-  return product<N, true>(p, s);
+  return product<N, true>(&p, 1, s);
 }
 
 size_t backward_need(int64_t m, int64_t f, int64_t k, bool dx, bool dw) {
@@ -763,32 +841,37 @@ vs_status backward(const uint16_t *x, int64_t ldx, const uint16_t *wg, int64_t l
                        ldh, pre, act, m, f, fp, mp, tc, rows, cols);
     VS_HIP(hipGetLastError());
   }
+  Args q[2] = {};
+  int count = 0;
   if (dx) {
     VS_TRY(transpose(wg, ldg, f, k, wt, 2 * fp, fp, s));
     VS_TRY(transpose(wu, ldu, f, k, wt + fp, 2 * fp, fp, s));
-    Args p{};
-    p.a = rows;
-    p.b[0] = wt;
-    p.lda = p.ldb[0] = 2 * fp;
-    p.m = m;
-    p.n = k;
-    p.k = 2 * fp;
-    p.c = dx;
-    if (m && k) VS_TRY((product<N, false>(p, s)));
+    if (m) {
+      Args &p = q[count++];
+      p.a = rows;
+      p.b[0] = wt;
+      p.lda = p.ldb[0] = 2 * fp;
+      p.m = m;
+      p.n = k;
+      p.k = 2 * fp;
+      p.c = dx;
+    }
   }
   if (dw) {
     VS_TRY(transpose(x, ldx, m, k, xt, mp, mp, s));
-    Args p{};
-    p.a = cols;
-    p.b[0] = xt;
-    p.lda = p.ldb[0] = mp;
-    p.m = 2 * f;
-    p.n = k;
-    p.k = mp;
-    p.c = dw;
-    if (f && k) VS_TRY((product<N, false>(p, s)));
+    if (f) {
+      Args &p = q[count++];
+      p.a = cols;
+      p.b[0] = xt;
+      p.lda = p.ldb[0] = mp;
+      p.m = 2 * f;
+      p.n = k;
+      p.k = mp;
+      p.c = dw;
+    }
   }
-  return VS_OK;
+  if (count == 2 && q[1].k > q[0].k) std::swap(q[0], q[1]);
+  return count ? product<N, false>(q, count, s) : VS_OK;
 }
 
 }  // namespace
