@@ -547,58 +547,75 @@ __global__ __launch_bounds__(256) void pad_kernel(const uint16_t *__restrict__ s
   }
 }
 
-// dst[c][r] = src[r][c], rows of dst padded with zeros to ld_d (a multiple of 8): 64 x 64 tiles
-// through LDS.  Tiles (x: columns of src, y: rows, folded into one grid dimension).
-__global__ __launch_bounds__(256) void transpose_kernel(const uint16_t *__restrict__ src,
-                                                        int64_t ld, int rows, int cols,
-                                                        uint16_t *__restrict__ dst, int64_t ld_d,
-                                                        int rows_p, int tiles_c) {
-  __shared__ uint16_t tile[64][66];
-  const int c0 = static_cast<int>(blockIdx.x % tiles_c) * 64;
-  const int r0 = static_cast<int>(blockIdx.x / tiles_c) * 64;
+// What the backward products read, written by one launch: blocks [0, slope) form dg and du,
+// the rest transpose up to three matrices.
+struct Turn {
+  const uint16_t *src;  // [rows][cols], row stride ld
+  int64_t ld;
+  int rows, cols;
+  uint16_t *dst;        // [cols][rows_p], row stride ld_d; rows_p a multiple of 8, zeros behind rows
+  int64_t ld_d;
+  int rows_p;
+  unsigned tiles_c, tiles;
+};
+struct Prepare {
+  const uint16_t *dh;
+  int64_t ld;
+  const float2 *pre;
+  int act, m, f, fp, mp;
+  uint16_t *rows, *cols;  // dg, du as [m][2 fp] (dg, then du) and transposed [2 f][mp]; either may be null
+  unsigned tiles_c, tiles;
+  Turn turn[3];
+};
+
+constexpr int kLd = 72;  // elements of an LDS row of 64: 16-byte aligned
+
+// Eight values of column c of an LDS tile from row r on.
+__device__ __forceinline__ uint4 column(const uint16_t (&tile)[64][kLd], int r, int c) {
+  uint32_t e[4];
+#pragma unroll
+  for (int j = 0; j < 4; j++)
+    e[j] = tile[r + 2 * j][c] | (static_cast<uint32_t>(tile[r + 2 * j + 1][c]) << 16);
+  return uint4{e[0], e[1], e[2], e[3]};
+}
+
+// 64 x 64 tile: rows in 16-byte pieces into LDS, columns in 16-byte pieces out of it.
+__device__ __forceinline__ void turn_tile(const Turn &t, unsigned block, uint16_t (&tile)[64][kLd]) {
+  const int c0 = static_cast<int>(block % t.tiles_c) * 64, r0 = static_cast<int>(block / t.tiles_c) * 64;
   const int a = threadIdx.x >> 3, b = (threadIdx.x & 7) * 8;
+  uint4 v[2];
 #pragma unroll
   for (int i = 0; i < 2; i++) {
     const int r = r0 + a + 32 * i;
-    uint16_t v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    if (r < rows) {
-      const uint16_t *s = src + r * ld + c0 + b;
-      if (c0 + b + 8 <= cols) {
-        __builtin_memcpy(v, s, 16);
-      } else {
-        for (int j = 0; j < 8; j++)
-          if (c0 + b + j < cols) v[j] = s[j];
-      }
+    v[i] = uint4{0, 0, 0, 0};
+    if (r >= t.rows || c0 + b >= t.cols) continue;
+    const uint16_t *s = t.src + r * t.ld + c0 + b;
+    if (c0 + b + 8 <= t.cols) {
+      __builtin_memcpy(&v[i], s, 16);
+    } else {
+      uint32_t e[4] = {0, 0, 0, 0};
+      for (int j = 0; j < 8; j++)
+        if (c0 + b + j < t.cols) e[j / 2] |= static_cast<uint32_t>(s[j]) << (16 * (j & 1));
+      v[i] = uint4{e[0], e[1], e[2], e[3]};
     }
-#pragma unroll
-    for (int j = 0; j < 8; j++) tile[a + 32 * i][b + j] = v[j];
   }
+#pragma unroll
+  for (int i = 0; i < 2; i++) *reinterpret_cast<uint4 *>(&tile[a + 32 * i][b]) = v[i];
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < 2; i++) {
     const int c = c0 + a + 32 * i, r = r0 + b;
-    if (c >= cols || r >= rows_p) continue;
-    uint32_t e[4];
-#pragma unroll
-    for (int j = 0; j < 4; j++)
-      e[j] = tile[b + 2 * j][a + 32 * i] | (static_cast<uint32_t>(tile[b + 2 * j + 1][a + 32 * i]) << 16);
-    *reinterpret_cast<uint4 *>(dst + c * ld_d + r) = uint4{e[0], e[1], e[2], e[3]};
+    if (c < t.cols && r < t.rows_p)
+      *reinterpret_cast<uint4 *>(t.dst + c * t.ld_d + r) = column(tile, b, a + 32 * i);
   }
 }
 
-// (dh, g, u) -> dg, du as rows [m][2 fp] (dg, then du) and transposed [2 f][mp]; zeros in the
-// padding of both.  Either output may be null.  64 x 64 tiles: a wave reads two rows of 64 pairs
+// (dh, g, u) -> dg, du of a 64 x 64 tile, zeros in the padding: a wave reads two rows of 64 pairs
 // (16 bytes, two columns, a lane), the results meet in LDS and leave 16 bytes a lane both ways.
 template <class N>
-__global__ __launch_bounds__(256) void slope_kernel(const uint16_t *__restrict__ dh, int64_t ld,
-                                                    const float2 *__restrict__ pre, int kind, int m,
-                                                    int f, int fp, int mp, int tiles_c,
-                                                    uint16_t *__restrict__ rows,
-                                                    uint16_t *__restrict__ cols) {
-  constexpr int LD = 72;  // elements of an LDS row: 16-byte aligned
-  __shared__ __attribute__((aligned(16))) uint16_t tile[2][64][LD];
-  const int c0 = static_cast<int>(blockIdx.x % tiles_c) * 64;
-  const int r0 = static_cast<int>(blockIdx.x / tiles_c) * 64;
+__device__ __forceinline__ void slope_tile(const Prepare &p, uint16_t (&tile)[2][64][kLd]) {
+  const int c0 = static_cast<int>(blockIdx.x % p.tiles_c) * 64;
+  const int r0 = static_cast<int>(blockIdx.x / p.tiles_c) * 64;
   {
     const int r1 = threadIdx.x / 32, c = (threadIdx.x % 32) * 2;
     float4 gu[8];
@@ -608,56 +625,64 @@ __global__ __launch_bounds__(256) void slope_kernel(const uint16_t *__restrict__
       const int r = r0 + r1 + 8 * i;
       gu[i] = float4{0.f, 0.f, 0.f, 0.f};
       d[i] = 0;
-      if (r >= m || c0 + c >= f) continue;
-      const float2 *p = pre + static_cast<int64_t>(r) * f + c0 + c;
-      const uint16_t *q = dh + r * ld + c0 + c;
-      if (c0 + c + 2 <= f) {
-        __builtin_memcpy(&gu[i], p, 16);
+      if (r >= p.m || c0 + c >= p.f) continue;
+      const float2 *s = p.pre + static_cast<int64_t>(r) * p.f + c0 + c;
+      const uint16_t *q = p.dh + r * p.ld + c0 + c;
+      if (c0 + c + 2 <= p.f) {
+        __builtin_memcpy(&gu[i], s, 16);
         __builtin_memcpy(&d[i], q, 4);
       } else {
-        gu[i].x = p->x;
-        gu[i].y = p->y;
+        gu[i].x = s->x;
+        gu[i].y = s->y;
         d[i] = *q;
       }
     }
 #pragma unroll
     for (int i = 0; i < 8; i++) {
       const float d0 = N::load(static_cast<uint16_t>(d[i])), d1 = N::load(static_cast<uint16_t>(d[i] >> 16));
-      const uint32_t dg = N::save(d0 * gu[i].y * act_slope(kind, gu[i].x)) |
-                          static_cast<uint32_t>(N::save(d1 * gu[i].w * act_slope(kind, gu[i].z))) << 16;
-      const uint32_t du = N::save(d0 * act(kind, gu[i].x)) |
-                          static_cast<uint32_t>(N::save(d1 * act(kind, gu[i].z))) << 16;
-      // a pair past the end of its row or of the rows is 0 by d = 0
+      const uint32_t dg = N::save(d0 * gu[i].y * act_slope(p.act, gu[i].x)) |
+                          static_cast<uint32_t>(N::save(d1 * gu[i].w * act_slope(p.act, gu[i].z))) << 16;
+      const uint32_t du = N::save(d0 * act(p.act, gu[i].x)) |
+                          static_cast<uint32_t>(N::save(d1 * act(p.act, gu[i].z))) << 16;
+      // a pair past the end of its row or of the rows is 0: d, g and u are
       *reinterpret_cast<uint32_t *>(&tile[0][r1 + 8 * i][c]) = dg;
       *reinterpret_cast<uint32_t *>(&tile[1][r1 + 8 * i][c]) = du;
     }
   }
   __syncthreads();
   const int a = threadIdx.x >> 3, b = (threadIdx.x & 7) * 8;
-  if (rows && c0 + b < fp)
 #pragma unroll
-    for (int i = 0; i < 2; i++) {
-      const int lr = a + 32 * i;
-      if (r0 + lr >= m) continue;
-      uint16_t *dst = rows + static_cast<int64_t>(r0 + lr) * (2 * fp) + c0 + b;
+  for (int i = 0; i < 2; i++) {
+    const int lr = a + 32 * i;
+    if (p.rows && c0 + b < p.fp && r0 + lr < p.m) {
+      uint16_t *dst = p.rows + static_cast<int64_t>(r0 + lr) * (2 * p.fp) + c0 + b;
       *reinterpret_cast<uint4 *>(dst) = *reinterpret_cast<const uint4 *>(&tile[0][lr][b]);
-      *reinterpret_cast<uint4 *>(dst + fp) = *reinterpret_cast<const uint4 *>(&tile[1][lr][b]);
+      *reinterpret_cast<uint4 *>(dst + p.fp) = *reinterpret_cast<const uint4 *>(&tile[1][lr][b]);
     }
-  if (!cols) return;
+  }
 #pragma unroll
-  for (int k = 0; k < 2; k++)
+  for (int i = 0; i < 2; i++) {
+    const int c = c0 + a + 32 * i, r = r0 + b;
+    if (!p.cols || c >= p.f || r >= p.mp) continue;
 #pragma unroll
-    for (int i = 0; i < 2; i++) {
-      const int c = c0 + a + 32 * i, r = r0 + b;
-      if (c >= f || r >= mp) continue;
-      uint32_t e[4];
-#pragma unroll
-      for (int j = 0; j < 4; j++)
-        e[j] = tile[k][b + 2 * j][a + 32 * i] |
-               (static_cast<uint32_t>(tile[k][b + 2 * j + 1][a + 32 * i]) << 16);
-      *reinterpret_cast<uint4 *>(cols + (static_cast<int64_t>(k) * f + c) * mp + r) =
-          uint4{e[0], e[1], e[2], e[3]};
-    }
+    for (int k = 0; k < 2; k++)
+      *reinterpret_cast<uint4 *>(p.cols + (static_cast<int64_t>(k) * p.f + c) * p.mp + r) =
+          column(tile[k], b, a + 32 * i);
+  }
+}
+
+template <class N>
+__global__ __launch_bounds__(256) void prepare_kernel(Prepare p) {
+  __shared__ __attribute__((aligned(16))) uint16_t tile[2][64][kLd];
+  unsigned block = blockIdx.x;
+  if (block < p.tiles) {
+    slope_tile<N>(p, tile);
+    return;
+  }
+  block -= p.tiles;
+  int i = 0;
+  while (i < 2 && block >= p.turn[i].tiles) block -= p.turn[i++].tiles;
+  turn_tile(p.turn[i], block, tile[0]);
 }
 
 // -------------------------------------------------------------------- host
@@ -699,14 +724,39 @@ vs_status launch_tile(const Args *q, int count, hipStream_t s) {
   return VS_OK;
 }
 
-// Large tiles once they give every CU one, else 128 x 128.
+// Estimated time, in units of 1 us at the sizes below, of `count` products with tiles of C.  A tile
+// of nk k tiles takes `fixed` + `step` nk when the chip is full of them and `fixed` + `alone` nk
+// when there are few (fewer share the caches and the power).  Measured at x [m][k], f outputs, both
+// ways round: 1000 x 4096 x 4096 takes 83 us in 256 x 256 tiles and 60 in 128 x 256,
+// 4096 x 4096 x 4096 192 and 233 (243 in 128 x 128), 256 x 2048 x 8192 43, 30 and 23.
+template <class C>
+double estimate(const Args *q, int count) {
+  constexpr double fixed = C::XH == 4 ? 6.5 : C::YH == 2 ? 4.8 : 3.5;
+  constexpr double step = C::XH == 4 ? 1.36 : C::YH == 2 ? 0.83 : 0.89;
+  constexpr double alone = C::XH == 4 ? 0.92 : C::YH == 2 ? 0.59 : 0.42;
+  const double slots = device_cu_count() * (160 * 1024 / C::kLds);
+  double total = 0, longest = 0, t = 0;
+  for (int i = 0; i < count; i++) {
+    const double nk = (q[i].k + C::BK - 1) / C::BK, n = static_cast<double>(tiles_of<C>(q[i]));
+    const int64_t rounds = static_cast<int64_t>(n / slots);
+    const double rest = n - static_cast<double>(rounds) * slots;
+    t = static_cast<double>(rounds) * (fixed + step * nk) +
+        (rest > 0 ? fixed + std::max(alone, step * rest / slots) * nk : 0);
+    total += n * (fixed + step * nk) / slots;
+    longest = std::max(longest, fixed + alone * nk);
+  }
+  return count == 1 ? t : std::max(longest, total);
+}
+
 template <class N, bool GATED>
 vs_status product(const Args *q, int count, hipStream_t s) {
   using Large = Cfg<4, 2, GATED>;
-  int64_t large = 0;
-  for (int i = 0; i < count; i++) large += tiles_of<Large>(q[i]);
-  if (large >= 256) return launch_tile<N, Large>(q, count, s);
-  return launch_tile<N, Cfg<2, 1, GATED>>(q, count, s);
+  using Wide = Cfg<2, 2, GATED>;
+  using Small = Cfg<2, 1, GATED>;
+  const double l = estimate<Large>(q, count), w = estimate<Wide>(q, count), sm = estimate<Small>(q, count);
+  if (l <= w && l <= sm) return launch_tile<N, Large>(q, count, s);
+  if (w <= sm) return launch_tile<N, Wide>(q, count, s);
+  return launch_tile<N, Small>(q, count, s);
 }
 
 // Bump allocator over the caller's workspace or the library's pool.
@@ -740,17 +790,6 @@ vs_status pad(const uint16_t *src, int64_t ld, int64_t rows, int cols, uint16_t 
   if (work == 0) return VS_OK;
   const unsigned grid = static_cast<unsigned>(std::min<int64_t>((work + 255) / 256, 1 << 20));
   hipLaunchKernelGGL(pad_kernel, dim3(grid), dim3(256), 0, s, src, ld, rows, cols, cp, dst);
-  VS_HIP(hipGetLastError());
-  return VS_OK;
-}
-
-vs_status transpose(const uint16_t *src, int64_t ld, int rows, int cols, uint16_t *dst, int64_t ld_d,
-                    int rows_p, hipStream_t s) {
-  const int tc = (cols + 63) / 64;
-  const int64_t tiles = static_cast<int64_t>(tc) * ((rows_p + 63) / 64);
-  if (tiles == 0) return VS_OK;
-  hipLaunchKernelGGL(transpose_kernel, dim3(static_cast<unsigned>(tiles)), dim3(256), 0, s, src, ld,
-                     rows, cols, dst, ld_d, rows_p, tc);
   VS_HIP(hipGetLastError());
   return VS_OK;
 }
@@ -833,19 +872,34 @@ vs_status backward(const uint16_t *x, int64_t ldx, const uint16_t *wg, int64_t l
   uint16_t *wt = dx ? sp.take(static_cast<size_t>(k) * 2 * fp) : nullptr;
   uint16_t *cols = dw ? sp.take(static_cast<size_t>(2) * f * mp) : nullptr;
   uint16_t *xt = dw ? sp.take(static_cast<size_t>(k) * mp) : nullptr;
-  const int tc = (fp + 63) / 64;
-  const int64_t tiles = static_cast<int64_t>(tc) * ((mp + 63) / 64);
-  VS_REQUIRE(tiles < (1ll << 24), "gated_linear: too many tiles");
-  if (tiles) {
-    hipLaunchKernelGGL((slope_kernel<N>), dim3(static_cast<unsigned>(tiles)), dim3(256), 0, s, dh,
-                       ldh, pre, act, m, f, fp, mp, tc, rows, cols);
-    VS_HIP(hipGetLastError());
-  }
+  Prepare pr{};
+  pr.dh = dh;
+  pr.ld = ldh;
+  pr.pre = pre;
+  pr.act = act;
+  pr.m = m;
+  pr.f = f;
+  pr.fp = fp;
+  pr.mp = mp;
+  pr.rows = rows;
+  pr.cols = cols;
+  pr.tiles_c = (fp + 63) / 64;
+  int64_t blocks = static_cast<int64_t>(pr.tiles_c) * ((mp + 63) / 64);
+  VS_REQUIRE(blocks < (1ll << 23), "gated_linear: too many tiles");
+  pr.tiles = static_cast<unsigned>(blocks);
+  int turns = 0;
+  const auto turn = [&](const uint16_t *src, int64_t ld, int r, int c, uint16_t *dst, int64_t ld_d, int rp) {
+    Turn &t = pr.turn[turns++];
+    t = Turn{src, ld, r, c, dst, ld_d, rp, static_cast<unsigned>((c + 63) / 64), 0};
+    const int64_t n = static_cast<int64_t>(t.tiles_c) * ((rp + 63) / 64);
+    t.tiles = static_cast<unsigned>(std::min<int64_t>(n, 1ll << 23));
+    blocks += n;
+  };
   Args q[2] = {};
   int count = 0;
   if (dx) {
-    VS_TRY(transpose(wg, ldg, f, k, wt, 2 * fp, fp, s));
-    VS_TRY(transpose(wu, ldu, f, k, wt + fp, 2 * fp, fp, s));
+    turn(wg, ldg, f, k, wt, 2 * fp, fp);
+    turn(wu, ldu, f, k, wt + fp, 2 * fp, fp);
     if (m) {
       Args &p = q[count++];
       p.a = rows;
@@ -858,7 +912,7 @@ vs_status backward(const uint16_t *x, int64_t ldx, const uint16_t *wg, int64_t l
     }
   }
   if (dw) {
-    VS_TRY(transpose(x, ldx, m, k, xt, mp, mp, s));
+    turn(x, ldx, m, k, xt, mp, mp);
     if (f) {
       Args &p = q[count++];
       p.a = cols;
@@ -869,6 +923,11 @@ vs_status backward(const uint16_t *x, int64_t ldx, const uint16_t *wg, int64_t l
       p.k = mp;
       p.c = dw;
     }
+  }
+  VS_REQUIRE(blocks < (1ll << 23), "gated_linear: too many tiles");
+  if (blocks) {
+    hipLaunchKernelGGL((prepare_kernel<N>), dim3(static_cast<unsigned>(blocks)), dim3(256), 0, s, pr);
+    VS_HIP(hipGetLastError());
   }
   if (count == 2 && q[1].k > q[0].k) std::swap(q[0], q[1]);
   return count ? product<N, false>(q, count, s) : VS_OK;
