@@ -15,7 +15,7 @@
 // side, once as they are and once transposed, x and the weights are transposed, so every product
 // has both operands contiguous in its reduction dimension.
 //
-// Few rows (up to 64): bound by reading the weights.  No LDS staging: a wave streams rows of Wg
+// Few rows (all up to 16, and up to 64 where it is faster): bound by reading the weights.  No LDS staging: a wave streams rows of Wg
 // and Wu straight into matrix-core fragments, the waves of a workgroup cut k, and their sums meet
 // in LDS in a fixed order.
 //
@@ -26,6 +26,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <cmath>
 #include <cstdint>
 #include <type_traits>
 #include <utility>
@@ -445,17 +446,24 @@ __global__ __launch_bounds__(512) void tile_kernel(Work work) {
 // ---------------------------------------------------------------- few rows
 constexpr int kFewWaves = 8;
 
-// RT row tiles of 16.  A workgroup owns 16 outputs; step: 64 k, a lane's two 16-byte loads of a
-// weight row are neighbouring halves of a 128-byte line across the four 16-lane groups.
-template <class N, int RT>
+// RT row tiles of 16, CT column tiles of 16 outputs.  The rows are read once per workgroup (from
+// the caches), the weights once.  A step is 64 k, for which a lane's two 16-byte loads of a weight
+// row are the halves of a 128-byte line across the four 16-lane groups.  The next step's weights
+// and rows are loaded before the current step is multiplied.
+template <class N, int RT, int CT>
 __global__ __launch_bounds__(64 * kFewWaves) void few_kernel(Args p) {
-  __shared__ float part[kFewWaves][2][RT][4][64];
+  constexpr int H = kFewWaves / 2;
+  __shared__ float part[H][2 * CT * RT * 4][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int l16 = lane & 15, lq = lane >> 4;
-  const int n0 = blockIdx.x * 16;
-  const int n = n0 + l16 < p.n ? n0 + l16 : p.n - 1;
-  const uint16_t *w[2] = {p.b[0] + n * p.ldb[0], p.b[1] + n * p.ldb[1]};
-  const uint16_t *xr[RT];
+  const int n0 = blockIdx.x * (16 * CT);
+  const uint16_t *w[2][CT], *xr[RT];
+#pragma unroll
+  for (int c = 0; c < CT; c++) {
+    const int n = n0 + 16 * c + l16 < p.n ? n0 + 16 * c + l16 : p.n - 1;
+#pragma unroll
+    for (int i = 0; i < 2; i++) w[i][c] = p.b[i] + n * p.ldb[i];
+  }
 #pragma unroll
   for (int t = 0; t < RT; t++) {
     const int row = 16 * t + l16 < p.m ? 16 * t + l16 : p.m - 1;  // copies of it are not stored
@@ -463,9 +471,12 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_kernel(Args p) {
   }
   const int steps = (p.k + 63) / 64, per = (steps + kFewWaves - 1) / kFewWaves;
   const int first = wave * per, last = first + per < steps ? first + per : steps;
-  const auto load = [&](const uint16_t *row, int k0) {
+  struct Step {
+    u32x4 w[2][2][CT], x[2][RT];
+  };
+  const auto load = [&](const uint16_t *row, int k0, bool whole) {
     u32x4 v = {0, 0, 0, 0};
-    if (k0 + 8 <= p.k) {
+    if (whole || k0 + 8 <= p.k) {
       __builtin_memcpy(&v, row + k0, 16);
     } else {
       uint32_t e[4] = {0, 0, 0, 0};
@@ -475,50 +486,81 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_kernel(Args p) {
     }
     return v;
   };
-  floatx4 acc[2][RT];
+  const auto fetch = [&](Step &s, int st, bool whole) {
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      const int k0 = st * 64 + 32 * h + 8 * lq;
+#pragma unroll
+      for (int i = 0; i < 2; i++)
+#pragma unroll
+        for (int c = 0; c < CT; c++) s.w[h][i][c] = load(w[i][c], k0, whole);
+#pragma unroll
+      for (int t = 0; t < RT; t++) s.x[h][t] = load(xr[t], k0, whole);
+    }
+  };
+  floatx4 acc[2][CT][RT];
 #pragma unroll
   for (int i = 0; i < 2; i++)
 #pragma unroll
-    for (int t = 0; t < RT; t++) acc[i][t] = floatx4{0.f, 0.f, 0.f, 0.f};
-  u32x4 wv[2][2], nw[2][2];
-  if (first < last)
-    for (int h = 0; h < 2; h++)
-      for (int i = 0; i < 2; i++) wv[h][i] = load(w[i], first * 64 + 32 * h + 8 * lq);
-  for (int st = first; st < last; st++) {
-    if (st + 1 < last)
+    for (int c = 0; c < CT; c++)
 #pragma unroll
-      for (int h = 0; h < 2; h++)
-#pragma unroll
-        for (int i = 0; i < 2; i++) nw[h][i] = load(w[i], (st + 1) * 64 + 32 * h + 8 * lq);
+      for (int t = 0; t < RT; t++) acc[i][c][t] = floatx4{0.f, 0.f, 0.f, 0.f};
+  const auto multiply = [&](const Step &s) {
 #pragma unroll
     for (int h = 0; h < 2; h++)
 #pragma unroll
-      for (int t = 0; t < RT; t++) {
-        const u32x4 xv = load(xr[t], st * 64 + 32 * h + 8 * lq);
+      for (int t = 0; t < RT; t++)
 #pragma unroll
-        for (int i = 0; i < 2; i++) acc[i][t] = mma<N>(xv, wv[h][i], acc[i][t]);
-      }
+        for (int i = 0; i < 2; i++)
 #pragma unroll
-    for (int h = 0; h < 2; h++)
-#pragma unroll
-      for (int i = 0; i < 2; i++) wv[h][i] = nw[h][i];
+          for (int c = 0; c < CT; c++) acc[i][c][t] = mma<N>(s.x[h][t], s.w[h][i][c], acc[i][c][t]);
+  };
+  // whole steps two at a time, so neither step's registers are copied
+  const int whole = last * 64 <= p.k ? last : last - 1;
+  Step s0, s1;
+  int st = first;
+  if (st < whole) fetch(s0, st, true);
+  for (; st + 1 < whole; st += 2) {
+    fetch(s1, st + 1, true);
+    multiply(s0);
+    if (st + 2 < whole) fetch(s0, st + 2, true);
+    multiply(s1);
   }
+  if (st < whole) {
+    multiply(s0);
+    st++;
+  }
+  if (st < last) {
+    fetch(s0, st, false);
+    multiply(s0);
+  }
+  // waves 4..7 add to waves 0..3, and those four are added in order
+  const auto slot = [&](int i, int c, int t, int r) { return ((i * CT + c) * RT + t) * 4 + r; };
 #pragma unroll
-  for (int i = 0; i < 2; i++)
+  for (int half = 1; half >= 0; half--) {
+    if (wave / H == half)
 #pragma unroll
-    for (int t = 0; t < RT; t++)
+      for (int i = 0; i < 2; i++)
 #pragma unroll
-      for (int r = 0; r < 4; r++) part[wave][i][t][r][lane] = acc[i][t][r];
-  __syncthreads();
-  for (int i = threadIdx.x; i < RT * 256; i += 64 * kFewWaves) {
-    const int t = i / 256, r = i / 64 % 4, l = i % 64;
+        for (int c = 0; c < CT; c++)
+#pragma unroll
+          for (int t = 0; t < RT; t++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+              float *at = &part[wave % H][slot(i, c, t, r)][lane];
+              *at = half ? acc[i][c][t][r] : *at + acc[i][c][t][r];
+            }
+    __syncthreads();
+  }
+  for (int e = threadIdx.x; e < CT * RT * 256; e += 64 * kFewWaves) {
+    const int c = e / (RT * 256), t = e / 256 % RT, r = e / 64 % 4, l = e % 64;
     float g = 0.f, u = 0.f;
 #pragma unroll
-    for (int v = 0; v < kFewWaves; v++) {
-      g += part[v][0][t][r][l];
-      u += part[v][1][t][r][l];
+    for (int v = 0; v < H; v++) {
+      g += part[v][slot(0, c, t, r)][l];
+      u += part[v][slot(1, c, t, r)][l];
     }
-    const int row = 16 * t + 4 * (l / 16) + r, col = n0 + l % 16;
+    const int row = 16 * t + 4 * (l / 16) + r, col = n0 + 16 * c + l % 16;
     if (row >= p.m || col >= p.n) continue;
     const int64_t at = static_cast<int64_t>(row) * p.n + col;
     p.c[at] = N::save(act(p.act, g) * u);
@@ -805,13 +847,12 @@ vs_status check(const char *who, int dtype, int act, int64_t m, int64_t f, int64
 }
 
 struct ForwardNeed {
-  bool few, px, pg, pu;
+  bool px, pg, pu;  // copies to rows that the DMA can read
   size_t bytes;
 };
 ForwardNeed forward_need(int64_t m, int64_t f, int64_t k, bool dx, bool dg, bool du) {
   ForwardNeed q{};
-  q.few = m <= kFewRows;
-  if (q.few) return q;
+  if (m <= kFewRows) return q;
   q.px = !dx;
   q.pg = !dg;
   q.pu = !du;
@@ -820,18 +861,52 @@ ForwardNeed forward_need(int64_t m, int64_t f, int64_t k, bool dx, bool dg, bool
   return q;
 }
 
+template <class N, int RT, int CT>
+void launch_few_as(const Args &p, hipStream_t s) {
+  hipLaunchKernelGGL((few_kernel<N, RT, CT>), dim3(static_cast<unsigned>((p.n + 16 * CT - 1) / (16 * CT))),
+                     dim3(64 * kFewWaves), 0, s, p);
+}
+
+// Column tiles of few_kernel for up to kFewRows rows; 0: the tile kernel is faster.  One CU takes in
+// about 31 bytes a nanosecond of weights and rows this way (8192 x 16384 at 64 rows: 132 us with two
+// column tiles, 185 with one), workgroups of two column tiles one at a time.  The tile kernel moves
+// more bytes at once but fills the chip only with many outputs (33 rows of 4096 x 10240: 42 us
+// against 53; of 2048 x 2048: 20 against 11).
+int few_columns(const Args &p, bool all_direct) {
+  const int rt = (p.m + 15) / 16;
+  if (rt == 1) return 1;
+  const double cu = device_cu_count();
+  const auto few = [&](int ct) {
+    const double groups = (p.n + 16 * ct - 1) / (16 * ct) / cu;
+    const double rounds = ct == 2 ? std::ceil(groups) : std::max(1.0, groups);
+    return 2 + rounds * (64.0 * ct + 32.0 * rt) * p.k / 31e3;
+  };
+  const double one = few(1), two = few(2);
+  const double tile = 5 + std::max(estimate<Cfg<2, 1, true>>(&p, 1), 4.0 * p.n * p.k / 4.6e6);
+  if (all_direct && tile < std::min(one, two)) return 0;
+  return one <= two ? 1 : 2;
+}
+
+template <class N>
+void launch_few(const Args &p, int ct, hipStream_t s) {
+  if (p.m <= 16) launch_few_as<N, 1, 1>(p, s);
+  else if (p.m <= 32) ct == 2 ? launch_few_as<N, 2, 2>(p, s) : launch_few_as<N, 2, 1>(p, s);
+  else if (p.m <= 48) ct == 2 ? launch_few_as<N, 3, 2>(p, s) : launch_few_as<N, 3, 1>(p, s);
+  else ct == 2 ? launch_few_as<N, 4, 2>(p, s) : launch_few_as<N, 4, 1>(p, s);
+}
+
 template <class N>
 vs_status forward(Args p, void *workspace, size_t bytes, hipStream_t s) {
-  const ForwardNeed q = forward_need(p.m, p.n, p.k, direct(p.a, p.lda, p.k),
-                                     direct(p.b[0], p.ldb[0], p.k), direct(p.b[1], p.ldb[1], p.k));
-  if (q.few) {
-    const dim3 grid(static_cast<unsigned>((p.n + 15) / 16)), block(64 * kFewWaves);
-    if (p.m <= 16) hipLaunchKernelGGL((few_kernel<N, 1>), grid, block, 0, s, p);
-    else if (p.m <= 32) hipLaunchKernelGGL((few_kernel<N, 2>), grid, block, 0, s, p);
-    else hipLaunchKernelGGL((few_kernel<N, 4>), grid, block, 0, s, p);
-    VS_HIP(hipGetLastError());
-    return VS_OK;
+  const bool da = direct(p.a, p.lda, p.k), dg = direct(p.b[0], p.ldb[0], p.k),
+             du = direct(p.b[1], p.ldb[1], p.k);
+  if (p.m <= kFewRows) {
+    if (const int ct = few_columns(p, da && dg && du)) {
+      launch_few<N>(p, ct, s);
+      VS_HIP(hipGetLastError());
+      return VS_OK;
+    }
   }
+  const ForwardNeed q = forward_need(p.m, p.n, p.k, da, dg, du);
   DeviceBuffer own;
   Space sp;
   VS_TRY(open_space(sp, own, workspace, bytes, q.bytes, s));
@@ -849,7 +924,7 @@ vs_status forward(Args p, void *workspace, size_t bytes, hipStream_t s) {
       p.b[i] = d;
       p.ldb[i] = kp;
     }
-  p.k = kp;
+  p.k = kp;  // (the same where nothing was copied: a direct operand has whole pieces)
   return product<N, true>(&p, 1, s);
 }
 

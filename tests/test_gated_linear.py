@@ -103,7 +103,7 @@ def test_activations(dev, act, m):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("shape", [(4096, 200, 2100), (4100, 1000, 2056), (2100, 2048, 5000), (70, 4096, 3000),
-                                   (60, 1027, 4099)])
+                                   (60, 1027, 4099), (35, 1024, 17000), (20, 512, 16000), (1000, 1024, 1030)])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_large_tiles(shape, dtype):
     """Shapes whose forward or backward products take the large tiles, ragged in every dimension."""
