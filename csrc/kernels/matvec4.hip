@@ -17,11 +17,14 @@
 // where sum x comes from one more product, with ones, in the layout it is needed in.  The factor
 // 16 costs at most 3 of fp32's 24 bits against the sum of |x (q - z)|; weights are never rounded.
 //
-// A lane loads 16 bytes of its column's row: 32 neighbouring k, of which a matrix instruction
-// takes 8 from each of the four 16-lane groups.  Two swaps of half and quarter waves transpose
-// the four registers against the four groups, so that one instruction sees 32 neighbouring k
-// and any group of 32 or more can be scaled.  The waves of a workgroup share its columns and cut
-// k; their sums meet in LDS in a fixed order.
+// A step is 128 k of 16 columns: 64 bytes of each row, which four neighbouring lanes load.  (16
+// neighbouring lanes on 16 rows, the order the matrix instruction wants, cost the cache four times
+// the lookups and ran at 2.8 TB/s however many loads were in flight.)  Through LDS a lane gets 16
+// bytes of its column: 32 neighbouring k, of which an instruction takes 8 from each of the four
+// 16-lane groups.  Two swaps of half and quarter waves transpose the four registers against the
+// four groups, so that one instruction sees 32 neighbouring k and any group of 32 or more can be
+// scaled.  The waves of a workgroup share its columns and cut k; their sums meet in LDS in a fixed
+// order.  28000 x 8192 with groups of 64: 33 us for one row, 39 for 16 (3.8 and 3.3 TB/s).
 // Copyright 2026 veles.simd_amd authors. Apache-2.0.
 #include <hip/hip_runtime.h>
 
@@ -41,9 +44,10 @@ typedef float floatx4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
-constexpr int kWaves = 8;
 constexpr int kBlock = 128;  // k of one step: 16 bytes of q per lane
+constexpr int kDepth = 2;
 
 struct Args {
   const uint16_t *x;
@@ -70,21 +74,22 @@ __device__ __forceinline__ floatx4 mma(const Frag &a, const Frag &b, floatx4 c) 
                                                   __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
-// Eight 4-bit numbers as 16 + q: pair p is (q_p, q_{p + 4}).
+// Eight 4-bit numbers as 16 + q: pair p is (q_p, q_{p + 4}).  `base` holds 16 twice; it comes in a
+// register, where the mask and it can be operands of one and-or.
 template <class N>
-__device__ __forceinline__ Frag unpack(uint32_t w) {
+__device__ __forceinline__ Frag unpack(uint32_t w, uint32_t base) {
   constexpr bool B = std::is_same_v<N, num::BF16>;
-  constexpr uint32_t mask = B ? 0x00780078u : 0x03c003c0u, one = B ? 0x41804180u : 0x4c004c00u;
+  constexpr uint32_t mask = B ? 0x00780078u : 0x03c003c0u;
   Frag f;
-  f.r[0] = ((B ? w << 3 : w << 6) & mask) | one;
-  f.r[1] = ((B ? w >> 1 : w << 2) & mask) | one;
-  f.r[2] = ((B ? w >> 5 : w >> 2) & mask) | one;
-  f.r[3] = ((B ? w >> 9 : w >> 6) & mask) | one;
+  f.r[0] = ((B ? w << 3 : w << 6) & mask) | base;
+  f.r[1] = ((B ? w >> 1 : w << 2) & mask) | base;
+  f.r[2] = ((B ? w >> 5 : w >> 2) & mask) | base;
+  f.r[3] = ((B ? w >> 9 : w >> 6) & mask) | base;
   return f;
 }
 
 // Eight neighbouring values of x in the order that unpack() gives the weights.
-__device__ __forceinline__ Frag pairs(const uint4 &v) {
+__device__ __forceinline__ Frag pairs(const u32x4 &v) {
   Frag f;
   f.r[0] = __builtin_amdgcn_perm(v.z, v.x, 0x05040100);  // 0, 4
   f.r[1] = __builtin_amdgcn_perm(v.z, v.x, 0x07060302);  // 1, 5
@@ -111,95 +116,124 @@ __device__ __forceinline__ void transpose(uint32_t (&w)[4]) {
 #endif
 }
 
-// What one lane loads for one step.  CT column tiles of 16; NG groups in a step.
-template <int CT, int NG>
-struct Loaded {
-  uint32_t q[CT][4];
-  uint4 x[4];
-  uint16_t s[CT][NG];
-  uint8_t z[CT][NG];
-};
-
 // CT: column tiles of 16 per workgroup; GS: MFMA steps of 32 per group (1, 2, 4; 4 covers larger
 // groups through span); RV: accumulator rows in use, ceil(m / 4): row m of x is put where it
 // comes out in accumulator register m / 4, so few rows scale few registers.
-template <class N, int CT, int GS, int RV>
+//
+// kDepth steps of weights and x are in flight per wave.  Their loads are issued unconditionally (past
+// the end the last step again): a load under a condition would make the compiler wait for all.
+// Four neighbouring lanes load the 64 bytes of one row and the fragments are formed through LDS: a
+// load in fragment order (16 rows in 16 neighbouring lanes) costs the cache four times the lookups.
+template <class N, int kWaves, int CT, int GS, int RV>
 __global__ __launch_bounds__(64 * kWaves) void matvec4_kernel(Args p) {
-  constexpr int NG = 4 / GS;
-  using L = Loaded<CT, NG>;
-  __shared__ float part[kWaves][CT][RV][64];
+  constexpr int NG = 4 / GS;                 // groups in a step
+  constexpr int kStage = 8;                  // steps whose scales a wave keeps in LDS
+  constexpr int kCols = 16 * CT, kSlots = kStage * NG;
+  constexpr int kShare = 64 / kCols;         // lanes that fetch scales for one column
+  constexpr int kMine = kSlots / kShare;
+  static_assert(kCols <= 64 && kSlots % kShare == 0, "a wave fetches the scales of its columns");
+  // a wave's scales and zero points and one step of rows, then the waves' sums
+  union Shared {
+    struct {
+      uint32_t sz[kWaves][kSlots][kCols];
+      u32x4 turn[kWaves][CT + 4][64];
+    };
+    float part[kWaves][CT][RV][64];
+  };
+  __shared__ Shared lds;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int l16 = lane & 15, lq = lane >> 4;
-  const int m0 = blockIdx.y * 16, n0 = blockIdx.x * (16 * CT);
-  const int row = m0 + l16 / 4 + 4 * (l16 % 4);  // A row l16
-  const bool has = row < p.m;
-  const uint16_t *xr = p.x + (has ? row : 0) * p.ldx;
+  const int m0 = blockIdx.y * 16, n0 = blockIdx.x * kCols;
+  const int r4 = lane / 4, c4 = lane % 4;    // row and 16-byte chunk that this lane loads
+  const int row = m0 + r4 / 4 + 4 * (r4 % 4);  // A row r4
+  const uint16_t *xr = p.x + (row < p.m ? row : 0) * p.ldx;  // copies of row 0 are not stored
   const uint8_t *qr[CT];
-  int64_t sr[CT];
 #pragma unroll
-  for (int c = 0; c < CT; c++) {
-    const int64_t n = n0 + 16 * c + l16 < p.n ? n0 + 16 * c + l16 : p.n - 1;
-    qr[c] = p.q + n * p.ldq;
-    sr[c] = n * p.groups;
-  }
+  for (int c = 0; c < CT; c++)
+    qr[c] = p.q + (n0 + 16 * c + r4 < p.n ? n0 + 16 * c + r4 : p.n - 1) * p.ldq;
+  // chunk c of row r lies at 4 r + (c ^ r / 4 % 4): reads and writes without bank conflicts
+  u32x4 *turn = &lds.turn[wave][0][0];
+  const int put = 4 * r4 + (c4 ^ (r4 / 4 % 4)), get = 4 * l16 + (lq ^ (l16 / 4 % 4));
   const int blocks = (p.k + kBlock - 1) / kBlock, bytes = (p.k + 1) / 2;
   const int per = (blocks + kWaves - 1) / kWaves;
   const int first = wave * per, last = first + per < blocks ? first + per : blocks;
+  const int whole = last * kBlock <= p.k ? last : last - 1;  // steps that end inside their row
 
-  const auto fetch = [&](int kb, L &v) {
-    const int qo = kb * (kBlock / 2) + 16 * lq;
-    if ((kb + 1) * kBlock <= p.k) {
+  struct Step {
+    u32x4 x[4], q[CT];
+  };
+  const auto fetch = [&](int kb, Step &v) {
 #pragma unroll
-      for (int c = 0; c < CT; c++) __builtin_memcpy(v.q[c], qr[c] + qo, 16);
+    for (int j = 0; j < 4; j++) __builtin_memcpy(&v.x[j], xr + kb * kBlock + 32 * j + 8 * c4, 16);
 #pragma unroll
-      for (int j = 0; j < 4; j++) {
-        v.x[j] = uint4{0, 0, 0, 0};
-        if (has) __builtin_memcpy(&v.x[j], xr + kb * kBlock + 32 * j + 8 * lq, 16);
-      }
-    } else {  // the row ends inside
+    for (int c = 0; c < CT; c++) __builtin_memcpy(&v.q[c], qr[c] + kb * (kBlock / 2) + 16 * c4, 16);
+  };
+  // Scales (low half) and 16 + zero points (high half) of steps [kb, kb + kStage): this lane's
+  // kMine neighbouring groups of one column.
+  const int scol = lane % kCols, part = lane / kCols;
+  const int64_t srow = static_cast<int64_t>(n0 + scol < p.n ? n0 + scol : p.n - 1) * p.groups;
+  struct Scales {
+    uint16_t s[kMine];
+    uint8_t z[kMine];
+  };
+  const auto fetch_scales = [&](int kb, Scales &v) {
+    const int g0 = NG > 1 ? kb * NG : kb / p.span;
+    const int g = g0 + part * kMine;
+    if (p.span == 1 && g0 + kSlots <= p.groups) {
+      __builtin_memcpy(v.s, p.s + srow + g, sizeof(v.s));
+      if (p.z) __builtin_memcpy(v.z, p.z + srow + g, sizeof(v.z));
+    } else {
 #pragma unroll
-      for (int c = 0; c < CT; c++)
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-          uint32_t w = 0;
-          for (int b = 0; b < 4; b++)
-            if (qo + 4 * j + b < bytes) w |= static_cast<uint32_t>(qr[c][qo + 4 * j + b]) << (8 * b);
-          v.q[c][j] = w;
-        }
-#pragma unroll
-      for (int j = 0; j < 4; j++) {
-        uint32_t w[4] = {0, 0, 0, 0};
-        const int k0 = kb * kBlock + 32 * j + 8 * lq;
-        for (int e = 0; e < 8; e++)
-          if (has && k0 + e < p.k) w[e / 2] |= static_cast<uint32_t>(xr[k0 + e]) << (16 * (e & 1));
-        v.x[j] = uint4{w[0], w[1], w[2], w[3]};
+      for (int i = 0; i < kMine; i++) {
+        int at = NG > 1 || p.span == 1 ? g + i : (kb + part * kMine + i) / p.span;
+        at = at < p.groups ? at : p.groups - 1;
+        v.s[i] = p.s[srow + at];
+        if (p.z) v.z[i] = p.z[srow + at];
       }
     }
+  };
+  const auto keep_scales = [&](const Scales &v) {
 #pragma unroll
-    for (int c = 0; c < CT; c++)
-#pragma unroll
-      for (int i = 0; i < NG; i++) {
-        int g = NG > 1 ? kb * NG + i : kb / p.span;
-        g = g < p.groups ? g : p.groups - 1;
-        v.s[c][i] = p.s[sr[c] + g];
-        v.z[c][i] = p.z ? p.z[sr[c] + g] : 8;
-      }
+    for (int i = 0; i < kMine; i++)
+      lds.sz[wave][part * kMine + i][scol] =
+          v.s[i] | static_cast<uint32_t>(p.z ? v.z[i] + 16 : 24) << 16;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
   };
 
   const Frag ones = std::is_same_v<N, num::BF16>
                         ? Frag{{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u}}
                         : Frag{{0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u}};
+  uint32_t base = std::is_same_v<N, num::BF16> ? 0x41804180u : 0x4c004c00u;
+  asm volatile("" : "+v"(base));
   float sum[CT][RV];
 #pragma unroll
   for (int c = 0; c < CT; c++)
 #pragma unroll
     for (int r = 0; r < RV; r++) sum[c][r] = 0.f;
-  L cur, next;
-  if (first < last) fetch(first, cur);
-  for (int kb = first; kb < last; kb++) {
-    if (kb + 1 < last) fetch(kb + 1, next);
+  const auto multiply = [&](const Step &v, int slot) {
+    // LDS works in order within a wave: the reads see these writes, and the next step's writes
+    // come after them
 #pragma unroll
-    for (int c = 0; c < CT; c++) transpose(cur.q[c]);
+    for (int j = 0; j < 4; j++) turn[64 * j + put] = v.x[j];
+#pragma unroll
+    for (int c = 0; c < CT; c++) turn[64 * (4 + c) + put] = v.q[c];
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    u32x4 x[4];
+    uint32_t q[CT][4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) x[j] = turn[64 * j + get];
+#pragma unroll
+    for (int c = 0; c < CT; c++) {
+      const u32x4 w = turn[64 * (4 + c) + get];
+#pragma unroll
+      for (int j = 0; j < 4; j++) q[c][j] = w[j];
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int c = 0; c < CT; c++) transpose(q[c]);
 #pragma unroll
     for (int i = 0; i < NG; i++) {
       const floatx4 none = {0.f, 0.f, 0.f, 0.f};
@@ -208,57 +242,112 @@ __global__ __launch_bounds__(64 * kWaves) void matvec4_kernel(Args p) {
       for (int c = 0; c < CT; c++) acc[c] = none;
 #pragma unroll
       for (int j = i * GS; j < (i + 1) * GS; j++) {
-        const Frag a = pairs(cur.x[j]);
+        const Frag a = pairs(x[j]);
         sx = mma<N>(a, ones, sx);
 #pragma unroll
-        for (int c = 0; c < CT; c++) acc[c] = mma<N>(a, unpack<N>(cur.q[c][j]), acc[c]);
+        for (int c = 0; c < CT; c++) acc[c] = mma<N>(a, unpack<N>(q[c][j], base), acc[c]);
       }
 #pragma unroll
       for (int c = 0; c < CT; c++) {
-        const float s = N::load(cur.s[c][i]), z = -16.f - static_cast<float>(cur.z[c][i]);
+        const uint32_t sz = lds.sz[wave][slot * NG + i][16 * c + l16];
+        const float s = N::load(static_cast<uint16_t>(sz)), z = -static_cast<float>(sz >> 16);
 #pragma unroll
         for (int r = 0; r < RV; r++) sum[c][r] = fmaf(s, fmaf(z, sx[r], acc[c][r]), sum[c][r]);
       }
     }
-    cur = next;
+  };
+  Scales sc;
+  Step v[kDepth];
+  if (first < last) fetch_scales(first, sc);
+  if (first < whole)
+#pragma unroll
+    for (int u = 0; u < kDepth; u++) fetch(first + u < whole ? first + u : whole - 1, v[u]);
+  for (int kb = first; kb < last; kb += kStage) {
+    if (kb != first) {
+      __builtin_amdgcn_wave_barrier();  // the last steps' reads of the image come first
+      fetch_scales(kb, sc);
+    }
+    keep_scales(sc);
+    const int end = kb + kStage < whole ? kb + kStage : whole;
+    int i = kb;
+    for (; i + kDepth <= end; i += kDepth)
+#pragma unroll
+      for (int u = 0; u < kDepth; u++) {
+        multiply(v[u], i + u - kb);
+        fetch(i + u + kDepth < whole ? i + u + kDepth : whole - 1, v[u]);
+      }
+#pragma unroll
+    for (int u = 0; u < kDepth - 1; u++)  // the last steps of the wave
+      if (i + u < end) multiply(v[u], i + u - kb);
+    if (whole < last && last - kb <= kStage) {  // the row ends inside the last step
+      Step t;
+      const int k0 = whole * kBlock;
+#pragma unroll
+      for (int c = 0; c < CT; c++) {
+        uint32_t w[4] = {0, 0, 0, 0};
+        const int o = k0 / 2 + 16 * c4;
+#pragma unroll
+        for (int e = 0; e < 16; e++)
+          if (o + e < bytes) w[e / 4] |= static_cast<uint32_t>(qr[c][o + e]) << (8 * (e & 3));
+        t.q[c] = u32x4{w[0], w[1], w[2], w[3]};
+      }
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        uint32_t w[4] = {0, 0, 0, 0};
+        const int o = k0 + 32 * j + 8 * c4;
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+          if (o + e < p.k) w[e / 2] |= static_cast<uint32_t>(xr[o + e]) << (16 * (e & 1));
+        t.x[j] = u32x4{w[0], w[1], w[2], w[3]};
+      }
+      multiply(t, whole - kb);
+    }
   }
+  __syncthreads();  // the images make room for the sums
 #pragma unroll
   for (int c = 0; c < CT; c++)
 #pragma unroll
-    for (int r = 0; r < RV; r++) part[wave][c][r][lane] = sum[c][r];
+    for (int r = 0; r < RV; r++) lds.part[wave][c][r][lane] = sum[c][r];
   __syncthreads();
   for (int i = threadIdx.x; i < CT * RV * 64; i += 64 * kWaves) {
     const int c = i / (RV * 64), r = i / 64 % RV, l = i % 64;
     float v = 0.f;
 #pragma unroll
-    for (int w = 0; w < kWaves; w++) v += part[w][c][r][l];
+    for (int w = 0; w < kWaves; w++) v += lds.part[w][c][r][l];
     const int mm = m0 + l / 16 + 4 * r, nn = n0 + 16 * c + l % 16;
     if (mm < p.m && nn < p.n) p.y[static_cast<int64_t>(mm) * p.n + nn] = N::save(v);
   }
 }
 
-template <class N, int CT, int GS>
+template <class N, int W, int CT, int GS>
 void launch(const Args &p, hipStream_t s) {
   const dim3 grid(static_cast<unsigned>((p.n + 16 * CT - 1) / (16 * CT)),
                   static_cast<unsigned>((p.m + 15) / 16));
-  const dim3 block(64 * kWaves);
-  if (p.m <= 4) hipLaunchKernelGGL((matvec4_kernel<N, CT, GS, 1>), grid, block, 0, s, p);
-  else if (p.m <= 8) hipLaunchKernelGGL((matvec4_kernel<N, CT, GS, 2>), grid, block, 0, s, p);
-  else hipLaunchKernelGGL((matvec4_kernel<N, CT, GS, 4>), grid, block, 0, s, p);
+  const dim3 block(64 * W);
+  if (p.m <= 4) hipLaunchKernelGGL((matvec4_kernel<N, W, CT, GS, 1>), grid, block, 0, s, p);
+  else if (p.m <= 8) hipLaunchKernelGGL((matvec4_kernel<N, W, CT, GS, 2>), grid, block, 0, s, p);
+  else hipLaunchKernelGGL((matvec4_kernel<N, W, CT, GS, 4>), grid, block, 0, s, p);
 }
 
+template <class N, int W, int CT>
+void launch_group(const Args &p, int group, hipStream_t s) {
+  if (group == 32) launch<N, W, CT, 1>(p, s);
+  else if (group == 64) launch<N, W, CT, 2>(p, s);
+  else launch<N, W, CT, 4>(p, s);
+}
+
+// Waves and column tiles of a workgroup: the most columns (x is read and rearranged once for all of
+// them), then the fewest waves (each starts and ends a pipeline), that still make about 2048 waves,
+// eight for each CU.  One row, us: 28000 x 8192 g64 33 with (4 waves, 4 tiles), 35 (4, 2), 43
+// (8, 2), 42 (8, 1); 8192 x 8192 g128 19, 14, 12, 14; 4096 x 4096 g128 10.5, 7.6, 7.3, 6.2;
+// 16384 x 2048 g128 8.6, 7.3, 9.8, 10.7.
 template <class N>
 void launch_type(const Args &p, int group, hipStream_t s) {
-  const bool wide = p.m > 4 && p.n >= 64 * 128;
-  if (wide) {
-    if (group == 32) launch<N, 4, 1>(p, s);
-    else if (group == 64) launch<N, 4, 2>(p, s);
-    else launch<N, 4, 4>(p, s);
-  } else {
-    if (group == 32) launch<N, 1, 1>(p, s);
-    else if (group == 64) launch<N, 1, 2>(p, s);
-    else launch<N, 1, 4>(p, s);
-  }
+  const auto waves = [&](int w, int ct) { return (p.n + 16 * ct - 1) / (16 * ct) * w; };
+  if (waves(4, 4) >= 1700) launch_group<N, 4, 4>(p, group, s);
+  else if (waves(4, 2) >= 1700) launch_group<N, 4, 2>(p, group, s);
+  else if (waves(8, 2) >= 1700) launch_group<N, 8, 2>(p, group, s);
+  else launch_group<N, 8, 1>(p, group, s);
 }
 
 }  // namespace

@@ -25,24 +25,21 @@ def _inputs(m, n, k, group, dtype, dev, zeros=True, seed=0):
 
 
 def _weight(q, s, z, k, group):
-    q, s = q.cpu(), s.cpu().double()
-    w = torch.zeros(q.shape[0], 2 * q.shape[1], dtype=torch.float64)
+    w = torch.zeros(q.shape[0], 2 * q.shape[1], dtype=torch.float64, device=q.device)
     w[:, 0::2], w[:, 1::2] = (q % 16).double(), (q // 16).double()
-    out = torch.zeros(q.shape[0], k, dtype=torch.float64)
-    for j in range(k):
-        out[:, j] = (w[:, j] - (8.0 if z is None else z.cpu()[:, j // group].double())) * s[:, j // group]
-    return out
+    at = torch.arange(k, device=q.device) // group
+    return (w[:, :k] - (8.0 if z is None else z[:, at].double())) * s[:, at].double()
 
 
 def _check(y, x, q, s, z, group):
     k = x.shape[-1]
-    xd = x.detach().double().cpu().reshape(-1, k)
+    xd = x.detach().double().reshape(-1, k)
     ref = xd @ _weight(q, s, z, k, group).t()
-    at = torch.arange(k) // group
-    size = xd.abs() @ (32.0 * s.cpu().double()[:, at]).t()
+    at = torch.arange(k, device=x.device) // group
+    size = xd.abs() @ (32.0 * s.double()[:, at]).t()
     tol = (k / 32 + 48) * U * size
     tol = tol + torch.finfo(y.dtype).eps / 2 * (ref.abs() + tol) + torch.finfo(y.dtype).smallest_normal
-    got = y.double().cpu().reshape(ref.shape)
+    got = y.double().reshape(ref.shape)
     assert ((got - ref).abs() <= tol).all(), ((got - ref).abs() / tol).max().item()
 
 
@@ -61,8 +58,11 @@ def test_values(dev, dtype, group, m, n, k):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("m,n,k,group", [(1, 4097, 4100, 128), (3, 1001, 1500, 32), (7, 8200, 512, 64), (16, 9000, 1030, 32),
-                                         (12, 8193, 384, 128)])
+                                         (12, 8193, 384, 128), (2, 40, 17000, 32), (9, 33, 20001, 64), (4, 17, 18432, 256),
+                                         (3, 13700, 4500, 64), (16, 13700, 4224, 32), (5, 27300, 5000, 128),
+                                         (16, 27205, 270, 32), (1, 27200, 9000, 384), (33, 8200, 1100, 128)])
 def test_larger(m, n, k, group):
+    """Every shape of workgroup, waves with more steps than they keep scales for, a last group that ends early."""
     x, q, s, z = _inputs(m, n, k, group, torch.bfloat16, "cuda")
     _check(ops.matvec_int4(x, q, s, z, group), x, q, s, z, group)
 
@@ -116,7 +116,7 @@ def test_quantize(dev, symmetric, k):
     w[3] = w[3].abs() + 1
     q, s, z = ops.quantize_int4(w, 64, symmetric)
     assert q.shape == (7, (k + 1) // 2) and s.dtype == torch.bfloat16 and (z is None) == symmetric
-    kept = _weight(q, s, z, k, 64)
+    kept = _weight(q, s, z, k, 64).cpu()
     step = s.double().cpu()[:, torch.arange(k) // 64]
     off = (kept - w.double().cpu()).abs()
     # bf16 rounds the step by up to 2^-8 of it: 15 steps (7) end up to 15 / 256 of a step short
