@@ -446,57 +446,70 @@ __global__ __launch_bounds__(512) void tile_kernel(Work work) {
 // ---------------------------------------------------------------- few rows
 constexpr int kFewWaves = 8;
 
+// Eight values of a row from k0 on, zeros from k on.  The tensor ends at `end`: before it, what lies
+// behind the row may be read (and is masked).
+__device__ __forceinline__ u32x4 row_end(const uint16_t *row, int k0, int k, const uint16_t *end) {
+  u32x4 v = {0, 0, 0, 0};
+  if (k0 >= k) return v;
+  if (row + k0 + 8 <= end) {
+    __builtin_memcpy(&v, row + k0, 16);
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+      v[i] &= k0 + 2 * i + 1 < k ? 0xffffffffu : k0 + 2 * i < k ? 0xffffu : 0u;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+      if (k0 + i < k) v[i / 2] |= static_cast<uint32_t>(row[k0 + i]) << (16 * (i & 1));
+  }
+  return v;
+}
+
 // RT row tiles of 16, CT column tiles of 16 outputs.  The rows are read once per workgroup (from
-// the caches), the weights once.  A step is 64 k, for which a lane's two 16-byte loads of a weight
-// row are the halves of a 128-byte line across the four 16-lane groups.  The next step's weights
-// and rows are loaded before the current step is multiplied.
+// the caches), the weights once.  A step is 64 k: the 128 bytes of a row are loaded by eight
+// neighbouring lanes and fragments are formed through LDS, a 2 KB image of 16 rows each.  (Loads
+// in fragment order, 16 rows in 16 neighbouring lanes, cost the cache four times the lookups:
+// one CU took in 31 bytes a nanosecond that way.)  Two steps are in flight; their loads are
+// issued unconditionally (past the end the last step again), since a load under a condition would
+// make the compiler wait for all.
 template <class N, int RT, int CT>
 __global__ __launch_bounds__(64 * kFewWaves) void few_kernel(Args p) {
-  constexpr int H = kFewWaves / 2;
-  __shared__ float part[H][2 * CT * RT * 4][64];
+  constexpr int H = kFewWaves / 2, kImages = 2 * CT + RT;
+  union Shared {
+    u32x4 image[kFewWaves][kImages][128];
+    float part[H][2 * CT * RT * 4][64];
+  };
+  __shared__ Shared lds;
+  auto &part = lds.part;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int l16 = lane & 15, lq = lane >> 4;
+  const int r8 = lane / 8, c8 = lane % 8;  // row (of 8) and 16-byte chunk that this lane loads
   const int n0 = blockIdx.x * (16 * CT);
-  const uint16_t *w[2][CT], *xr[RT];
+  const uint16_t *row[kImages][2];  // Wg and Wu of each column tile, then the rows of x
 #pragma unroll
-  for (int c = 0; c < CT; c++) {
-    const int n = n0 + 16 * c + l16 < p.n ? n0 + 16 * c + l16 : p.n - 1;
+  for (int h = 0; h < 2; h++) {
 #pragma unroll
-    for (int i = 0; i < 2; i++) w[i][c] = p.b[i] + n * p.ldb[i];
-  }
+    for (int c = 0; c < CT; c++) {
+      const int n = n0 + 16 * c + 8 * h + r8 < p.n ? n0 + 16 * c + 8 * h + r8 : p.n - 1;
 #pragma unroll
-  for (int t = 0; t < RT; t++) {
-    const int row = 16 * t + l16 < p.m ? 16 * t + l16 : p.m - 1;  // copies of it are not stored
-    xr[t] = p.a + row * p.lda;
+      for (int i = 0; i < 2; i++) row[2 * c + i][h] = p.b[i] + n * p.ldb[i];
+    }
+#pragma unroll
+    for (int t = 0; t < RT; t++) {
+      const int m = 16 * t + 8 * h + r8 < p.m ? 16 * t + 8 * h + r8 : p.m - 1;
+      row[2 * CT + t][h] = p.a + m * p.lda;  // copies of the last row are not stored
+    }
   }
   const int steps = (p.k + 63) / 64, per = (steps + kFewWaves - 1) / kFewWaves;
   const int first = wave * per, last = first + per < steps ? first + per : steps;
+  const int whole = last * 64 <= p.k ? last : last - 1;  // steps that end inside their rows
   struct Step {
-    u32x4 w[2][2][CT], x[2][RT];
+    u32x4 v[kImages][2];
   };
-  const auto load = [&](const uint16_t *row, int k0, bool whole) {
-    u32x4 v = {0, 0, 0, 0};
-    if (whole || k0 + 8 <= p.k) {
-      __builtin_memcpy(&v, row + k0, 16);
-    } else {
-      uint32_t e[4] = {0, 0, 0, 0};
-      for (int i = 0; i < 8; i++)
-        if (k0 + i < p.k) e[i / 2] |= static_cast<uint32_t>(row[k0 + i]) << (16 * (i & 1));
-      v = u32x4{e[0], e[1], e[2], e[3]};
-    }
-    return v;
-  };
-  const auto fetch = [&](Step &s, int st, bool whole) {
+  const auto fetch = [&](Step &s, int st) {
 #pragma unroll
-    for (int h = 0; h < 2; h++) {
-      const int k0 = st * 64 + 32 * h + 8 * lq;
+    for (int j = 0; j < kImages; j++)
 #pragma unroll
-      for (int i = 0; i < 2; i++)
-#pragma unroll
-        for (int c = 0; c < CT; c++) s.w[h][i][c] = load(w[i][c], k0, whole);
-#pragma unroll
-      for (int t = 0; t < RT; t++) s.x[h][t] = load(xr[t], k0, whole);
-    }
+      for (int h = 0; h < 2; h++) __builtin_memcpy(&s.v[j][h], row[j][h] + st * 64 + 8 * c8, 16);
   };
   floatx4 acc[2][CT][RT];
 #pragma unroll
@@ -505,35 +518,61 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_kernel(Args p) {
     for (int c = 0; c < CT; c++)
 #pragma unroll
       for (int t = 0; t < RT; t++) acc[i][c][t] = floatx4{0.f, 0.f, 0.f, 0.f};
+  u32x4 *image = &lds.image[wave][0][0];
   const auto multiply = [&](const Step &s) {
+    // LDS works in order within a wave: the reads see these writes, and the next step's writes
+    // come after them
 #pragma unroll
-    for (int h = 0; h < 2; h++)
+    for (int j = 0; j < kImages; j++)
+#pragma unroll
+      for (int h = 0; h < 2; h++)
+        image[128 * j + 8 * (8 * h + r8) + swz(8 * h + r8, c8)] = s.v[j][h];
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      const int at = 8 * l16 + swz(l16, 4 * h + lq);
+      u32x4 w[2 * CT], x[RT];
+#pragma unroll
+      for (int j = 0; j < 2 * CT; j++) w[j] = image[128 * j + at];
+#pragma unroll
+      for (int t = 0; t < RT; t++) x[t] = image[128 * (2 * CT + t) + at];
 #pragma unroll
       for (int t = 0; t < RT; t++)
 #pragma unroll
         for (int i = 0; i < 2; i++)
 #pragma unroll
-          for (int c = 0; c < CT; c++) acc[i][c][t] = mma<N>(s.x[h][t], s.w[h][i][c], acc[i][c][t]);
+          for (int c = 0; c < CT; c++) acc[i][c][t] = mma<N>(x[t], w[2 * c + i], acc[i][c][t]);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
   };
-  // whole steps two at a time, so neither step's registers are copied
-  const int whole = last * 64 <= p.k ? last : last - 1;
-  Step s0, s1;
-  int st = first;
-  if (st < whole) fetch(s0, st, true);
-  for (; st + 1 < whole; st += 2) {
-    fetch(s1, st + 1, true);
-    multiply(s0);
-    if (st + 2 < whole) fetch(s0, st + 2, true);
-    multiply(s1);
+  if (first < whole) {
+    Step v[2];
+#pragma unroll
+    for (int u = 0; u < 2; u++) fetch(v[u], first + u < whole ? first + u : whole - 1);
+    int st = first;
+    for (; st + 2 <= whole; st += 2)
+#pragma unroll
+      for (int u = 0; u < 2; u++) {
+        multiply(v[u]);
+        fetch(v[u], st + u + 2 < whole ? st + u + 2 : whole - 1);
+      }
+    if (st < whole) multiply(v[0]);
   }
-  if (st < whole) {
-    multiply(s0);
-    st++;
+  if (first < last && whole < last) {  // the rows end inside the last step
+    Step t;
+    const int k0 = whole * 64 + 8 * c8;
+    const uint16_t *end[3] = {p.b[0] + (p.n - 1) * p.ldb[0] + p.k, p.b[1] + (p.n - 1) * p.ldb[1] + p.k,
+                              p.a + (p.m - 1) * p.lda + p.k};
+#pragma unroll
+    for (int j = 0; j < kImages; j++)
+#pragma unroll
+      for (int h = 0; h < 2; h++)
+        t.v[j][h] = row_end(row[j][h], k0, p.k, end[j < 2 * CT ? j % 2 : 2]);
+    multiply(t);
   }
-  if (st < last) {
-    fetch(s0, st, false);
-    multiply(s0);
-  }
+  __syncthreads();  // the images make room for the sums
   // waves 4..7 add to waves 0..3, and those four are added in order
   const auto slot = [&](int i, int c, int t, int r) { return ((i * CT + c) * RT + t) * 4 + r; };
 #pragma unroll
@@ -868,18 +907,18 @@ void launch_few_as(const Args &p, hipStream_t s) {
 }
 
 // Column tiles of few_kernel for up to kFewRows rows; 0: the tile kernel is faster.  One CU takes in
-// about 31 bytes a nanosecond of weights and rows this way (8192 x 16384 at 64 rows: 132 us with two
-// column tiles, 185 with one), workgroups of two column tiles one at a time.  The tile kernel moves
-// more bytes at once but fills the chip only with many outputs (33 rows of 4096 x 10240: 42 us
-// against 53; of 2048 x 2048: 20 against 11).
+// about 40 bytes a nanosecond of weights and rows this way and the chip about 5.5 TB/s of weights;
+// workgroups of two column tiles run one at a time.  us at 48 rows with one tile, two tiles and the
+// tile kernel: 8192 x 16384 114, 98, 125; 2048 x 6144 19, 17, 22; 4096 x 10240 46, 50, 42;
+// 4096 x 4096 17, 23, 36.
 int few_columns(const Args &p, bool all_direct) {
   const int rt = (p.m + 15) / 16;
   if (rt == 1) return 1;
-  const double cu = device_cu_count();
+  const double cu = device_cu_count(), memory = 4.0 * p.n * p.k / 5.5e6;
   const auto few = [&](int ct) {
     const double groups = (p.n + 16 * ct - 1) / (16 * ct) / cu;
     const double rounds = ct == 2 ? std::ceil(groups) : std::max(1.0, groups);
-    return 2 + rounds * (64.0 * ct + 32.0 * rt) * p.k / 31e3;
+    return 3 + std::max(memory, rounds * (64.0 * ct + 32.0 * rt) * p.k / 40e3);
   };
   const double one = few(1), two = few(2);
   const double tile = 5 + std::max(estimate<Cfg<2, 1, true>>(&p, 1), 4.0 * p.n * p.k / 4.6e6);

@@ -280,25 +280,37 @@ __global__ __launch_bounds__(64 * kWaves) void matvec4_kernel(Args p) {
     for (int u = 0; u < kDepth - 1; u++)  // the last steps of the wave
       if (i + u < end) multiply(v[u], i + u - kb);
     if (whole < last && last - kb <= kStage) {  // the row ends inside the last step
+      // Bytes of q behind a row may be read where the tensor goes on (x is zero there).
       Step t;
-      const int k0 = whole * kBlock;
+      const int o = whole * (kBlock / 2) + 16 * c4;
+      const uint8_t *qend = p.q + (p.n - 1) * p.ldq + bytes;
+      const uint16_t *xend = p.x + (p.m - 1) * p.ldx + p.k;
 #pragma unroll
       for (int c = 0; c < CT; c++) {
-        uint32_t w[4] = {0, 0, 0, 0};
-        const int o = k0 / 2 + 16 * c4;
+        t.q[c] = u32x4{0, 0, 0, 0};
+        if (qr[c] + o + 16 <= qend) {
+          __builtin_memcpy(&t.q[c], qr[c] + o, 16);
+        } else {
 #pragma unroll
-        for (int e = 0; e < 16; e++)
-          if (o + e < bytes) w[e / 4] |= static_cast<uint32_t>(qr[c][o + e]) << (8 * (e & 3));
-        t.q[c] = u32x4{w[0], w[1], w[2], w[3]};
+          for (int e = 0; e < 16; e++)
+            if (o + e < bytes) t.q[c][e / 4] |= static_cast<uint32_t>(qr[c][o + e]) << (8 * (e & 3));
+        }
       }
 #pragma unroll
       for (int j = 0; j < 4; j++) {
-        uint32_t w[4] = {0, 0, 0, 0};
-        const int o = k0 + 32 * j + 8 * c4;
+        const int k0 = whole * kBlock + 32 * j + 8 * c4;
+        t.x[j] = u32x4{0, 0, 0, 0};
+        if (k0 >= p.k) continue;
+        if (xr + k0 + 8 <= xend) {
+          __builtin_memcpy(&t.x[j], xr + k0, 16);
 #pragma unroll
-        for (int e = 0; e < 8; e++)
-          if (o + e < p.k) w[e / 2] |= static_cast<uint32_t>(xr[o + e]) << (16 * (e & 1));
-        t.x[j] = u32x4{w[0], w[1], w[2], w[3]};
+          for (int e = 0; e < 4; e++)
+            t.x[j][e] &= k0 + 2 * e + 1 < p.k ? 0xffffffffu : k0 + 2 * e < p.k ? 0xffffu : 0u;
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; e++)
+            if (k0 + e < p.k) t.x[j][e / 2] |= static_cast<uint32_t>(xr[k0 + e]) << (16 * (e & 1));
+        }
       }
       multiply(t, whole - kb);
     }
