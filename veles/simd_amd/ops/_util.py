@@ -17,9 +17,31 @@ def stream_of(t: torch.Tensor) -> ctypes.c_void_p:
     return ctypes.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
 
 
-def raw_stream(t: torch.Tensor) -> int:
-    """Handle of t's device's current stream."""
-    return torch._C._cuda_getCurrentRawStream(t.device.index)
+_ENTRIES: dict = {}
+_get_device = getattr(torch._C, "_cuda_getDevice", None)
+_get_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def launch(t: torch.Tensor, name: str, *args) -> None:
+    """Call the vs_* function `name` with `args` and, as the last argument, the current stream of
+    t's GPU, with that GPU as the current device.  Bound functions are kept and the device is only
+    switched where it has to be: in a decoding loop the host's time per call counts."""
+    fn = _ENTRIES.get(name)
+    if fn is None:
+        require_gpu_tensor(t, name)
+        fn = _ENTRIES[name] = getattr(_lib.lib(), name)
+    dev = t.get_device()
+    if _get_device() != dev:
+        with torch.cuda.device(dev):
+            return _lib.call(name, *args, _get_stream(dev))
+    if _lib._RANGES:
+        return _lib.call(name, *args, _get_stream(dev))
+    status = fn(*args, _get_stream(dev))
+    if status:
+        _lib.check(status, name)
+
+
+_PLAIN = (torch.Tensor, torch.nn.Parameter)
 
 
 def plain_call(*tensors) -> bool:
@@ -31,8 +53,7 @@ def plain_call(*tensors) -> bool:
         return False
     grad = torch.is_grad_enabled()
     for t in tensors:
-        if t is not None and (type(t) not in (torch.Tensor, torch.nn.Parameter)
-                              or (grad and t.requires_grad)):
+        if t is not None and (type(t) not in _PLAIN or (grad and t.requires_grad)):
             return False
     return True
 

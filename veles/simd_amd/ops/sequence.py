@@ -8,13 +8,13 @@ from __future__ import annotations
 import torch
 
 from .. import _lib
-from ._util import on_device, plain_call, ptr, raw_stream, require_gpu_tensor
+from ._util import launch, plain_call
 
 DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 5}
 
 
 def _opt(t):
-    return None if t is None else ptr(t)
+    return None if t is None else t.data_ptr()
 
 
 def _rows_last(t: torch.Tensor) -> torch.Tensor:
@@ -26,6 +26,10 @@ def _same_device(name, first, **others):
     for n, t in others.items():
         if t is not None and t.device != first.device:
             raise ValueError(f"{name}: {n} is on {t.device}, x on {first.device}")
+
+
+def _new(x: torch.Tensor, *shape) -> torch.Tensor:
+    return torch.empty(shape, dtype=x.dtype, device=x.device)
 
 
 # ------------------------------------------------------- gated recurrence
@@ -76,8 +80,7 @@ def _recurrence_cpu(x, gate, state, lengths, save):
         h = torch.where(on[s][:, None], h + i[:, s] * (xd[:, s] - h), h)
         y[:, s] = torch.where(on[s][:, None], h, 0.0)
     # the CPU backward starts from the initial state: one tile
-    starts = (torch.zeros(b, d) if state is None else state)[:, None].clone() if save else x.new_empty(
-        0, dtype=torch.float32)
+    starts = (torch.zeros(b, d) if state is None else state)[:, None].clone() if save else None
     return y.to(x.dtype), h.float(), starts
 
 
@@ -85,20 +88,18 @@ def _recurrence_impl(x, gate, state, lengths, save):
     _check_recurrence("veles::gated_recurrence", x, gate, state, lengths)
     if not x.is_cuda:
         return _recurrence_cpu(x, gate, state, lengths, save)
-    require_gpu_tensor(x, "veles::gated_recurrence")
     b, t, d = x.shape
     x, gate = _rows_last(x), _rows_last(gate)
     state = None if state is None else state.contiguous()
     lengths = None if lengths is None else lengths.contiguous()
     y = torch.empty((b, t, d), dtype=x.dtype, device=x.device)
     final = torch.empty((b, d), dtype=torch.float32, device=x.device)
-    starts = torch.empty((b, _tiles(t), d) if save else (0,), dtype=torch.float32, device=x.device)
+    starts = torch.empty((b, _tiles(t), d), dtype=torch.float32, device=x.device) if save else None
     ws = _recurrence_workspace(x)
-    with on_device(x):
-        _lib.call("vs_gated_recurrence", DTYPES[x.dtype], ptr(x), x.stride(0), x.stride(1), ptr(gate),
-                  gate.stride(0), gate.stride(1), _opt(state), _opt(lengths),
-                  int(lengths is not None and lengths.dtype == torch.int64), b, t, d, ptr(y), ptr(final),
-                  ptr(starts) if save else None, _opt(ws), 0 if ws is None else ws.numel(), raw_stream(x))
+    launch(x, "vs_gated_recurrence", DTYPES[x.dtype], x.data_ptr(), x.stride(0), x.stride(1), gate.data_ptr(),
+           gate.stride(0), gate.stride(1), _opt(state), _opt(lengths),
+           int(lengths is not None and lengths.dtype == torch.int64), b, t, d, y.data_ptr(), final.data_ptr(),
+           _opt(starts), _opt(ws), 0 if ws is None else ws.numel())
     return y, final, starts
 
 
@@ -136,7 +137,6 @@ def _recurrence_backward_impl(x, gate, lengths, starts, dy, dfinal):
         raise ValueError(f"{name}: saved states {tuple(starts.shape)}, {want} expected")
     if not x.is_cuda:
         return _recurrence_backward_cpu(x, gate, lengths, starts, dy, dfinal)
-    require_gpu_tensor(x, name)
     x, gate = _rows_last(x), _rows_last(gate)
     dy = None if dy is None else _rows_last(dy)
     dfinal = None if dfinal is None else dfinal.contiguous()
@@ -146,12 +146,11 @@ def _recurrence_backward_impl(x, gate, lengths, starts, dy, dfinal):
     dg = torch.empty_like(dx)
     dstate = torch.empty((b, d), dtype=torch.float32, device=x.device)
     ws = _recurrence_workspace(x)
-    with on_device(x):
-        _lib.call("vs_gated_recurrence_backward", DTYPES[x.dtype], ptr(x), x.stride(0), x.stride(1),
-                  ptr(gate), gate.stride(0), gate.stride(1), _opt(lengths),
-                  int(lengths is not None and lengths.dtype == torch.int64), ptr(starts), _opt(dy),
-                  0 if dy is None else dy.stride(0), 0 if dy is None else dy.stride(1), _opt(dfinal), b, t, d,
-                  ptr(dx), ptr(dg), ptr(dstate), _opt(ws), 0 if ws is None else ws.numel(), raw_stream(x))
+    launch(x, "vs_gated_recurrence_backward", DTYPES[x.dtype], x.data_ptr(), x.stride(0), x.stride(1),
+           gate.data_ptr(), gate.stride(0), gate.stride(1), _opt(lengths),
+           int(lengths is not None and lengths.dtype == torch.int64), starts.data_ptr(), _opt(dy),
+           0 if dy is None else dy.stride(0), 0 if dy is None else dy.stride(1), _opt(dfinal), b, t, d,
+           dx.data_ptr(), dg.data_ptr(), dstate.data_ptr(), _opt(ws), 0 if ws is None else ws.numel())
     return dx, dg, dstate
 
 
@@ -181,6 +180,14 @@ def _recurrence_grad(ctx, dy, dfinal, _):
     return dx if need[0] else None, dg if need[1] else None, dstate if need[2] else None, None, None
 
 
+def _with_empty(impl):
+    """impl for the dispatcher: what is not saved (None, last) becomes an empty float32 tensor."""
+    def op(x, *args):
+        *out, saved = impl(x, *args)
+        return (*out, x.new_empty(0, dtype=torch.float32) if saved is None else saved)
+    return op
+
+
 def _no_second_derivative(name):
     def setup(ctx, inputs, output):
         pass
@@ -192,7 +199,7 @@ def _no_second_derivative(name):
 
 torch.library.define("veles::gated_recurrence",
                      "(Tensor x, Tensor gate, Tensor? state, Tensor? lengths, bool save) -> (Tensor, Tensor, Tensor)")
-torch.library.impl("veles::gated_recurrence", "default", _recurrence_impl)
+torch.library.impl("veles::gated_recurrence", "default", _with_empty(_recurrence_impl))
 torch.library.register_fake("veles::gated_recurrence", _recurrence_fake)
 torch.library.register_autograd("veles::gated_recurrence", _recurrence_grad, setup_context=_recurrence_setup)
 torch.library.define("veles::gated_recurrence_backward",
@@ -229,24 +236,29 @@ def gated_recurrence(x: torch.Tensor, gate: torch.Tensor, state: torch.Tensor | 
     return y, final
 
 
-def _step_impl(x, gate, state):
+def _check_step(x, gate, state):
     name = "veles::gated_recurrence_step"
-    if x.dim() != 2:
-        raise ValueError(f"{name}: x and gate are [batch, channels]; got {tuple(x.shape)}")
-    if gate.dim() != 2:
-        raise ValueError(f"{name}: x and gate are [batch, channels]; got {tuple(gate.shape)}")
+    for t in (x, gate):
+        if t.dim() != 2:
+            raise ValueError(f"{name}: x and gate are [batch, channels]; got {tuple(t.shape)}")
     _check_recurrence(name, x[:, None], gate[:, None], state, None)
     if not state.is_contiguous():
         raise ValueError(f"{name}: the state is updated in place and has to be contiguous")
+
+
+def _step_impl(x, gate, state):
+    # the usual case in one expression; _check_step names what is wrong otherwise
+    if not (x.dim() == 2 and x.shape == gate.shape == state.shape and x.dtype is gate.dtype
+            and x.dtype in DTYPES and state.dtype is torch.float32 and state.is_contiguous()
+            and x.device == gate.device == state.device):
+        _check_step(x, gate, state)
     if not x.is_cuda:
         state += torch.sigmoid(-gate.double()) * (x.double() - state)
         return state.to(x.dtype, copy=True)
-    require_gpu_tensor(x, name)
     x, gate = _rows_last(x), _rows_last(gate)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    with on_device(x):
-        _lib.call("vs_gated_recurrence_step", DTYPES[x.dtype], ptr(x), x.stride(0), ptr(gate), gate.stride(0),
-                  ptr(state), x.shape[0], x.shape[1], ptr(y), raw_stream(x))
+    y = _new(x, *x.shape)
+    launch(x, "vs_gated_recurrence_step", DTYPES[x.dtype], x.data_ptr(), x.stride(0), gate.data_ptr(),
+           gate.stride(0), state.data_ptr(), x.shape[0], x.shape[1], y.data_ptr())
     return y
 
 
@@ -285,9 +297,9 @@ def _check_matvec(name, x, qweight, scales, zeros, group_size):
     groups = (n, -(-k // group_size))
     if scales.dtype != x.dtype:
         raise TypeError(f"{name}: scales are {scales.dtype}, x {x.dtype}")
-    if tuple(scales.shape) != groups:
+    if scales.shape != groups:
         raise ValueError(f"{name}: scales {tuple(scales.shape)}, {groups} expected")
-    if zeros is not None and (zeros.dtype != torch.uint8 or tuple(zeros.shape) != groups):
+    if zeros is not None and (zeros.dtype != torch.uint8 or zeros.shape != groups):
         raise ValueError(f"{name}: zeros {zeros.dtype} {tuple(zeros.shape)}, uint8 {groups} expected")
     if n > 1 and k > 2 and qweight.stride(1) != 1:
         raise ValueError(f"{name}: the bytes of a row of qweight have to be neighbours")
@@ -303,14 +315,12 @@ def _matvec_impl(x, qweight, scales, zeros, group_size):
         at = torch.arange(k) // group_size
         z = 8.0 if zeros is None else zeros.double()[:, at]
         return (x.double() @ ((q - z) * scales.double()[:, at]).t()).to(x.dtype)
-    require_gpu_tensor(x, name)
     rows = _as_rows(x)
-    y = torch.empty((*x.shape[:-1], n), dtype=x.dtype, device=x.device)
+    y = _new(x, *x.shape[:-1], n)
     scales = scales.contiguous()
     zeros = None if zeros is None else zeros.contiguous()
-    with on_device(x):
-        _lib.call("vs_matvec_int4", DTYPES[x.dtype], ptr(rows), rows.stride(0), ptr(qweight), qweight.stride(0),
-                  ptr(scales), _opt(zeros), group_size, rows.shape[0], n, k, ptr(y), raw_stream(x))
+    launch(x, "vs_matvec_int4", DTYPES[x.dtype], rows.data_ptr(), rows.stride(0), qweight.data_ptr(),
+           qweight.stride(0), scales.data_ptr(), _opt(zeros), group_size, rows.shape[0], n, k, y.data_ptr())
     return y
 
 
@@ -435,17 +445,17 @@ def _gated_impl(x, w_gate, w_up, activation, save):
     if not x.is_cuda:
         g, u = rows.double() @ w_gate.double().t(), rows.double() @ w_up.double().t()
         h = (_act_cpu(activation, g) * u).to(x.dtype).view(*x.shape[:-1], f)
-        return h, (torch.stack([g, u], -1).float() if save else x.new_empty(0, dtype=torch.float32))
-    require_gpu_tensor(x, name)
+        return h, torch.stack([g, u], -1).float() if save else None
     w_gate, w_up = _weight_rows(w_gate), _weight_rows(w_up)
-    h = torch.empty((*x.shape[:-1], f), dtype=x.dtype, device=x.device)
-    pre = torch.empty((m, f, 2) if save else (0,), dtype=torch.float32, device=x.device)
-    size = int(_lib.lib().vs_gated_linear_workspace(m, f, k))
-    ws = torch.empty(size, dtype=torch.uint8, device=x.device) if size and not _aligned(rows, w_gate, w_up) else None
-    with on_device(x):
-        _lib.call("vs_gated_linear", DTYPES[x.dtype], ACTIVATIONS[activation], ptr(rows), rows.stride(0), ptr(w_gate),
-                  w_gate.stride(0), ptr(w_up), w_up.stride(0), m, f, k, ptr(h), ptr(pre) if save else None, _opt(ws),
-                  0 if ws is None else size, raw_stream(x))
+    h = _new(x, *x.shape[:-1], f)
+    pre = torch.empty((m, f, 2), dtype=torch.float32, device=x.device) if save else None
+    size, ws = 0, None
+    if not _aligned(rows, w_gate, w_up):
+        size = int(_lib.lib().vs_gated_linear_workspace(m, f, k))
+        ws = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
+    launch(x, "vs_gated_linear", DTYPES[x.dtype], ACTIVATIONS[activation], rows.data_ptr(), rows.stride(0),
+           w_gate.data_ptr(), w_gate.stride(0), w_up.data_ptr(), w_up.stride(0), m, f, k, h.data_ptr(),
+           _opt(pre), _opt(ws), size)
     return h, pre
 
 
@@ -471,16 +481,15 @@ def _gated_backward_impl(x, w_gate, w_up, pre, dh, activation, want_dx, want_dw)
         dx = (dg @ w_gate.double() + du @ w_up.double()).to(x.dtype).view(x.shape) if want_dx else x.new_empty(0)
         dw = torch.cat([dg.t() @ rows.double(), du.t() @ rows.double()]).to(x.dtype) if want_dw else x.new_empty(0)
         return dx, dw
-    require_gpu_tensor(x, name)
     w_gate, w_up, pre = _weight_rows(w_gate), _weight_rows(w_up), pre.contiguous()
     dx = torch.empty(x.shape if want_dx else (0,), dtype=x.dtype, device=x.device)
     dw = torch.empty((2 * f, k) if want_dw else (0,), dtype=x.dtype, device=x.device)
     size = int(_lib.lib().vs_gated_linear_backward_workspace(m, f, k, int(want_dx), int(want_dw)))
     ws = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
-    with on_device(x):
-        _lib.call("vs_gated_linear_backward", DTYPES[x.dtype], ACTIVATIONS[activation], ptr(rows), rows.stride(0),
-                  ptr(w_gate), w_gate.stride(0), ptr(w_up), w_up.stride(0), ptr(pre), ptr(dhr), dhr.stride(0), m, f, k,
-                  ptr(dx) if want_dx else None, ptr(dw) if want_dw else None, _opt(ws), size, raw_stream(x))
+    launch(x, "vs_gated_linear_backward", DTYPES[x.dtype], ACTIVATIONS[activation], rows.data_ptr(),
+           rows.stride(0), w_gate.data_ptr(), w_gate.stride(0), w_up.data_ptr(), w_up.stride(0), pre.data_ptr(),
+           dhr.data_ptr(), dhr.stride(0), m, f, k, dx.data_ptr() if want_dx else None,
+           dw.data_ptr() if want_dw else None, _opt(ws), size)
     return dx, dw
 
 
@@ -515,7 +524,7 @@ def _gated_grad(ctx, dh, _):
 
 torch.library.define("veles::gated_linear",
                      "(Tensor x, Tensor w_gate, Tensor w_up, str activation, bool save) -> (Tensor, Tensor)")
-torch.library.impl("veles::gated_linear", "default", _gated_impl)
+torch.library.impl("veles::gated_linear", "default", _with_empty(_gated_impl))
 torch.library.register_fake("veles::gated_linear", _gated_fake)
 torch.library.register_autograd("veles::gated_linear", _gated_grad, setup_context=_gated_setup)
 torch.library.define("veles::gated_linear_backward",
