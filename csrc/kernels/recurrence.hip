@@ -15,17 +15,20 @@
 // of steps is one map too, and runs compose: (a2, b2) o (a1, b1) = (a2 a1, a2 b1 + b2).
 //
 // Bound: bandwidth.  Forward reads x and g and writes y; backward reads x, g, dy and writes
-// dx, dg.  The split that keeps it to one pass over the data: a workgroup owns 64 V channels of
-// one sequence and walks time in tiles of W x L steps, wave w the L steps from w L on.  A wave
-// reduces its steps to one map per channel, the W maps meet in LDS (one barrier a tile, two
-// images in turn), every wave composes them to its own initial state, and the steps run again
-// from registers.  The next tile's loads are issued before the tile is worked on.  The state
-// never leaves fp32 registers.  Backward recomputes h from the state at the start of each tile,
-// which the forward pass keeps (4 bytes per channel and tile, 1/32 to 1/64 of a read of y).
+// dx, dg.  The split that keeps it to one pass over the data: a workgroup works on a tile of W x L
+// steps of 64 V channels, wave w on L of them.  A wave reduces its steps to one map per channel,
+// the W maps meet in LDS, every wave composes them to its own initial state, and the steps run
+// again from registers.  The state never leaves fp32.  Backward recomputes h from the state at the
+// start of each tile, which the forward pass keeps (4 bytes per channel and tile, 1/64 of a read
+// of y in 16 bits).
 //
-// Few sequences and channels leave most of the chip idle, so time is cut into segments then: a
-// first kernel computes each segment's map (two of the three or five streams are read twice),
-// and the second composes the maps before its own segment.
+// Between tiles the maps pass through memory: a tile publishes its map as soon as it has it, and
+// composes its initial state from the maps of the tiles before it in its run of kRun tiles and the
+// state at the start of the run, which the last tile of the run before publishes.  What is composed
+// with what does not depend on timing, so results are the same bits every time.  Measured against
+// a workgroup that walks the tiles of its channels (forward, us): 1 x 65536 x 1024 fp32 164 against
+// 2017 (295 with time cut into segments whose maps a first kernel computes, which reads x and g
+// twice), 4 x 4096 x 4096 bf16 100 against 136, 8 x 2048 x 8192 bf16 173 against 186.
 // Copyright 2026 veles.simd_amd authors. Apache-2.0.
 #include <hip/hip_runtime.h>
 
@@ -52,10 +55,13 @@ struct Args {
   void *y, *dx, *dg;                 // [batch][t][d]
   float *final, *dstate;             // [batch][d]
   float *starts;                     // [batch][tiles][d]: state at the start of each tile, or null
-  float *maps;                       // [batch][segs][2][d]: the segments' maps
-  int64_t t, tiles, seg_tiles;       // steps; tiles in all; tiles per segment
-  int64_t b0;                        // first sequence of this launch
-  int d, slabs, segs;
+  uint64_t *maps;                    // [batch][tiles][d]: a tile's map (product low, sum high)
+  uint32_t *heads;                   // [batch][runs][d]: what enters a run of tiles
+  uint32_t *ticket;                  // null where a sequence is one tile
+  int64_t t, tiles;                  // steps, tiles
+  int64_t group0;                    // first group (sequence and slab of 64 V channels) of this launch
+  unsigned groups;                   // groups of this launch
+  int d, slabs;
 };
 
 __device__ __forceinline__ int64_t steps_of(const Args &p, int64_t b) {
@@ -110,94 +116,14 @@ struct Shape {
     for (int v = 0; v < V; v++) z.set(v, 0.f);
     return z;
   }
-};
 
-// Carries `s` through the maps of `count` segments from `from` on (step +1 or -1).  Each wave
-// composes its share of them, eight loads in flight, and the W results meet in LDS.
-template <int V, int W>
-__device__ __forceinline__ void compose(const Args &p, int64_t b, int c, int lane, int wave, int from,
-                                        int count, int step, float (&la)[W][64 * V],
-                                        float (&le)[W][64 * V], float (&s)[V]) {
-  const int per = (count + W - 1) / W;
-  const int lo = wave * per, hi = lo + per < count ? lo + per : count;
-  float a[V], e[V];
-#pragma unroll
-  for (int v = 0; v < V; v++) {
-    a[v] = 1.f;
-    e[v] = 0.f;
-  }
-#pragma unroll 8
-  for (int j = lo; j < hi; j++) {
-    const float *m = p.maps + (b * p.segs + from + step * j) * 2 * p.d + c;
-#pragma unroll
-    for (int v = 0; v < V; v++) {
-      e[v] = fmaf(m[v], e[v], m[p.d + v]);
-      a[v] *= m[v];
+  // Shares of the wave's steps and their map: product a, end e from a zero state.
+  __device__ __forceinline__ static void forward_map(P (&x)[L], P (&g)[L], int64_t t, int64_t len,
+                                                     float (&i)[L][V], float (&a)[V], float (&e)[V]) {
+    if (t + L > len) {
+      blank(x, t, len, 0.f);
+      blank(g, t, len, __builtin_inff());
     }
-  }
-#pragma unroll
-  for (int v = 0; v < V; v++) {
-    la[wave][lane * V + v] = a[v];
-    le[wave][lane * V + v] = e[v];
-  }
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < W; w++)
-#pragma unroll
-    for (int v = 0; v < V; v++) s[v] = fmaf(la[w][lane * V + v], s[v], le[w][lane * V + v]);
-  __syncthreads();  // the images are free again
-}
-
-// ---------------------------------------------------------------- forward
-// OUT: the whole pass; else only the segments' maps.
-template <class N, int V, int W, int L, bool OUT>
-__global__ __launch_bounds__(64 * W) void forward_kernel(Args p) {
-  using S = Shape<N, V, W, L>;
-  using P = typename S::P;
-  __shared__ float maps[2][2][W][S::kLanes];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t row = blockIdx.x / p.slabs, b = p.b0 + row;
-  const int slab = static_cast<int>(blockIdx.x - row * p.slabs);
-  const int seg = blockIdx.y;
-  const int c0 = slab * S::kLanes + lane * V;
-  const bool in = c0 < p.d;
-  const int c = in ? c0 : 0;
-  const int64_t len = steps_of(p, b);
-  const int64_t first = seg * p.seg_tiles;
-  const int64_t last = first + p.seg_tiles < p.tiles ? first + p.seg_tiles : p.tiles;
-
-  float ca[V], h0[V];  // the segment's map so far (not OUT) or the state (OUT)
-#pragma unroll
-  for (int v = 0; v < V; v++) {
-    ca[v] = 1.f;
-    h0[v] = OUT && p.state ? p.state[b * p.d + c + v] : 0.f;
-  }
-  if (OUT && p.segs > 1) compose<V, W>(p, b, c, lane, wave, 0, seg, 1, maps[0][0], maps[0][1], h0);
-
-  P x[L], g[L], nx[L], ng[L];
-  const int64_t mine = static_cast<int64_t>(wave) * L;
-  if (first * S::kTile < len) {
-    S::load(x, p.x, b * p.xb, p.xt, c, first * S::kTile + mine, len);
-    S::load(g, p.g, b * p.gb, p.gt, c, first * S::kTile + mine, len);
-  }
-  for (int64_t tile = first; tile < last; tile++) {
-    const int64_t t0 = tile * S::kTile + mine;
-    if (tile * S::kTile >= len) {  // padding only (the same for the whole workgroup)
-      if (OUT && in)
-        for (int s = 0; s < L; s++)
-          if (t0 + s < p.t) S::store(p.y, b * p.t + t0 + s, p.d, c, S::zero());
-      continue;
-    }
-    if (tile + 1 < last && (tile + 1) * S::kTile < len) {
-      S::load(nx, p.x, b * p.xb, p.xt, c, t0 + S::kTile, len);
-      S::load(ng, p.g, b * p.gb, p.gt, c, t0 + S::kTile, len);
-    }
-    const bool full = t0 + L <= len;
-    if (!full) {
-      S::blank(x, t0, len, 0.f);
-      S::blank(g, t0, len, __builtin_inff());
-    }
-    float i[L][V], a[V], e[V];
 #pragma unroll
     for (int v = 0; v < V; v++) {
       a[v] = 1.f;
@@ -211,139 +137,30 @@ __global__ __launch_bounds__(64 * W) void forward_kernel(Args p) {
         e[v] = fmaf(i[s][v], x[s][v] - e[v], e[v]);
         a[v] = fmaf(-i[s][v], a[v], a[v]);
       }
-    float (*m)[W][S::kLanes] = maps[tile & 1];
-#pragma unroll
-    for (int v = 0; v < V; v++) {
-      m[0][wave][lane * V + v] = a[v];
-      m[1][wave][lane * V + v] = e[v];
-    }
-    __syncthreads();
-    float h[V];
-    if (OUT && p.starts && wave == 0 && in)
-#pragma unroll
-      for (int v = 0; v < V; v++) p.starts[(b * p.tiles + tile) * p.d + c + v] = h0[v];
-#pragma unroll
-    for (int w = 0; w < W; w++)
-#pragma unroll
-      for (int v = 0; v < V; v++) {
-        const float ma = m[0][w][lane * V + v], me = m[1][w][lane * V + v];
-        if (w == wave) h[v] = h0[v];
-        h0[v] = fmaf(ma, h0[v], me);
-        if (!OUT) ca[v] *= ma;
-      }
-    if (OUT) {
-#pragma unroll
-      for (int s = 0; s < L; s++) {
-        P y;
-#pragma unroll
-        for (int v = 0; v < V; v++) {
-          h[v] = fmaf(i[s][v], x[s][v] - h[v], h[v]);
-          y.set(v, h[v]);
-        }
-        if (full ? in : in && t0 + s < p.t)
-          S::store(p.y, b * p.t + t0 + s, p.d, c, full || t0 + s < len ? y : S::zero());
-      }
-    }
+  }
+  // Runs the steps from state h and stores y.
+  __device__ __forceinline__ static void forward_steps(const Args &p, int64_t b, int c, bool in, bool full,
+                                                       int64_t t, int64_t len, const P (&x)[L],
+                                                       const float (&i)[L][V], float (&h)[V]) {
 #pragma unroll
     for (int s = 0; s < L; s++) {
-      x[s] = nx[s];
-      g[s] = ng[s];
-    }
-  }
-  if (wave != 0 || !in) return;
-  if (OUT) {
-    if (seg == p.segs - 1)
-#pragma unroll
-      for (int v = 0; v < V; v++) p.final[b * p.d + c + v] = h0[v];
-  } else {
-    float *m = p.maps + (b * p.segs + seg) * 2 * p.d + c;
-#pragma unroll
-    for (int v = 0; v < V; v++) {
-      m[v] = ca[v];
-      m[p.d + v] = h0[v];
-    }
-  }
-}
-
-// --------------------------------------------------------------- backward
-template <class N, int V, int W, int L, bool OUT>
-__global__ __launch_bounds__(64 * W) void backward_kernel(Args p) {
-  using S = Shape<N, V, W, L>;
-  using P = typename S::P;
-  __shared__ float maps[2][3][W][S::kLanes];  // product; forward end from zero; backward end from zero
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t row = blockIdx.x / p.slabs, b = p.b0 + row;
-  const int slab = static_cast<int>(blockIdx.x - row * p.slabs);
-  const int seg = blockIdx.y + (OUT ? 0 : 1);
-  const int c0 = slab * S::kLanes + lane * V;
-  const bool in = c0 < p.d;
-  const int c = in ? c0 : 0;
-  const int64_t len = steps_of(p, b);
-  const int64_t first = seg * p.seg_tiles;
-  const int64_t last = first + p.seg_tiles < p.tiles ? first + p.seg_tiles : p.tiles;
-
-  float ca[V], m0[V];
-#pragma unroll
-  for (int v = 0; v < V; v++) {
-    ca[v] = 1.f;
-    m0[v] = OUT && p.dfinal ? p.dfinal[b * p.d + c + v] : 0.f;
-  }
-  if (OUT && p.segs > 1)
-    compose<V, W>(p, b, c, lane, wave, p.segs - 1, p.segs - 1 - seg, -1, maps[0][0], maps[0][1], m0);
-
-  P x[L], g[L], dy[L], nx[L], ng[L], ndy[L];
-  float st[V], nst[V];
-#pragma unroll
-  for (int v = 0; v < V; v++) st[v] = nst[v] = 0.f;
-  const int64_t mine = static_cast<int64_t>(wave) * L;
-  const auto fetch = [&](int64_t tile, P (&fx)[L], P (&fg)[L], P (&fd)[L], float (&fs)[V]) {
-    const int64_t t = tile * S::kTile + mine;
-    if (OUT) {
-      S::load(fx, p.x, b * p.xb, p.xt, c, t, len);
-#pragma unroll
-      for (int v = 0; v < V; v++) fs[v] = p.starts[(b * p.tiles + tile) * p.d + c + v];
-    }
-    S::load(fg, p.g, b * p.gb, p.gt, c, t, len);
-    if (p.dy) S::load(fd, p.dy, b * p.yb, p.yt, c, t, len);
-  };
-  bool have = false;
-  for (int64_t tile = last - 1; tile >= first; tile--) {
-    const int64_t t0 = tile * S::kTile + mine;
-    if (tile * S::kTile >= len) {
-      if (OUT && in)
-        for (int s = 0; s < L; s++)
-          if (t0 + s < p.t) {
-            S::store(p.dx, b * p.t + t0 + s, p.d, c, S::zero());
-            S::store(p.dg, b * p.t + t0 + s, p.d, c, S::zero());
-          }
-      continue;
-    }
-    if (!have) {
-      fetch(tile, x, g, dy, st);
-      have = true;
-    }
-    if (tile > first) fetch(tile - 1, nx, ng, ndy, nst);
-    const bool full = t0 + L <= len;
-    if (!p.dy) S::blank(dy, 0, 0, 0.f);
-    if (!full) {
-      if (OUT) S::blank(x, t0, len, 0.f);
-      S::blank(g, t0, len, __builtin_inff());
-      S::blank(dy, t0, len, 0.f);
-    }
-    float i[L][V], a[V], e[V], q[V];
-#pragma unroll
-    for (int v = 0; v < V; v++) {
-      a[v] = 1.f;
-      e[v] = q[v] = 0.f;
-    }
-#pragma unroll
-    for (int s = 0; s < L; s++)
+      P y;
 #pragma unroll
       for (int v = 0; v < V; v++) {
-        i[s][v] = share(g[s][v]);
-        a[v] = fmaf(-i[s][v], a[v], a[v]);
-        if (OUT) e[v] = fmaf(i[s][v], x[s][v] - e[v], e[v]);
+        h[v] = fmaf(i[s][v], x[s][v] - h[v], h[v]);
+        y.set(v, h[v]);
       }
+      if (full ? in : in && t + s < p.t)
+        store(p.y, b * p.t + t + s, p.d, c, full || t + s < len ? y : zero());
+    }
+  }
+  // End q of the wave's steps backward from a zero m (the product is the forward one).
+  __device__ __forceinline__ static void backward_map(const Args &p, P (&dy)[L], int64_t t, int64_t len,
+                                                      const float (&i)[L][V], float (&q)[V]) {
+    if (!p.dy) blank(dy, 0, 0, 0.f);
+    else if (t + L > len) blank(dy, t, len, 0.f);
+#pragma unroll
+    for (int v = 0; v < V; v++) q[v] = 0.f;
 #pragma unroll
     for (int s = L - 1; s >= 0; s--)
 #pragma unroll
@@ -351,82 +168,297 @@ __global__ __launch_bounds__(64 * W) void backward_kernel(Args p) {
         const float l = q[v] + dy[s][v];
         q[v] = fmaf(-i[s][v], l, l);
       }
-    float (*m)[W][S::kLanes] = maps[tile & 1];
+  }
+  // Runs the steps forward from state h, then backward from m, and stores dx and dg.
+  __device__ __forceinline__ static void backward_steps(const Args &p, int64_t b, int c, bool in,
+                                                        bool full, int64_t t, int64_t len,
+                                                        const P (&x)[L], const P (&dy)[L],
+                                                        const float (&i)[L][V], float (&h)[V],
+                                                        float (&m)[V]) {
+    float before[L][V];  // h_{t-1} - x_t
+#pragma unroll
+    for (int s = 0; s < L; s++)
+#pragma unroll
+      for (int v = 0; v < V; v++) {
+        before[s][v] = h[v] - x[s][v];
+        h[v] = fmaf(-i[s][v], before[s][v], h[v]);
+      }
+#pragma unroll
+    for (int s = L - 1; s >= 0; s--) {
+      P ox, og;
+#pragma unroll
+      for (int v = 0; v < V; v++) {
+        const float l = m[v] + dy[s][v];
+        const float il = i[s][v] * l;
+        m[v] = l - il;
+        ox.set(v, il);
+        og.set(v, (1.f - i[s][v]) * il * before[s][v]);
+      }
+      if (full ? in : in && t + s < p.t) {
+        const bool on = full || t + s < len;
+        store(p.dx, b * p.t + t + s, p.d, c, on ? ox : zero());
+        store(p.dg, b * p.t + t + s, p.d, c, on ? og : zero());
+      }
+    }
+  }
+  __device__ __forceinline__ static void zero_gradients(const Args &p, int64_t b, int c, bool in,
+                                                        int64_t t) {
+    if (in)
+      for (int s = 0; s < L; s++)
+        if (t + s < p.t) {
+          store(p.dx, b * p.t + t + s, p.d, c, zero());
+          store(p.dg, b * p.t + t + s, p.d, c, zero());
+        }
+  }
+};
+
+// ------------------------------------------------------------------ chain
+// Workgroups take tiles by a counter, position by position along time (from the end in the backward
+// pass).  A tile waits for earlier positions only, which have lower numbers, and a workgroup takes
+// its number when it already runs: by induction over the numbers every wait ends.  Maps and
+// states are published and polled as single relaxed atomics at device scope, 64 or 32 bits that are
+// never all ones when they are valid (a NaN is stored as the canonical one), so no other memory has
+// to be ordered with them.  The buffers are set to all ones before the launch.
+constexpr int kRun = 16;
+constexpr uint32_t kNone = 0xffffffffu;
+constexpr int kPolls = 1 << 18;  // a fraction of a second; then a NaN goes on in place of what did not come
+
+__device__ __forceinline__ uint32_t bits(float f) {
+  return f == f ? __float_as_uint(f) : 0x7fc00000u;
+}
+
+struct Map {
+  float a, e;
+};
+__device__ __forceinline__ void publish(uint64_t *at, Map m) {
+  __hip_atomic_store(at, bits(m.a) | static_cast<uint64_t>(bits(m.e)) << 32, __ATOMIC_RELAXED,
+                     __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ Map await(uint64_t *at) {
+  for (int n = 0; n < kPolls; n++) {
+    const uint64_t v = __hip_atomic_load(at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (v != ~0ull) return Map{__uint_as_float(static_cast<uint32_t>(v)), __uint_as_float(v >> 32)};
+    __builtin_amdgcn_s_sleep(1);
+  }
+  return Map{__builtin_nanf(""), __builtin_nanf("")};
+}
+__device__ __forceinline__ void publish(uint32_t *at, float s) {
+  __hip_atomic_store(at, bits(s), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float await(uint32_t *at) {
+  for (int n = 0; n < kPolls; n++) {
+    const uint32_t v = __hip_atomic_load(at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (v != kNone) return __uint_as_float(v);
+    __builtin_amdgcn_s_sleep(1);
+  }
+  return __builtin_nanf("");
+}
+
+__global__ __launch_bounds__(256) void ones_kernel(uint4 *p, int64_t n) {
+  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll)
+    p[i] = uint4{kNone, kNone, kNone, kNone};
+}
+
+template <int V, int W>
+struct Chain {
+  static constexpr int kLanes = 64 * V;
+  float run[kRun - 1][2][kLanes];  // maps of the tiles before this one in its run
+  float head[kLanes];              // what enters the run
+  unsigned ticket;
+};
+
+// This workgroup's position along the chain, its sequence and its slab of channels.  (Workgroups that
+// stay and draw their next number while they work were slower, 194 us against 164 at
+// 1 x 65536 x 1024 fp32: the tiles behind wait for a number whose workgroup is not free yet.)
+struct Place {
+  int64_t pos, b;
+  int slab;
+};
+template <int V, int W>
+__device__ __forceinline__ Place take(const Args &p, Chain<V, W> &ch) {
+  unsigned t = blockIdx.x;
+  if (p.ticket) {
+    if (threadIdx.x == 0) ch.ticket = atomicAdd(p.ticket, 1u) + 1u;  // it starts at all ones
+    __syncthreads();
+    t = __builtin_amdgcn_readfirstlane(ch.ticket);
+  }
+  const unsigned pos = t / p.groups;
+  const int64_t group = p.group0 + (t - pos * p.groups), b = group / p.slabs;
+  return Place{pos, b, static_cast<int>(group - b * p.slabs)};
+}
+
+// Publishes this tile's map, and brings `s` to what enters the tile: `initial` at position 0.
+// False: a tile of padding that nothing waits for beyond its map.
+template <int V, int W>
+__device__ __forceinline__ bool enter(const Args &p, Chain<V, W> &ch, int64_t b, int64_t pos, int c,
+                                      bool in, int lane, int wave, bool live, const float *initial,
+                                      const float (&ta)[V], const float (&te)[V], float (&s)[V]) {
+  const int64_t runs = (p.tiles + kRun - 1) / kRun, q = pos / kRun;
+  const int before = static_cast<int>(pos - q * kRun);
+  const bool closes = before == kRun - 1 && pos + 1 < p.tiles, last = pos + 1 == p.tiles;
+  uint64_t *maps = p.maps + (b * p.tiles + pos) * p.d + c;
+  if (!closes && !last) {  // the state after those two goes on by itself
+    if (wave == 0 && in)
+#pragma unroll
+      for (int v = 0; v < V; v++) publish(maps + v, Map{ta[v], te[v]});
+    if (!live) return false;
+  }
+  for (int j = wave; j < before; j += W)
 #pragma unroll
     for (int v = 0; v < V; v++) {
-      m[0][wave][lane * V + v] = a[v];
-      m[1][wave][lane * V + v] = e[v];
-      m[2][wave][lane * V + v] = q[v];
+      Map m = {1.f, 0.f};
+      if (in) m = await(maps + v - static_cast<int64_t>(before - j) * p.d);
+      ch.run[j][0][lane * V + v] = m.a;
+      ch.run[j][1][lane * V + v] = m.e;
+    }
+  if (wave == W - 1)
+#pragma unroll
+    for (int v = 0; v < V; v++) {
+      float h = 0.f;
+      if (q == 0) h = initial ? initial[b * p.d + c + v] : 0.f;
+      else if (in) h = await(p.heads + (b * runs + q) * p.d + c + v);
+      ch.head[lane * V + v] = h;
+    }
+  __syncthreads();
+#pragma unroll
+  for (int v = 0; v < V; v++) s[v] = ch.head[lane * V + v];
+  for (int j = 0; j < before; j++)
+#pragma unroll
+    for (int v = 0; v < V; v++)
+      s[v] = fmaf(ch.run[j][0][lane * V + v], s[v], ch.run[j][1][lane * V + v]);
+  if (closes && wave == 0 && in)
+#pragma unroll
+    for (int v = 0; v < V; v++)
+      publish(p.heads + (b * runs + q + 1) * p.d + c + v, fmaf(ta[v], s[v], te[v]));
+  return true;
+}
+
+template <class N, int V, int W, int L>
+__global__ __launch_bounds__(64 * W) void forward_kernel(Args p) {
+  using S = Shape<N, V, W, L>;
+  using P = typename S::P;
+  __shared__ float maps[2][W][S::kLanes];
+  __shared__ Chain<V, W> ch;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const auto [pos, b, slab] = take(p, ch);
+  const int c0 = slab * S::kLanes + lane * V;
+  const bool in = c0 < p.d;
+  const int c = in ? c0 : 0;
+  const int64_t len = steps_of(p, b), t0 = pos * S::kTile + wave * L;
+  const bool live = pos * S::kTile < len, full = t0 + L <= len;
+  P x[L], g[L];
+  float i[L][V], ta[V], te[V], s[V];
+#pragma unroll
+  for (int v = 0; v < V; v++) {
+    ta[v] = 1.f;
+    te[v] = 0.f;
+  }
+  if (live) {
+    float a[V], e[V];
+    S::load(x, p.x, b * p.xb, p.xt, c, t0, len);
+    S::load(g, p.g, b * p.gb, p.gt, c, t0, len);
+    S::forward_map(x, g, t0, len, i, a, e);
+#pragma unroll
+    for (int v = 0; v < V; v++) {
+      maps[0][wave][lane * V + v] = a[v];
+      maps[1][wave][lane * V + v] = e[v];
     }
     __syncthreads();
-    float h[V], mm[V];
-    if (OUT) {
 #pragma unroll
-      for (int w = 0; w < W; w++)
+    for (int w = 0; w < W; w++)
 #pragma unroll
-        for (int v = 0; v < V; v++) {
-          if (w == wave) h[v] = st[v];
-          st[v] = fmaf(m[0][w][lane * V + v], st[v], m[1][w][lane * V + v]);
-        }
+      for (int v = 0; v < V; v++) {
+        te[v] = fmaf(maps[0][w][lane * V + v], te[v], maps[1][w][lane * V + v]);
+        ta[v] *= maps[0][w][lane * V + v];
+      }
+  }
+  if (!enter(p, ch, b, pos, c, in, lane, wave, live, p.state, ta, te, s)) {
+    if (in)
+      for (int k = 0; k < L; k++)
+        if (t0 + k < p.t) S::store(p.y, b * p.t + t0 + k, p.d, c, S::zero());
+    return;
+  }
+  if (wave == 0 && in)
+#pragma unroll
+    for (int v = 0; v < V; v++) {
+      if (live && p.starts) p.starts[(b * p.tiles + pos) * p.d + c + v] = s[v];
+      if (pos + 1 == p.tiles) p.final[b * p.d + c + v] = fmaf(ta[v], s[v], te[v]);
     }
+  if (!live) {
+    if (in)
+      for (int k = 0; k < L; k++)
+        if (t0 + k < p.t) S::store(p.y, b * p.t + t0 + k, p.d, c, S::zero());
+    return;
+  }
+  for (int w = 0; w < wave; w++)
+#pragma unroll
+    for (int v = 0; v < V; v++) s[v] = fmaf(maps[0][w][lane * V + v], s[v], maps[1][w][lane * V + v]);
+  S::forward_steps(p, b, c, in, full, t0, len, x, i, s);
+}
+
+template <class N, int V, int W, int L>
+__global__ __launch_bounds__(64 * W) void backward_kernel(Args p) {
+  using S = Shape<N, V, W, L>;
+  using P = typename S::P;
+  __shared__ float maps[3][W][S::kLanes];
+  __shared__ Chain<V, W> ch;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const auto [pos, b, slab] = take(p, ch);
+  const int64_t tile = p.tiles - 1 - pos;
+  const int c0 = slab * S::kLanes + lane * V;
+  const bool in = c0 < p.d;
+  const int c = in ? c0 : 0;
+  const int64_t len = steps_of(p, b), t0 = tile * S::kTile + wave * L;
+  const bool live = tile * S::kTile < len, full = t0 + L <= len;
+  P x[L], g[L], dy[L];
+  float i[L][V], h[V], ta[V], te[V], m[V];
+#pragma unroll
+  for (int v = 0; v < V; v++) {
+    ta[v] = 1.f;
+    te[v] = h[v] = 0.f;
+  }
+  if (live) {
+    float a[V], e[V], q[V];
+#pragma unroll
+    for (int v = 0; v < V; v++) h[v] = p.starts[(b * p.tiles + tile) * p.d + c + v];
+    S::load(x, p.x, b * p.xb, p.xt, c, t0, len);
+    S::load(g, p.g, b * p.gb, p.gt, c, t0, len);
+    if (p.dy) S::load(dy, p.dy, b * p.yb, p.yt, c, t0, len);
+    S::forward_map(x, g, t0, len, i, a, e);
+    S::backward_map(p, dy, t0, len, i, q);
+#pragma unroll
+    for (int v = 0; v < V; v++) {
+      maps[0][wave][lane * V + v] = a[v];
+      maps[1][wave][lane * V + v] = e[v];
+      maps[2][wave][lane * V + v] = q[v];
+    }
+    __syncthreads();
 #pragma unroll
     for (int w = W - 1; w >= 0; w--)
 #pragma unroll
       for (int v = 0; v < V; v++) {
-        const float ma = m[0][w][lane * V + v];
-        if (w == wave) mm[v] = m0[v];
-        m0[v] = fmaf(ma, m0[v], m[2][w][lane * V + v]);
-        if (!OUT) ca[v] *= ma;
+        te[v] = fmaf(maps[0][w][lane * V + v], te[v], maps[2][w][lane * V + v]);
+        ta[v] *= maps[0][w][lane * V + v];
       }
-    if (OUT) {
-      float before[L][V];  // h_{t-1} - x_t
-#pragma unroll
-      for (int s = 0; s < L; s++)
-#pragma unroll
-        for (int v = 0; v < V; v++) {
-          before[s][v] = h[v] - x[s][v];
-          h[v] = fmaf(-i[s][v], before[s][v], h[v]);
-        }
-#pragma unroll
-      for (int s = L - 1; s >= 0; s--) {
-        P ox, og;
-#pragma unroll
-        for (int v = 0; v < V; v++) {
-          const float l = mm[v] + dy[s][v];
-          const float il = i[s][v] * l;
-          mm[v] = l - il;
-          ox.set(v, il);
-          og.set(v, (1.f - i[s][v]) * il * before[s][v]);
-        }
-        if (full ? in : in && t0 + s < p.t) {
-          const bool on = full || t0 + s < len;
-          S::store(p.dx, b * p.t + t0 + s, p.d, c, on ? ox : S::zero());
-          S::store(p.dg, b * p.t + t0 + s, p.d, c, on ? og : S::zero());
-        }
-      }
-    }
-#pragma unroll
-    for (int s = 0; s < L; s++) {
-      x[s] = nx[s];
-      g[s] = ng[s];
-      dy[s] = ndy[s];
-    }
-#pragma unroll
-    for (int v = 0; v < V; v++) st[v] = nst[v];
   }
-  if (wave != 0 || !in) return;
-  if (OUT) {
-    if (seg == 0 && p.dstate)
-#pragma unroll
-      for (int v = 0; v < V; v++) p.dstate[b * p.d + c + v] = m0[v];
-  } else {
-    float *m = p.maps + (b * p.segs + seg) * 2 * p.d + c;
-#pragma unroll
-    for (int v = 0; v < V; v++) {
-      m[v] = ca[v];
-      m[p.d + v] = m0[v];
-    }
+  if (!enter(p, ch, b, pos, c, in, lane, wave, live, p.dfinal, ta, te, m)) {
+    S::zero_gradients(p, b, c, in, t0);
+    return;
   }
+  if (wave == 0 && in && pos + 1 == p.tiles && p.dstate)
+#pragma unroll
+    for (int v = 0; v < V; v++) p.dstate[b * p.d + c + v] = fmaf(ta[v], m[v], te[v]);
+  if (!live) {
+    S::zero_gradients(p, b, c, in, t0);
+    return;
+  }
+  for (int w = 0; w < wave; w++)
+#pragma unroll
+    for (int v = 0; v < V; v++) h[v] = fmaf(maps[0][w][lane * V + v], h[v], maps[1][w][lane * V + v]);
+  for (int w = W - 1; w > wave; w--)
+#pragma unroll
+    for (int v = 0; v < V; v++) m[v] = fmaf(maps[0][w][lane * V + v], m[v], maps[2][w][lane * V + v]);
+  S::backward_steps(p, b, c, in, full, t0, len, x, dy, i, h, m);
 }
 
 // ------------------------------------------------------------ single step
@@ -451,55 +483,64 @@ __global__ __launch_bounds__(256) void step_kernel(const typename N::store *__re
 constexpr int kSteps = 16;  // steps of a wave in a tile
 
 // Waves along time.  A short sequence would leave most of a tall tile empty.
-int waves_of(int64_t t) { return t <= 2 * kSteps ? 1 : 8; }
+int waves_of(int64_t t) { return t <= kSteps ? 1 : t <= 2 * kSteps ? 2 : 8; }
 int64_t tiles_of(int64_t t) {
   const int tile = kSteps * waves_of(t);
   return (t + tile - 1) / tile;
 }
 
+// Workgroups of one launch: a grid holds fewer than 2^32 threads.
+constexpr int64_t kMostTiles = 1 << 22;
+
 struct Plan {
-  int lanes, slabs, segs;
-  int64_t seg_tiles;
+  int slabs;
+  int64_t groups, at_once;             // groups, and those of one launch
+  size_t tickets, maps, heads, bytes;  // sizes of the chain's buffers, and of the workspace
 };
 
-// Two 16-bit channels a lane where alignment allows it (a wave then reads 256 bytes of a step,
-// as with one fp32 channel); time in segments until there are two workgroups for each CU.
-Plan plan(int64_t batch, int64_t t, int d, bool pairs) {
+// Two 16-bit channels a lane where alignment allows it: a wave then reads 256 bytes of a step, as
+// with one fp32 channel (4 x 4096 x 4096 bf16: 100 us against 125).
+Plan plan(int64_t batch, int64_t t, int64_t d, bool pairs) {
   Plan q{};
-  q.lanes = 64 * (pairs ? 2 : 1);
-  q.slabs = (d + q.lanes - 1) / q.lanes;
-  const int64_t tiles = tiles_of(t), groups = batch * q.slabs;
-  const int64_t segs = std::max<int64_t>(1, std::min(tiles, 512 / groups));
-  q.seg_tiles = (tiles + segs - 1) / segs;
-  q.segs = q.seg_tiles ? static_cast<int>((tiles + q.seg_tiles - 1) / q.seg_tiles) : 1;
+  const int lanes = pairs ? 128 : 64;
+  const int64_t tiles = std::max<int64_t>(1, tiles_of(t));
+  q.slabs = static_cast<int>((d + lanes - 1) / lanes);
+  q.groups = batch * q.slabs;
+  q.at_once = std::max<int64_t>(1, std::min(q.groups, kMostTiles / tiles));
+  if (tiles > 1) {
+    const int64_t launches = (q.groups + q.at_once - 1) / q.at_once;
+    q.tickets = static_cast<size_t>(launches + 3) / 4 * 16;
+    q.maps = static_cast<size_t>(batch) * tiles * d * sizeof(uint64_t);
+    q.heads = static_cast<size_t>(batch) * ((tiles + kRun - 1) / kRun) * d * sizeof(uint32_t);
+    q.bytes = (q.tickets + q.maps + q.heads + 15) / 16 * 16;
+  }
   return q;
 }
 
 template <class N, int V, int W>
-void launch(bool back, const Args &p, int64_t groups, hipStream_t s) {
-  const dim3 block(64 * W), all(static_cast<unsigned>(groups), static_cast<unsigned>(p.segs)),
-      inner(static_cast<unsigned>(groups), static_cast<unsigned>(p.segs - 1));
-  if (back) {
-    if (p.segs > 1)
-      hipLaunchKernelGGL((backward_kernel<N, V, W, kSteps, false>), inner, block, 0, s, p);
-    hipLaunchKernelGGL((backward_kernel<N, V, W, kSteps, true>), all, block, 0, s, p);
-  } else {
-    if (p.segs > 1)
-      hipLaunchKernelGGL((forward_kernel<N, V, W, kSteps, false>), inner, block, 0, s, p);
-    hipLaunchKernelGGL((forward_kernel<N, V, W, kSteps, true>), all, block, 0, s, p);
-  }
+void launch(bool back, const Args &p, hipStream_t s) {
+  const unsigned grid = p.groups * static_cast<unsigned>(p.tiles);
+  if (back) hipLaunchKernelGGL((backward_kernel<N, V, W, kSteps>), dim3(grid), dim3(64 * W), 0, s, p);
+  else hipLaunchKernelGGL((forward_kernel<N, V, W, kSteps>), dim3(grid), dim3(64 * W), 0, s, p);
+}
+
+template <class N, int V>
+void launch_waves(bool back, const Args &p, hipStream_t s) {
+  const int w = waves_of(p.t);
+  if (w == 1) launch<N, V, 1>(back, p, s);
+  else if (w == 2) launch<N, V, 2>(back, p, s);
+  else launch<N, V, 8>(back, p, s);
 }
 
 template <class N>
-void launch_type(bool back, bool pairs, const Args &p, int64_t groups, hipStream_t s) {
-  const bool tall = waves_of(p.t) > 1;
+void launch_type(bool back, bool pairs, const Args &p, hipStream_t s) {
   if constexpr (sizeof(typename N::store) == 2) {
     if (pairs) {
-      tall ? launch<N, 2, 8>(back, p, groups, s) : launch<N, 2, 1>(back, p, groups, s);
+      launch_waves<N, 2>(back, p, s);
       return;
     }
   }
-  tall ? launch<N, 1, 8>(back, p, groups, s) : launch<N, 1, 1>(back, p, groups, s);
+  launch_waves<N, 1>(back, p, s);
 }
 
 vs_status check(const char *who, int dtype, int64_t batch, int64_t t, int64_t d) {
@@ -521,30 +562,36 @@ vs_status run(bool back, Args p, int dtype, int64_t batch, void *workspace, size
                      paired(p.g, p.gb, p.gt) && paired(p.dy, p.yb, p.yt) && paired(p.y, 0, 0) &&
                      paired(p.dx, 0, 0) && paired(p.dg, 0, 0);
   const Plan q = plan(batch, p.t, p.d, pairs);
-  p.tiles = tiles_of(p.t);
-  p.seg_tiles = q.seg_tiles;
-  p.segs = q.segs;
+  p.tiles = std::max<int64_t>(1, tiles_of(p.t));
+  VS_REQUIRE(p.tiles <= kMostTiles, "gated_recurrence: sequence too long (%lld steps)",
+             static_cast<long long>(p.t));
   p.slabs = q.slabs;
   DeviceBuffer own;
-  if (p.segs > 1) {
-    const size_t need = static_cast<size_t>(batch) * p.segs * 2 * p.d * sizeof(float);
+  if (q.bytes) {
+    uint8_t *base = static_cast<uint8_t *>(workspace);
     if (workspace) {
-      VS_REQUIRE(bytes >= need, "gated_recurrence: workspace of %zu bytes, %zu needed", bytes,
-                 need);
-      p.maps = static_cast<float *>(workspace);
+      VS_REQUIRE(bytes >= q.bytes && reinterpret_cast<uintptr_t>(workspace) % 16 == 0,
+                 "gated_recurrence: workspace of %zu bytes, %zu needed (16-byte aligned)", bytes,
+                 q.bytes);
     } else {
-      VS_TRY(own.alloc(need, s));
-      p.maps = own.as<float>();
+      VS_TRY(own.alloc(q.bytes, s));
+      base = own.as<uint8_t>();
     }
-  }
-  // a grid holds fewer than 2^32 threads
-  const int64_t most = std::max<int64_t>(1, (1 << 22) / q.slabs);
-  for (; p.b0 < batch; p.b0 += most) {
-    const int64_t groups = std::min(most, batch - p.b0) * q.slabs;
-    if (dtype == VS_F32) launch_type<num::F32>(back, pairs, p, groups, s);
-    else if (dtype == VS_F16) launch_type<num::F16>(back, pairs, p, groups, s);
-    else launch_type<num::BF16>(back, pairs, p, groups, s);
+    p.ticket = reinterpret_cast<uint32_t *>(base);
+    p.maps = reinterpret_cast<uint64_t *>(base + q.tickets);
+    p.heads = reinterpret_cast<uint32_t *>(base + q.tickets + q.maps);
+    const int64_t n = static_cast<int64_t>(q.bytes / 16);
+    hipLaunchKernelGGL(ones_kernel, dim3(elementwise_grid(static_cast<size_t>(n), 256)), dim3(256), 0, s,
+                       reinterpret_cast<uint4 *>(base), n);
     VS_HIP(hipGetLastError());
+  }
+  for (; p.group0 < q.groups; p.group0 += q.at_once) {
+    p.groups = static_cast<unsigned>(std::min(q.at_once, q.groups - p.group0));
+    if (dtype == VS_F32) launch_type<num::F32>(back, pairs, p, s);
+    else if (dtype == VS_F16) launch_type<num::F16>(back, pairs, p, s);
+    else launch_type<num::BF16>(back, pairs, p, s);
+    VS_HIP(hipGetLastError());
+    if (p.ticket) p.ticket++;  // each launch has its counter
   }
   return VS_OK;
 }
@@ -561,13 +608,7 @@ int64_t vs_gated_recurrence_tiles(int64_t t) { return t > 0 ? rec::tiles_of(t) :
 
 size_t vs_gated_recurrence_workspace(int64_t batch, int64_t t, int64_t d) {
   if (batch <= 0 || t <= 0 || d <= 0 || rec::check("", VS_F32, batch, t, d) != VS_OK) return 0;
-  size_t most = 0;
-  for (const bool pairs : {false, true}) {
-    const rec::Plan q = rec::plan(batch, t, static_cast<int>(d), pairs);
-    if (q.segs > 1)
-      most = std::max(most, static_cast<size_t>(batch) * q.segs * 2 * d * sizeof(float));
-  }
-  return most;
+  return std::max(rec::plan(batch, t, d, false).bytes, rec::plan(batch, t, d, true).bytes);
 }
 
 vs_status vs_gated_recurrence(int dtype, const void *x, int64_t x_batch, int64_t x_time,

@@ -115,10 +115,11 @@ def test_forward_and_gradients(dev, dtype, lengths, shape):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("shape", [(1, 9000, 1), (1, 6001, 70), (2, 5000, 200), (1, 4100, 512), (70001, 2, 3),
-                                   (300, 40, 130)])
+                                   (300, 40, 130), (1, 2048, 64), (3, 2049, 66), (600, 300, 128)])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_long_wide_and_many(shape, dtype):
-    """Time cut into segments, more sequences than one grid dimension of 65535, partly filled tiles."""
+    """Chains of tiles: runs that end with the sequence and one step behind, more tiles than workgroups that run at once,
+    more sequences than one grid dimension of 65535, partly filled tiles."""
     x, gate, h0, n = _inputs(*shape, dtype, "cuda", seed=5, lengths="ragged")
     if shape[0] == 1:
         n = torch.tensor([shape[1] - 37], device="cuda")
@@ -130,6 +131,19 @@ def test_long_wide_and_many(shape, dtype):
     want = _oracle(x, gate, h0, n, dy, df)
     for name, got in zip(("y", "final", "dx", "dgate", "dstate"), (y, final, *grads)):
         _close(name, got, want[name])
+
+
+@pytest.mark.gpu
+def test_more_tiles_than_one_grid():
+    """2^21 + 5 sequences of two tiles are two launches; every sequence gets the bits of a small call."""
+    b, t = (1 << 21) + 5, 129
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.randn(b, t, 1, device="cuda", generator=g)
+    gate = torch.randn(b, t, 1, device="cuda", generator=g) + 2
+    y, final = ops.gated_recurrence(x, gate)
+    rows = torch.tensor([0, 1, 77777, (1 << 21) - 1, 1 << 21, (1 << 21) + 4], device="cuda")
+    ys, fs = ops.gated_recurrence(x[rows], gate[rows])
+    assert torch.equal(y[rows], ys) and torch.equal(final[rows], fs)
 
 
 @pytest.mark.parametrize("dev", DEVICES)
@@ -167,7 +181,7 @@ def test_formula_gradient_agrees_with_differences(dev):
 def test_padding_is_never_read(dev, shape):
     """NaN and infinities behind the sequences' ends change nothing, forward and backward; lengths outside 0..t are clamped."""
     if dev == "cpu" and shape[1] > 1000:
-        pytest.skip("the segmented path is the GPU's")
+        pytest.skip("the chained path is the GPU's")
     b, t, d = shape
     x, gate, h0, _ = _inputs(b, t, d, torch.float32, dev, seed=3)
     n = torch.tensor([t - 3, 0, -5][:b], dtype=torch.int32, device=dev)
