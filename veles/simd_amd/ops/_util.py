@@ -44,18 +44,26 @@ def launch(t: torch.Tensor, name: str, *args) -> None:
 _PLAIN = (torch.Tensor, torch.nn.Parameter)
 
 
-def plain_call(*tensors) -> bool:
-    """True when a call needs none of the dispatcher's services: ordinary tensors, no gradient to
-    record, nothing tracing.  The implementation is then called directly, which takes several
-    microseconds of host time off the calls of a decoding loop."""
+def plain_tensors(*tensors) -> bool:
+    """True when a call needs none of the dispatcher's services: ordinary tensors, nothing tracing.
+    The implementation (or its autograd Function) is then called directly, which takes several
+    microseconds of host time off a call, and about a hundred off a training pass."""
     if torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack() \
             or torch._C._functorch.peek_interpreter_stack() is not None:
         return False
-    grad = torch.is_grad_enabled()
     for t in tensors:
-        if t is not None and (type(t) not in _PLAIN or (grad and t.requires_grad)):
+        if t is not None and type(t) not in _PLAIN:
             return False
     return True
+
+
+def records(*tensors) -> bool:
+    """True when autograd records a call on these tensors."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 @contextlib.contextmanager

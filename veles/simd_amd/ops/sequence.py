@@ -8,7 +8,7 @@ from __future__ import annotations
 import torch
 
 from .. import _lib
-from ._util import launch, plain_call
+from ._util import launch, plain_tensors, records
 
 DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 5}
 
@@ -172,12 +172,33 @@ def _recurrence_setup(ctx, inputs, output):
 
 
 def _recurrence_grad(ctx, dy, dfinal, _):
-    x, gate, lengths, starts = ctx.saved_tensors
+    return *_recurrence_grads(ctx, torch.ops.veles.gated_recurrence_backward, dy, dfinal), None, None
+
+
+def _recurrence_grads(ctx, backward, dy, dfinal):
     if dy is None and dfinal is None:
-        return None, None, None, None, None
-    dx, dg, dstate = torch.ops.veles.gated_recurrence_backward(x, gate, lengths, starts, dy, dfinal)
+        return None, None, None
+    x, gate, lengths, starts = ctx.saved_tensors
+    dx, dg, dstate = backward(x, gate, lengths, starts, dy, dfinal)
     need = ctx.needs_input_grad
-    return dx if need[0] else None, dg if need[1] else None, dstate if need[2] else None, None, None
+    return dx if need[0] else None, dg if need[1] else None, dstate if need[2] else None
+
+
+class _Recurrence(torch.autograd.Function):
+    """The op's autograd without the dispatcher."""
+
+    @staticmethod
+    def forward(ctx, x, gate, state, lengths):
+        y, final, starts = _recurrence_impl(x, gate, state, lengths, True)
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(x, gate, lengths, starts)
+        return y, final
+
+    @staticmethod
+    def backward(ctx, dy, dfinal):
+        # a graph of the gradients asks for second derivatives, which the op refuses by name
+        op = torch.ops.veles.gated_recurrence_backward if torch.is_grad_enabled() else _recurrence_backward_impl
+        return *_recurrence_grads(ctx, op, dy, dfinal), None
 
 
 def _with_empty(impl):
@@ -228,10 +249,11 @@ def gated_recurrence(x: torch.Tensor, gate: torch.Tensor, state: torch.Tensor | 
     The state is held in float32.  Differentiable in x, gate and state; in the padding the
     gradients are 0 and dy is not read.  Where the update meets an infinite state or value inside
     a sequence it follows the formula above (inf - inf is NaN)."""
-    if plain_call(x, gate, state, lengths):
+    save = records(x, gate, state)
+    if plain_tensors(x, gate, state, lengths):
+        if save:
+            return _Recurrence.apply(x, gate, state, lengths)
         return _recurrence_impl(x, gate, state, lengths, False)[:2]
-    save = torch.is_grad_enabled() and any(
-        v is not None and v.requires_grad for v in (x, gate, state))
     y, final, _ = torch.ops.veles.gated_recurrence(x, gate, state, lengths, save)
     return y, final
 
@@ -271,11 +293,11 @@ def gated_recurrence_step(x: torch.Tensor, gate: torch.Tensor, state: torch.Tens
     """One step of gated_recurrence for a batch of sequences: x, gate [batch, channels]; state
     (float32 [batch, channels], contiguous) is updated in place and returned as y in x's type.
     For generation: it records no gradient."""
-    if plain_call(x, gate, state):
-        return _step_impl(x, gate, state)
-    if torch.is_grad_enabled() and (x.requires_grad or gate.requires_grad or state.requires_grad):
+    if records(x, gate, state):
         raise RuntimeError("gated_recurrence_step records no gradient: call it under torch.no_grad(), or use "
                            "gated_recurrence")
+    if plain_tensors(x, gate, state):
+        return _step_impl(x, gate, state)
     return torch.ops.veles.gated_recurrence_step(x, gate, state)
 
 
@@ -347,10 +369,10 @@ def matvec_int4(x: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor,
     are float32; the result is rounded once, to x's type.  An infinite x gives NaN (the zero point is
     taken off the sum).  For generation: it records no gradient; more than 16 rows read the weights
     once for every 16.  quantize_int4 makes the operands."""
-    if plain_call(x, qweight, scales, zeros):
-        return _matvec_impl(x, qweight, scales, zeros, group_size)
-    if torch.is_grad_enabled() and (x.requires_grad or scales.requires_grad):
+    if records(x, scales):
         raise RuntimeError("matvec_int4 records no gradient: call it under torch.no_grad()")
+    if plain_tensors(x, qweight, scales, zeros):
+        return _matvec_impl(x, qweight, scales, zeros, group_size)
     return torch.ops.veles.matvec_int4(x, qweight, scales, zeros, group_size)
 
 
@@ -512,14 +534,35 @@ def _gated_setup(ctx, inputs, output):
 
 
 def _gated_grad(ctx, dh, _):
+    return *_gated_grads(ctx, torch.ops.veles.gated_linear_backward, dh), None, None
+
+
+def _gated_grads(ctx, backward, dh):
     if dh is None:
-        return None, None, None, None, None
+        return None, None, None
     x, w_gate, w_up, pre = ctx.saved_tensors
     need = ctx.needs_input_grad
-    dx, dw = torch.ops.veles.gated_linear_backward(x, w_gate, w_up, pre, dh, ctx.activation, need[0],
-                                                   need[1] or need[2])
+    dx, dw = backward(x, w_gate, w_up, pre, dh, ctx.activation, need[0], need[1] or need[2])
     f = w_gate.shape[0]
-    return dx if need[0] else None, dw[:f] if need[1] else None, dw[f:] if need[2] else None, None, None
+    return dx if need[0] else None, dw[:f] if need[1] else None, dw[f:] if need[2] else None
+
+
+class _Gated(torch.autograd.Function):
+    """The op's autograd without the dispatcher."""
+
+    @staticmethod
+    def forward(ctx, x, w_gate, w_up, activation):
+        h, pre = _gated_impl(x, w_gate, w_up, activation, True)
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(x, w_gate, w_up, pre)
+        ctx.activation = activation
+        return h
+
+    @staticmethod
+    def backward(ctx, dh):
+        # a graph of the gradients asks for second derivatives, which the op refuses by name
+        op = torch.ops.veles.gated_linear_backward if torch.is_grad_enabled() else _gated_backward_impl
+        return *_gated_grads(ctx, op, dh), None
 
 
 torch.library.define("veles::gated_linear",
@@ -549,7 +592,9 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor,
     in x and the weights; the float32 pairs (x @ w_gate.T, x @ w_up.T), 8 bytes per output, are kept for the
     backward pass, and the gradients of the two products are rounded to x's type before they are
     multiplied.  Up to 64 rows (generation) stream the weights once at memory speed."""
-    if plain_call(x, w_gate, w_up):
+    save = records(x, w_gate, w_up)
+    if plain_tensors(x, w_gate, w_up):
+        if save:
+            return _Gated.apply(x, w_gate, w_up, activation)
         return _gated_impl(x, w_gate, w_up, activation, False)[0]
-    save = torch.is_grad_enabled() and (x.requires_grad or w_gate.requires_grad or w_up.requires_grad)
     return torch.ops.veles.gated_linear(x, w_gate, w_up, activation, save)[0]
