@@ -383,7 +383,17 @@ __global__ __launch_bounds__(512) void tile_kernel(Work work) {
     // Results: rows of 16-bit values, two neighbouring 16-column blocks exchanged between odd and
     // even lane groups where there are two, so a lane stores 16 bytes.
     constexpr int NB = C::GATED ? YH : 2 * YH;
-    const bool vec = p.n % 8 == 0 && (reinterpret_cast<uintptr_t>(p.c) & 15) == 0;
+    // (Rows of any alignment: the memory pipeline takes unaligned 16-byte stores.)
+    const auto put = [&](uint16_t *out, int col, const auto &v) {
+      constexpr int E = sizeof(v) / 2;
+      if (col + E <= p.n) {
+        __builtin_memcpy(out + col, &v, sizeof(v));
+      } else {
+#pragma unroll
+        for (int e = 0; e < E; e++)
+          if (col + e < p.n) out[col + e] = static_cast<uint16_t>(v[e / 2] >> (16 * (e & 1)));
+      }
+    };
 #pragma unroll
     for (int i = 0; i < 2; i++)
 #pragma unroll
@@ -415,28 +425,18 @@ __global__ __launch_bounds__(512) void tile_kernel(Work work) {
         }
         if (row >= p.m) continue;
         uint16_t *out = p.c + static_cast<int64_t>(row) * p.n;
-        if (vec && NB % 2 == 0) {
+        if constexpr (NB % 2 == 0) {
 #if defined(__HIP_DEVICE_COMPILE__)
 #pragma unroll
           for (int b = 0; b + 1 < NB; b += 2) {
             const u32x2 lo = __builtin_amdgcn_permlane16_swap(w[b][0], w[b + 1][0], false, false);
             const u32x2 hi = __builtin_amdgcn_permlane16_swap(w[b][1], w[b + 1][1], false, false);
-            const int col = rn + 16 * (b + (lq & 1)) + 8 * (lq >> 1);
-            if (col < p.n) *reinterpret_cast<uint4 *>(out + col) = uint4{lo.x, hi.x, lo.y, hi.y};
+            put(out, rn + 16 * (b + (lq & 1)) + 8 * (lq >> 1), u32x4{lo.x, hi.x, lo.y, hi.y});
           }
 #endif
         } else {
 #pragma unroll
-          for (int b = 0; b < NB; b++) {
-            const int col = rn + 16 * b + 4 * lq;
-            if (vec) {
-              if (col < p.n) *reinterpret_cast<uint2 *>(out + col) = uint2{w[b][0], w[b][1]};
-            } else {
-#pragma unroll
-              for (int r = 0; r < 4; r++)
-                if (col + r < p.n) out[col + r] = static_cast<uint16_t>(w[b][r / 2] >> (16 * (r & 1)));
-            }
-          }
+          for (int b = 0; b < NB; b++) put(out, rn + 16 * b + 4 * lq, u32x2{w[b][0], w[b][1]});
         }
       }
     if (tile >= work.tiles) return;
@@ -608,23 +608,33 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_kernel(Args p) {
 }
 
 // ------------------------------------------------- layout and element-wise
-// [rows][cols] (row stride ld) copied to rows of cols_p, zeros behind: rows that the DMA can read.
-__global__ __launch_bounds__(256) void pad_kernel(const uint16_t *__restrict__ src, int64_t ld,
-                                                  int64_t rows, int cols, int cols_p,
-                                                  uint16_t *__restrict__ dst) {
-  const int chunks = cols_p / 8;
-  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < rows * chunks; i += gridDim.x * 256ll) {
+// Up to three matrices [rows][cols] (row stride ld) copied to rows of cols_p, zeros behind: rows that
+// the DMA can read.  One thread per 16-byte piece, the matrices one after the other.
+struct Pad {
+  const uint16_t *src[3];
+  int64_t ld[3], pieces[3];
+  uint16_t *dst[3];
+  int cols, cols_p;
+};
+__global__ __launch_bounds__(256) void pad_kernel(Pad p) {
+  const int chunks = p.cols_p / 8;
+  const int64_t all = p.pieces[0] + p.pieces[1] + p.pieces[2];
+  for (int64_t at = blockIdx.x * 256ll + threadIdx.x; at < all; at += gridDim.x * 256ll) {
+    int64_t i = at;
+    int j = 0;
+    while (i >= p.pieces[j]) i -= p.pieces[j++];
     const int64_t r = i / chunks;
     const int c = static_cast<int>(i - r * chunks) * 8;
-    const uint16_t *s = src + r * ld + c;
+    const uint16_t *s = p.src[j] + r * p.ld[j] + c;
     uint32_t e[4] = {0, 0, 0, 0};
-    if (c + 8 <= cols) {
+    if (c + 8 <= p.cols) {
       __builtin_memcpy(e, s, 16);
     } else {
-      for (int j = 0; j < 8; j++)
-        if (c + j < cols) e[j / 2] |= static_cast<uint32_t>(s[j]) << (16 * (j & 1));
+#pragma unroll
+      for (int k = 0; k < 8; k++)
+        if (c + k < p.cols) e[k / 2] |= static_cast<uint32_t>(s[k]) << (16 * (k & 1));
     }
-    *reinterpret_cast<uint4 *>(dst + r * cols_p + c) = uint4{e[0], e[1], e[2], e[3]};
+    *reinterpret_cast<uint4 *>(p.dst[j] + r * p.cols_p + c) = uint4{e[0], e[1], e[2], e[3]};
   }
 }
 
@@ -865,16 +875,6 @@ vs_status open_space(Space &sp, DeviceBuffer &own, void *workspace, size_t bytes
   return VS_OK;
 }
 
-vs_status pad(const uint16_t *src, int64_t ld, int64_t rows, int cols, uint16_t *dst, hipStream_t s) {
-  const int cp = up8(cols);
-  const int64_t work = rows * (cp / 8);
-  if (work == 0) return VS_OK;
-  const unsigned grid = static_cast<unsigned>(std::min<int64_t>((work + 255) / 256, 1 << 20));
-  hipLaunchKernelGGL(pad_kernel, dim3(grid), dim3(256), 0, s, src, ld, rows, cols, cp, dst);
-  VS_HIP(hipGetLastError());
-  return VS_OK;
-}
-
 vs_status check(const char *who, int dtype, int act, int64_t m, int64_t f, int64_t k) {
   VS_REQUIRE(dtype == VS_F16 || dtype == VS_BF16, "%s: unsupported dtype %d (fp16, bf16)", who, dtype);
   VS_REQUIRE(act >= VS_ACT_SILU && act <= VS_ACT_SIGMOID, "%s: unknown activation %d", who, act);
@@ -950,19 +950,26 @@ vs_status forward(Args p, void *workspace, size_t bytes, hipStream_t s) {
   Space sp;
   VS_TRY(open_space(sp, own, workspace, bytes, q.bytes, s));
   const int kp = up8(p.k);
-  if (q.px) {
-    uint16_t *d = sp.take(static_cast<size_t>(p.m) * kp);
-    VS_TRY(pad(p.a, p.lda, p.m, p.k, d, s));
-    p.a = d;
-    p.lda = kp;
+  Pad pd{};
+  pd.cols = p.k;
+  pd.cols_p = kp;
+  int n = 0;
+  const auto copy = [&](const uint16_t *&src, int64_t &ld, int64_t rows) {
+    pd.src[n] = src;
+    pd.ld[n] = ld;
+    pd.dst[n] = sp.take(static_cast<size_t>(rows) * kp);
+    pd.pieces[n] = rows * (kp / 8);
+    src = pd.dst[n++];
+    ld = kp;
+  };
+  if (q.px) copy(p.a, p.lda, p.m);
+  if (q.pg) copy(p.b[0], p.ldb[0], p.n);
+  if (q.pu) copy(p.b[1], p.ldb[1], p.n);
+  if (const int64_t all = pd.pieces[0] + pd.pieces[1] + pd.pieces[2]) {
+    const unsigned grid = static_cast<unsigned>(std::min<int64_t>((all + 255) / 256, 1 << 20));
+    hipLaunchKernelGGL(pad_kernel, dim3(grid), dim3(256), 0, s, pd);
+    VS_HIP(hipGetLastError());
   }
-  for (int i = 0; i < 2; i++)
-    if (i ? q.pu : q.pg) {
-      uint16_t *d = sp.take(static_cast<size_t>(p.n) * kp);
-      VS_TRY(pad(p.b[i], p.ldb[i], p.n, p.k, d, s));
-      p.b[i] = d;
-      p.ldb[i] = kp;
-    }
   p.k = kp;  // (the same where nothing was copied: a direct operand has whole pieces)
   return product<N, true>(&p, 1, s);
 }
