@@ -26,9 +26,11 @@
 // composes its initial state from the maps of the tiles before it in its run of kRun tiles and the
 // state at the start of the run, which the last tile of the run before publishes.  What is composed
 // with what does not depend on timing, so results are the same bits every time.  Measured against
-// a workgroup that walks the tiles of its channels (forward, us): 1 x 65536 x 1024 fp32 164 against
+// a workgroup that walks the tiles of its channels (forward, us): 1 x 65536 x 1024 fp32 154 against
 // 2017 (295 with time cut into segments whose maps a first kernel computes, which reads x and g
-// twice), 4 x 4096 x 4096 bf16 100 against 136, 8 x 2048 x 8192 bf16 173 against 186.
+// twice), 4 x 4096 x 4096 bf16 91 against 136, 8 x 2048 x 8192 bf16 167 against 186.  That is 5.2,
+// 4.4 and 4.8 TB/s; a large copy reaches 5.1 to 5.3 on the same card.  Backward: 245, 146 and 265 us
+// (5.5, 4.6 and 5.1 TB/s).
 // Copyright 2026 veles.simd_amd authors. Apache-2.0.
 #include <hip/hip_runtime.h>
 
@@ -57,7 +59,8 @@ struct Args {
   float *starts;                     // [batch][tiles][d]: state at the start of each tile, or null
   uint64_t *maps;                    // [batch][tiles][d]: a tile's map (product low, sum high)
   uint32_t *heads;                   // [batch][runs][d]: what enters a run of tiles
-  uint32_t *ticket;                  // null where a sequence is one tile
+  uint32_t *ticket;                  // a counter per group, or null where a sequence is one tile
+  int spread;                        // words between two counters
   int64_t t, tiles;                  // steps, tiles
   int64_t group0;                    // first group (sequence and slab of 64 V channels) of this launch
   unsigned groups;                   // groups of this launch
@@ -213,13 +216,15 @@ struct Shape {
 };
 
 // ------------------------------------------------------------------ chain
-// Workgroups take tiles by a counter, position by position along time (from the end in the backward
-// pass).  A tile waits for earlier positions only, which have lower numbers, and a workgroup takes
-// its number when it already runs: by induction over the numbers every wait ends.  Maps and
+// Workgroups take the tiles of a group (a sequence and a slab of channels) by a counter, position by
+// position along time (from the end in the backward pass).  A tile waits for earlier positions of
+// its group only, and a workgroup takes its position when it already runs: by induction over the
+// positions every wait ends.  (One counter for all tiles costs about 15 ns a workgroup, one after
+// the other: 16 x 1000 x 1536 fp16 47 us, 41 with a counter per group.)  Maps and
 // states are published and polled as single relaxed atomics at device scope, 64 or 32 bits that are
 // never all ones when they are valid (a NaN is stored as the canonical one), so no other memory has
 // to be ordered with them.  The buffers are set to all ones before the launch.
-constexpr int kRun = 16;
+constexpr int kRun = 8;  // 4 and 16 are slower where channels are few: 177 and 172 us at 1 x 65536 x 1024 fp32
 constexpr uint32_t kNone = 0xffffffffu;
 constexpr int kPolls = 1 << 18;  // a fraction of a second; then a NaN goes on in place of what did not come
 
@@ -264,26 +269,29 @@ struct Chain {
   static constexpr int kLanes = 64 * V;
   float run[kRun - 1][2][kLanes];  // maps of the tiles before this one in its run
   float head[kLanes];              // what enters the run
-  unsigned ticket;
+  unsigned pos;
 };
 
 // This workgroup's position along the chain, its sequence and its slab of channels.  (Workgroups that
-// stay and draw their next number while they work were slower, 194 us against 164 at
-// 1 x 65536 x 1024 fp32: the tiles behind wait for a number whose workgroup is not free yet.)
+// stay and draw their next tile while they work were slower, 194 us against 164 at
+// 1 x 65536 x 1024 fp32: the tiles behind wait for a position whose workgroup is not free yet.)
 struct Place {
   int64_t pos, b;
   int slab;
 };
 template <int V, int W>
 __device__ __forceinline__ Place take(const Args &p, Chain<V, W> &ch) {
-  unsigned t = blockIdx.x;
+  // A group moves on by one workgroup, so by one XCD, with every turn: if a slab stayed on its XCD,
+  // its 256-byte pieces of rows a power of two apart would use a few of that cache's channels
+  // (1 x 65536 x 2048 bf16: 208 us, 173 this way).
+  const unsigned turn = blockIdx.x / p.groups;
+  const int64_t group = p.group0 + (blockIdx.x + turn) % p.groups, b = group / p.slabs;
+  unsigned pos = 0;
   if (p.ticket) {
-    if (threadIdx.x == 0) ch.ticket = atomicAdd(p.ticket, 1u) + 1u;  // it starts at all ones
+    if (threadIdx.x == 0) ch.pos = atomicAdd(p.ticket + group * p.spread, 1u) + 1u;  // from all ones
     __syncthreads();
-    t = __builtin_amdgcn_readfirstlane(ch.ticket);
+    pos = __builtin_amdgcn_readfirstlane(ch.pos);
   }
-  const unsigned pos = t / p.groups;
-  const int64_t group = p.group0 + (t - pos * p.groups), b = group / p.slabs;
   return Place{pos, b, static_cast<int>(group - b * p.slabs)};
 }
 
@@ -495,11 +503,12 @@ constexpr int64_t kMostTiles = 1 << 22;
 struct Plan {
   int slabs;
   int64_t groups, at_once;             // groups, and those of one launch
+  int spread;                          // words between two counters: lines of their own where they are few
   size_t tickets, maps, heads, bytes;  // sizes of the chain's buffers, and of the workspace
 };
 
 // Two 16-bit channels a lane where alignment allows it: a wave then reads 256 bytes of a step, as
-// with one fp32 channel (4 x 4096 x 4096 bf16: 100 us against 125).
+// with one fp32 channel (4 x 4096 x 4096 bf16: 100 us against 125 when it was tried).
 Plan plan(int64_t batch, int64_t t, int64_t d, bool pairs) {
   Plan q{};
   const int lanes = pairs ? 128 : 64;
@@ -508,8 +517,8 @@ Plan plan(int64_t batch, int64_t t, int64_t d, bool pairs) {
   q.groups = batch * q.slabs;
   q.at_once = std::max<int64_t>(1, std::min(q.groups, kMostTiles / tiles));
   if (tiles > 1) {
-    const int64_t launches = (q.groups + q.at_once - 1) / q.at_once;
-    q.tickets = static_cast<size_t>(launches + 3) / 4 * 16;
+    q.spread = q.groups <= 4096 ? 64 : 1;
+    q.tickets = static_cast<size_t>(q.groups * q.spread + 3) / 4 * 16;
     q.maps = static_cast<size_t>(batch) * tiles * d * sizeof(uint64_t);
     q.heads = static_cast<size_t>(batch) * ((tiles + kRun - 1) / kRun) * d * sizeof(uint32_t);
     q.bytes = (q.tickets + q.maps + q.heads + 15) / 16 * 16;
@@ -578,6 +587,7 @@ vs_status run(bool back, Args p, int dtype, int64_t batch, void *workspace, size
       base = own.as<uint8_t>();
     }
     p.ticket = reinterpret_cast<uint32_t *>(base);
+    p.spread = q.spread;
     p.maps = reinterpret_cast<uint64_t *>(base + q.tickets);
     p.heads = reinterpret_cast<uint32_t *>(base + q.tickets + q.maps);
     const int64_t n = static_cast<int64_t>(q.bytes / 16);
@@ -591,7 +601,6 @@ vs_status run(bool back, Args p, int dtype, int64_t batch, void *workspace, size
     else if (dtype == VS_F16) launch_type<num::F16>(back, pairs, p, s);
     else launch_type<num::BF16>(back, pairs, p, s);
     VS_HIP(hipGetLastError());
-    if (p.ticket) p.ticket++;  // each launch has its counter
   }
   return VS_OK;
 }
