@@ -4,20 +4,22 @@
 //
 // with g = x Wg^T, u = x Wu^T in fp32.
 //
-// Many rows: bound by the matrix cores.  One kernel computes both products: a tile's B image holds
-// rows of Wg and Wu side by side, 32 and 32 for each wave, so a wave ends with g and u of the same
-// outputs in its accumulators and h is formed in registers.  Operand tiles (256 x 64 or 128 x 64
-// of each operand) go global -> LDS by DMA into two stages; the next tile's pieces are issued
-// before the current tile's products, waves 4-7 a quarter of a tile later than waves 0-3, so one
-// of the two waves of a SIMD multiplies while the other pays for issuing.  Rows past the end and
-// the ragged end of k read zeros through the buffer descriptor's range check.  The backward
-// products are the same kernel with one B operand: the gradients of g and u are written side by
-// side, once as they are and once transposed, x and the weights are transposed, so every product
-// has both operands contiguous in its reduction dimension.
+// Many rows: bound by the matrix cores.  One kernel computes both products: a tile's column halves
+// are rows of Wg and Wu for the same outputs, so a wave ends with g and u of the same outputs in
+// its accumulators and h is formed in registers.  Operand tiles go global -> LDS by DMA into two
+// stages, eight waves take a k tile in four phases with one half of them a barrier behind the other
+// (see tile_kernel).  Rows past the end and the ragged end of k read zeros through the buffer
+// descriptor's range check.  The backward products are the same kernel with one B operand: one
+// launch forms the gradients of g and u, side by side, as they are and transposed, and transposes x
+// and the weights, so both products have their operands contiguous in the reduction dimension; a
+// second launch computes both.  bf16, x [m][k], f outputs: 8192 x 4096 x 12288 takes 1120-1180 us
+// (1400-1470 TFLOP/s; a plain library product of this size 1081 us); forward and backward of
+// 4096 x 2048 x 6144 590-610 us, of which the three products' work is 426 us at that rate.
 //
-// Few rows (all up to 16, and up to 64 where it is faster): bound by reading the weights.  No LDS staging: a wave streams rows of Wg
-// and Wu straight into matrix-core fragments, the waves of a workgroup cut k, and their sums meet
-// in LDS in a fixed order.
+// Few rows (up to 16, and up to 64 where it is faster): bound by reading the weights.  The waves of
+// a workgroup cut k; each loads whole 128-byte stretches of the rows of Wg, Wu and x, forms
+// fragments through a small LDS image of its own, and the waves' sums meet in LDS in a fixed order.
+// bf16: 1 x 2048 x 6144 10.9 us (4.6 TB/s of weights), 33 x 4096 x 10240 41 us (4.1 TB/s).
 //
 // Roundings: h once; for training, g and u are kept in fp32 (a 16-bit copy would add its own
 // rounding to every gradient, 1.7 instead of 1.4 times the error of the result's own rounding);
@@ -243,19 +245,19 @@ __global__ __launch_bounds__(512) void tile_kernel(Work work) {
   const auto start_a = [&](auto half, auto buf, int tile) {
     constexpr int h = decltype(half)::value;
     uint8_t *dst = lds + decltype(buf)::value * C::kBuf + h * C::kHalfA + wid * (C::PA * 1024);
-    const int k0 = tile * C::BK;
+    const int k0 = tile * C::BK, at = k0 < p.k ? 2 * k0 : 0;  // (at stays inside the range)
 #pragma unroll
     for (int i = 0; i < C::PA; i++)
-      dma16(ra, dst + i * 1024, ka[i] < p.k - k0 ? offa[h][i] : kOut, 2 * k0);
+      dma16(ra, dst + i * 1024, ka[i] < p.k - k0 ? offa[h][i] : kOut, at);
   };
   const auto start_b = [&](auto half, auto buf, int tile) {
     constexpr int h = decltype(half)::value;
     uint8_t *dst = lds + decltype(buf)::value * C::kBuf + 2 * C::kHalfA + h * C::kHalfB +
                    wid * (C::PB * 1024);
-    const int k0 = tile * C::BK;
+    const int k0 = tile * C::BK, at = k0 < p.k ? 2 * k0 : 0;
 #pragma unroll
     for (int i = 0; i < C::PB; i++)
-      dma16(h ? rb1 : rb0, dst + i * 1024, kb[i] < p.k - k0 ? offb[h][i] : kOut, 2 * k0);
+      dma16(h ? rb1 : rb0, dst + i * 1024, kb[i] < p.k - k0 ? offb[h][i] : kOut, at);
   };
   // LDS addresses of this lane's fragments [buffer][32-deep step]
   uint32_t ata[2][2], atb[2][2];
@@ -1112,6 +1114,8 @@ vs_status vs_gated_linear_backward(int dtype, int act, const void *x, int64_t ld
   if (k == 0 || (!dx && !dw)) return VS_OK;
   VS_REQUIRE((m == 0 || f == 0) || (x && w_gate && w_up && pre && dh),
              "gated_linear_backward: null pointer");
+  // rows are the reduction of the weights' gradients: 256 of them, transposed, below 2^31 bytes
+  VS_REQUIRE(!dw || m < (1 << 22) - 8, "gated_linear_backward: too many rows for the weights' gradients (2^22)");
   const hipStream_t s = static_cast<hipStream_t>(stream);
   const auto u16 = [](const void *v) { return static_cast<const uint16_t *>(v); };
   const auto go = [&](auto tag) {

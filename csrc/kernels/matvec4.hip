@@ -380,29 +380,32 @@ vs_status vs_matvec_int4(int dtype, const void *x, int64_t ldx, const uint8_t *q
   VS_REQUIRE(group == 32 || group == 64 || (group > 0 && group % 128 == 0),
              "matvec_int4: group of %lld (32, 64 or a multiple of 128)",
              static_cast<long long>(group));
-  VS_REQUIRE(m <= (1 << 20) && n < (1ll << 30) && k < (1ll << 30) && group < (1ll << 30),
+  VS_REQUIRE(m < (1ll << 31) && n < (1ll << 30) && k < (1ll << 30) && group < (1ll << 30),
              "matvec_int4: dimension too large");
   if (m == 0 || n == 0) return VS_OK;
   VS_REQUIRE(y && (k == 0 || (x && qweight && scales)), "matvec_int4: null pointer");
   VS_REQUIRE(m == 1 || ldx >= k || ldx == 0, "matvec_int4: ldx < k");
   VS_REQUIRE(n == 1 || ldq >= (k + 1) / 2, "matvec_int4: ldq < (k + 1) / 2");
-  mv4::Args p{};
-  p.x = static_cast<const uint16_t *>(x);
-  p.ldx = ldx;
-  p.q = qweight;
-  p.ldq = ldq;
-  p.s = static_cast<const uint16_t *>(scales);
-  p.z = zeros;
-  p.y = static_cast<uint16_t *>(y);
-  p.m = static_cast<int>(m);
-  p.n = static_cast<int>(n);
-  p.k = static_cast<int>(k);
-  p.groups = static_cast<int>((k + group - 1) / group);
-  p.span = static_cast<int>(std::max<int64_t>(1, group / mv4::kBlock));
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  if (dtype == VS_BF16) mv4::launch_type<num::BF16>(p, static_cast<int>(group), s);
-  else mv4::launch_type<num::F16>(p, static_cast<int>(group), s);
-  VS_HIP(hipGetLastError());
+  constexpr int64_t kRows = 16 * kMaxGridY;  // rows of one launch
+  for (int64_t m0 = 0; m0 < m; m0 += kRows) {
+    mv4::Args p{};
+    p.x = static_cast<const uint16_t *>(x) + m0 * ldx;
+    p.ldx = ldx;
+    p.q = qweight;
+    p.ldq = ldq;
+    p.s = static_cast<const uint16_t *>(scales);
+    p.z = zeros;
+    p.y = static_cast<uint16_t *>(y) + m0 * n;
+    p.m = static_cast<int>(std::min(kRows, m - m0));
+    p.n = static_cast<int>(n);
+    p.k = static_cast<int>(k);
+    p.groups = static_cast<int>((k + group - 1) / group);
+    p.span = static_cast<int>(std::max<int64_t>(1, group / mv4::kBlock));
+    if (dtype == VS_BF16) mv4::launch_type<num::BF16>(p, static_cast<int>(group), s);
+    else mv4::launch_type<num::F16>(p, static_cast<int>(group), s);
+    VS_HIP(hipGetLastError());
+  }
   return VS_OK;
 }
 

@@ -226,7 +226,7 @@ struct Shape {
 // to be ordered with them.  The buffers are set to all ones before the launch.
 constexpr int kRun = 8;  // 4 and 16 are slower where channels are few: 177 and 172 us at 1 x 65536 x 1024 fp32
 constexpr uint32_t kNone = 0xffffffffu;
-constexpr int kPolls = 1 << 18;  // a fraction of a second; then a NaN goes on in place of what did not come
+constexpr int kPolls = 1 << 20;  // about a second; then a NaN goes on in place of what did not come
 
 __device__ __forceinline__ uint32_t bits(float f) {
   return f == f ? __float_as_uint(f) : 0x7fc00000u;

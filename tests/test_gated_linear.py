@@ -126,6 +126,10 @@ def test_shapes_strides_and_alignment(dev, m):
         return wide[:, off:off + v.shape[1]]
     for change in (lambda v: shifted(v, 1), lambda v: shifted(v, 8), lambda v: v.t().contiguous().t()):
         _all(change(x), change(wg), change(wu), change(dh), "silu")
+    far = torch.zeros(2 * (1 << 21) + 64, dtype=torch.bfloat16, device=dev)   # rows 2^21 elements apart
+    two = far.as_strided((2, 64), (1 << 21, 1)).copy_(x[:2])
+    _all(two, wg, wu, dh[:2], "silu")
+    _all(far.as_strided((1, 64), (1 << 22, 1)), wg, wu, dh[:1], "silu")
     one = x[:1].expand(m, 64)
     _all(one, wg, wu, dh[:, :1].expand(m, 40), "silu")
     _all(x, wg[:1].expand(40, 64), wu, dh, "silu")
@@ -194,6 +198,7 @@ def test_not_finite_rows_stay_in_their_rows(m):
     x2[1] = float("nan")
     x2[2, 5] = float("inf")
     got = ops.gated_linear(x2, wg, wu)
+    assert torch.isnan(ops.gated_linear(x2, wg, wu, "relu")[1]).all()
     keep = torch.ones(m, dtype=torch.bool)
     keep[1:3] = False
     assert torch.equal(got[keep], ref[keep]) and torch.isnan(got[1]).all() and not torch.isfinite(got[2]).all()
@@ -258,11 +263,15 @@ def test_native_refusals():
     assert call(m=100, f=100, k=65, ldx=65, ldw=65, ws=p, size=16) == 1 and b"workspace" in lib.vs_last_error()
     assert lib.vs_gated_linear_backward(5, 0, p, 8, p, 8, p, 8, None, p, 8, 1, 1, 8, p, p, None, 0, None) == 1
     assert lib.vs_gated_linear_workspace(-1, 1, 1) == 0
+    assert lib.vs_gated_linear_backward(5, 0, p, 8, p, 8, p, 8, p, p, 1, 1 << 22, 1, 8, None, p, p, 16, None) == 1
+    assert b"too many rows" in lib.vs_last_error()
 
 
 @pytest.mark.parametrize("dev", DEVICES)
 def test_opcheck(dev):
-    x, wg, wu, _ = _inputs(5, 24, 16, torch.bfloat16, dev)
+    x, wg, wu, dh = _inputs(5, 24, 16, torch.bfloat16, dev)
+    pre = torch.randn(5, 16, 2, device=dev)
+    torch.library.opcheck(torch.ops.veles.gated_linear_backward.default, (x, wg, wu, pre, dh, "gelu", True, True))
     for args in ((x, wg, wu, "gelu", False), (x.clone().requires_grad_(), wg.clone().requires_grad_(), wu, "silu", True)):
         torch.library.opcheck(torch.ops.veles.gated_linear.default, args)
 

@@ -295,6 +295,21 @@ def test_step_continues_a_prefill(dev, dtype, b, d):
         _close("state", state, (want_y[idx], ey[idx]))
 
 
+@pytest.mark.parametrize("dev", DEVICES)
+def test_step_counts_as_a_write(dev):
+    """A backward pass that needs the state as it was before the step refuses, as for any tensor written in place."""
+    x, gate, h0, _ = _inputs(2, 3, 4, torch.float32, dev)
+    h0 = h0.clone()
+    w = torch.randn_like(h0).requires_grad_()
+    loss = (w * h0).sum()
+    ops.gated_recurrence_step(x[:, 0], gate[:, 0], h0)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        loss.backward()
+    with torch.inference_mode():
+        s = torch.zeros(2, 4, device=dev)
+        ops.gated_recurrence_step(x[:, 0], gate[:, 0], s)
+
+
 @pytest.mark.gpu
 def test_runs_are_bitwise_alike_and_stream_ordered():
     x, gate, h0, n = _inputs(2, 3000, 96, torch.bfloat16, "cuda", seed=6, lengths="ragged")
@@ -399,6 +414,9 @@ OPCHECK = {
         (r(2, 9, 5).requires_grad_(), r(2, 9, 5).requires_grad_(), r(2, 5).requires_grad_(),
          torch.tensor([9, 3], device=dev), True), (r(2, 9, 5), r(2, 9, 5), None, None, False)],
     "gated_recurrence_step": lambda r, dev: [(r(3, 5), r(3, 5), r(3, 5))],
+    "gated_recurrence_backward": lambda r, dev: [
+        (r(2, 9, 5), r(2, 9, 5), torch.tensor([9, 3], device=dev), r(2, 1, 5), r(2, 9, 5), r(2, 5)),
+        (r(2, 9, 5), r(2, 9, 5), None, r(2, 1, 5), None, r(2, 5))],
 }
 
 

@@ -84,6 +84,8 @@ def test_shapes_strides_and_alignment(dev):
     assert torch.equal(ops.matvec_int4(x, q, s.t().contiguous().t(), z.t().contiguous().t(), 64), ref)
     one = ops.matvec_int4(x[:1].expand(6, 300), q, s, z, 64)
     assert torch.equal(one, ref[:1].expand(6, 40))
+    windows = x.flatten()[:350].as_strided((6, 300), (10, 1))   # rows that overlap
+    assert torch.equal(ops.matvec_int4(windows, q, s, z, 64), ops.matvec_int4(windows.contiguous(), q, s, z, 64))
 
 
 @pytest.mark.parametrize("dev", DEVICES)
@@ -127,6 +129,17 @@ def test_quantize(dev, symmetric, k):
 
 
 @pytest.mark.gpu
+def test_more_rows_than_one_grid():
+    """16 x 65535 rows fill a grid dimension; the rows behind them get the bits of a small call."""
+    m = 16 * 65535 + 3
+    x, q, s, z = _inputs(1, 20, 64, 32, torch.bfloat16, "cuda")
+    x = torch.randn(m, 64, device="cuda", generator=torch.Generator("cuda").manual_seed(2)).bfloat16()
+    y = ops.matvec_int4(x, q, s, z, 32)
+    for at in (0, 16 * 65535 - 1, 16 * 65535, m - 1):
+        assert torch.equal(y[at:at + 1], ops.matvec_int4(x[at:at + 1], q, s, z, 32))
+
+
+@pytest.mark.gpu
 def test_stream_and_capture():
     x, q, s, z = _inputs(2, 512, 2048, 128, torch.bfloat16, "cuda")
     cap = CapturedCall(lambda v: ops.matvec_int4(v, q, s, z), x)
@@ -150,7 +163,9 @@ def test_refusals(dev):
            (ValueError, (x, q, s, z, 48)), (ValueError, (x, q, s, z, 0)), (ValueError, (x, q, s, z, -128)),
            (ValueError, (x[:, :60], q, s, z, 32)), (ValueError, (x, q, s[:, :1], z, 32)), (ValueError, (x, q, s, z.int(), 32)),
            (ValueError, (x, q, s, z[:4], 32)), (ValueError, (x, q.t().contiguous().t(), s, z, 32)),
-           (ValueError, (x, q[0], s, z, 32))]
+           (ValueError, (x, q[0], s, z, 32)), (ValueError, (x, q[:, :1].expand(8, 32), s, z, 32)),
+           (ValueError, (x, q[:1].expand(8, 32), s, z, 32)),
+           (ValueError, (x, torch.zeros(1, 64, dtype=torch.uint8, device=dev)[:, ::2], s[:1], z[:1], 32))]
     for err, args in bad:
         with pytest.raises(err):
             ops.matvec_int4(*args)
@@ -173,7 +188,7 @@ def test_native_refusals():
     def call(dtype=5, x=p, ldx=64, ldq=32, group=32, m=1, n=1, k=64):
         return lib.vs_matvec_int4(dtype, x, ldx, p, ldq, p, None, group, m, n, k, p, None)
     for kw in (dict(dtype=0), dict(group=48), dict(group=0), dict(m=-1), dict(n=-1), dict(k=-1), dict(x=None),
-               dict(m=2, ldx=63), dict(n=2, ldq=31), dict(n=1 << 40), dict(m=1 << 40)):
+               dict(m=2, ldx=63), dict(n=2, ldq=31), dict(n=1 << 40), dict(k=1 << 40), dict(m=1 << 40)):
         assert call(**kw) == 1 and b"matvec_int4" in lib.vs_last_error()
 
 

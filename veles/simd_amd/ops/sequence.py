@@ -297,7 +297,10 @@ def gated_recurrence_step(x: torch.Tensor, gate: torch.Tensor, state: torch.Tens
         raise RuntimeError("gated_recurrence_step records no gradient: call it under torch.no_grad(), or use "
                            "gated_recurrence")
     if plain_tensors(x, gate, state):
-        return _step_impl(x, gate, state)
+        y = _step_impl(x, gate, state)
+        if not state.is_inference():
+            torch.autograd.graph.increment_version(state)   # as the dispatcher does for an op that writes
+        return y
     return torch.ops.veles.gated_recurrence_step(x, gate, state)
 
 
@@ -323,8 +326,8 @@ def _check_matvec(name, x, qweight, scales, zeros, group_size):
         raise ValueError(f"{name}: scales {tuple(scales.shape)}, {groups} expected")
     if zeros is not None and (zeros.dtype != torch.uint8 or zeros.shape != groups):
         raise ValueError(f"{name}: zeros {zeros.dtype} {tuple(zeros.shape)}, uint8 {groups} expected")
-    if n > 1 and k > 2 and qweight.stride(1) != 1:
-        raise ValueError(f"{name}: the bytes of a row of qweight have to be neighbours")
+    if (qweight.shape[1] > 1 and qweight.stride(1) != 1) or (n > 1 and qweight.stride(0) < qweight.shape[1]):
+        raise ValueError(f"{name}: the bytes of a row of qweight have to be neighbours and rows apart")
     _same_device(name, x, qweight=qweight, scales=scales, zeros=zeros)
 
 
@@ -337,7 +340,7 @@ def _matvec_impl(x, qweight, scales, zeros, group_size):
         at = torch.arange(k) // group_size
         z = 8.0 if zeros is None else zeros.double()[:, at]
         return (x.double() @ ((q - z) * scales.double()[:, at]).t()).to(x.dtype)
-    rows = _as_rows(x)
+    rows = x if x.dim() == 2 and x.is_contiguous() else _near_rows(_as_rows(x), True)
     y = _new(x, *x.shape[:-1], n)
     scales = scales.contiguous()
     zeros = None if zeros is None else zeros.contiguous()
@@ -436,9 +439,16 @@ def _as_rows(x: torch.Tensor) -> torch.Tensor:
     return _rows_last(x)
 
 
-def _weight_rows(w: torch.Tensor) -> torch.Tensor:
-    w = _rows_last(w)
-    return w if w.shape[0] <= 1 or w.stride(0) >= w.shape[1] else w.contiguous()
+_LD_MAX = 1 << 21   # the tile kernel keeps 32-bit offsets over 256 rows
+
+
+def _near_rows(t: torch.Tensor, shared: bool) -> torch.Tensor:
+    """[rows, k] with a row stride that the kernels take: at least k (or 0 if `shared`), below _LD_MAX."""
+    t = _rows_last(t)
+    ld = t.stride(0)
+    if ld < _LD_MAX and (ld >= t.shape[1] or t.shape[0] <= 1 or (shared and ld == 0)):
+        return t
+    return t.contiguous() if t.shape[0] > 1 else t.reshape(-1).view(t.shape)
 
 
 def _act_cpu(kind, g):
@@ -462,13 +472,13 @@ def _gated_impl(x, w_gate, w_up, activation, save):
     name = "veles::gated_linear"
     _check_gated(name, x, w_gate, w_up, activation)
     f, k = w_gate.shape
-    rows = _as_rows(x)
+    rows = _near_rows(_as_rows(x), True)
     m = rows.shape[0]
     if not x.is_cuda:
         g, u = rows.double() @ w_gate.double().t(), rows.double() @ w_up.double().t()
         h = (_act_cpu(activation, g) * u).to(x.dtype).view(*x.shape[:-1], f)
         return h, torch.stack([g, u], -1).float() if save else None
-    w_gate, w_up = _weight_rows(w_gate), _weight_rows(w_up)
+    w_gate, w_up = _near_rows(w_gate, False), _near_rows(w_up, False)
     h = _new(x, *x.shape[:-1], f)
     pre = torch.empty((m, f, 2), dtype=torch.float32, device=x.device) if save else None
     size, ws = 0, None
@@ -490,7 +500,7 @@ def _gated_backward_impl(x, w_gate, w_up, pre, dh, activation, want_dx, want_dw)
     name = "veles::gated_linear_backward"
     _check_gated(name, x, w_gate, w_up, activation)
     f, k = w_gate.shape
-    rows, dhr = _as_rows(x), _as_rows(dh)
+    rows, dhr = _near_rows(_as_rows(x), True), _as_rows(dh)
     m = rows.shape[0]
     if dh.dtype != x.dtype or tuple(dh.shape) != (*x.shape[:-1], f):
         raise ValueError(f"{name}: dh is {dh.dtype} {tuple(dh.shape)}, {x.dtype} {(*x.shape[:-1], f)} expected")
@@ -503,7 +513,7 @@ def _gated_backward_impl(x, w_gate, w_up, pre, dh, activation, want_dx, want_dw)
         dx = (dg @ w_gate.double() + du @ w_up.double()).to(x.dtype).view(x.shape) if want_dx else x.new_empty(0)
         dw = torch.cat([dg.t() @ rows.double(), du.t() @ rows.double()]).to(x.dtype) if want_dw else x.new_empty(0)
         return dx, dw
-    w_gate, w_up, pre = _weight_rows(w_gate), _weight_rows(w_up), pre.contiguous()
+    w_gate, w_up, pre = _near_rows(w_gate, False), _near_rows(w_up, False), pre.contiguous()
     dx = torch.empty(x.shape if want_dx else (0,), dtype=x.dtype, device=x.device)
     dw = torch.empty((2 * f, k) if want_dw else (0,), dtype=x.dtype, device=x.device)
     size = int(_lib.lib().vs_gated_linear_backward_workspace(m, f, k, int(want_dx), int(want_dw)))
@@ -591,7 +601,7 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor,
     function), relu or sigmoid.  Sums, activation and product are float32 and rounded once.  Differentiable
     in x and the weights; the float32 pairs (x @ w_gate.T, x @ w_up.T), 8 bytes per output, are kept for the
     backward pass, and the gradients of the two products are rounded to x's type before they are
-    multiplied.  Up to 64 rows (generation) stream the weights once at memory speed."""
+    multiplied (the weights' gradients take up to 2^22 - 9 rows).  Up to 64 rows (generation) stream the weights once at memory speed."""
     save = records(x, w_gate, w_up)
     if plain_tensors(x, w_gate, w_up):
         if save:
