@@ -601,9 +601,9 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_kernel(Args p) {
       g += part[v][slot(0, c, t, r)][l];
       u += part[v][slot(1, c, t, r)][l];
     }
-    const int row = 16 * t + 4 * (l / 16) + r, col = n0 + 16 * c + l % 16;
-    if (row >= p.m || col >= p.n) continue;
-    const int64_t at = static_cast<int64_t>(row) * p.n + col;
+    const int m = 16 * t + 4 * (l / 16) + r, n = n0 + 16 * c + l % 16;
+    if (m >= p.m || n >= p.n) continue;
+    const int64_t at = static_cast<int64_t>(m) * p.n + n;
     p.c[at] = N::save(act(p.act, g) * u);
     if (p.pre) p.pre[at] = make_float2(g, u);
   }

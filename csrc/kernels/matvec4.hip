@@ -323,11 +323,11 @@ __global__ __launch_bounds__(64 * kWaves) void matvec4_kernel(Args p) {
   __syncthreads();
   for (int i = threadIdx.x; i < CT * RV * 64; i += 64 * kWaves) {
     const int c = i / (RV * 64), r = i / 64 % RV, l = i % 64;
-    float v = 0.f;
+    float total = 0.f;
 #pragma unroll
-    for (int w = 0; w < kWaves; w++) v += lds.part[w][c][r][l];
+    for (int w = 0; w < kWaves; w++) total += lds.part[w][c][r][l];
     const int mm = m0 + l / 16 + 4 * r, nn = n0 + 16 * c + l % 16;
-    if (mm < p.m && nn < p.n) p.y[static_cast<int64_t>(mm) * p.n + nn] = N::save(v);
+    if (mm < p.m && nn < p.n) p.y[static_cast<int64_t>(mm) * p.n + nn] = N::save(total);
   }
 }
 

@@ -35,7 +35,7 @@ struct F16 {
   }
 };
 
-// One value, or two neighbouring 16-bit values in one register, as they lie in memory.
+// One value, or two neighbouring 16-bit values in one register, as they lie in memory; set in order.
 template <class N, int V>
 struct Pack;
 template <class N>
@@ -51,8 +51,8 @@ struct Pack<N, 2> {
     return N::load(static_cast<uint16_t>(i ? w >> 16 : w));
   }
   __device__ __forceinline__ void set(int i, float f) {
-    w = i ? (w & 0xffffu) | (static_cast<uint32_t>(N::save(f)) << 16)
-          : (w & 0xffff0000u) | N::save(f);
+    if (i == 0) w = N::save(f);
+    else w |= static_cast<uint32_t>(N::save(f)) << 16;
   }
 };
 
