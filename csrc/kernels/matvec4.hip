@@ -124,8 +124,11 @@ __device__ __forceinline__ void transpose(uint32_t (&w)[4]) {
 // the end the last step again): a load under a condition would make the compiler wait for all.
 // Four neighbouring lanes load the 64 bytes of one row and the fragments are formed through LDS: a
 // load in fragment order (16 rows in 16 neighbouring lanes) costs the cache four times the lookups.
+// Two waves a SIMD have to fit (28000 x 8192 g32, 16 rows: 43 us, 55 where the compiler took more
+// registers).  (Forming the next step's fragments while a step multiplies needs more registers
+// than it hides: 36 us against 34 for one row of 28000 x 8192 g64, where the loads alone take 26.)
 template <class N, int kWaves, int CT, int GS, int RV>
-__global__ __launch_bounds__(64 * kWaves) void matvec4_kernel(Args p) {
+__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))) void matvec4_kernel(Args p) {
   constexpr int NG = 4 / GS;                 // groups in a step
   constexpr int kStage = 8;                  // steps whose scales a wave keeps in LDS
   constexpr int kCols = 16 * CT, kSlots = kStage * NG;
