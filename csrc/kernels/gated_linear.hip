@@ -107,10 +107,11 @@ struct Work {
 
 // A tile of 2 (rows) x 4 (columns) waves, each with 2 x 2 quadrants of 16 XH x 16 YH products.
 // GATED: the column quadrants are Wg and Wu of the same outputs.
-template <int XH_, int YH_, bool GATED_>
+// SAVE: of the gated product, (g, u) are results too.
+template <int XH_, int YH_, bool GATED_, bool SAVE_ = false>
 struct Cfg {
   static constexpr int XH = XH_, YH = YH_, BK = 64;
-  static constexpr bool GATED = GATED_;
+  static constexpr bool GATED = GATED_, SAVE = SAVE_;
   static constexpr int BM = 64 * XH, BN = 128 * YH;    // products
   static constexpr int BO = GATED ? BN / 2 : BN;       // output columns
   static constexpr int kThreads = 512;
@@ -292,7 +293,9 @@ __global__ __launch_bounds__(512) void tile_kernel(Work work) {
     }
   };
   // Weights are the matrix instruction's first operand, so a lane ends with four neighbouring
-  // columns (4 lq + r of the 16) of one row (l16) of the result.
+  // columns (4 lq + r of the 16) of one row (l16) of the result.  SAVE: they are the second, and a
+  // lane ends with four rows of one column, since the pairs are most of what is written then and 16
+  // neighbouring lanes' pairs are 128 neighbouring bytes.
   floatx4 acc[2][XH][2][YH];
   const auto multiply = [&](auto ih, auto jh) {
     constexpr int i = decltype(ih)::value, j = decltype(jh)::value;
@@ -303,7 +306,8 @@ __global__ __launch_bounds__(512) void tile_kernel(Work work) {
       for (int x = 0; x < XH; x++)
 #pragma unroll
         for (int y = 0; y < YH; y++)
-          acc[i][x][j][y] = mma<N>(fb[j][y][ks], fa[x][ks], acc[i][x][j][y]);
+          acc[i][x][j][y] = C::SAVE ? mma<N>(fa[x][ks], fb[j][y][ks], acc[i][x][j][y])
+                                    : mma<N>(fb[j][y][ks], fa[x][ks], acc[i][x][j][y]);
     __builtin_amdgcn_s_setprio(0);
   };
   constexpr std::integral_constant<int, 0> c0{};
@@ -375,13 +379,45 @@ __global__ __launch_bounds__(512) void tile_kernel(Work work) {
     if (wid < 4) meet();
     wait_vmcnt<0>();  // the pieces started past the end of k have written their zeros
     meet();
-    const int rm = m0 + wm * (32 * XH) + l16, rn = n0 + wn * (C::GATED ? 16 * YH : 32 * YH);
+    const int rm = m0 + wm * (32 * XH), rn = n0 + wn * (C::GATED ? 16 * YH : 32 * YH);
     tile += gridDim.x;
     if (tile < work.tiles) {
       place(tile);
       start_tile();
     }
 
+    if constexpr (C::SAVE) {
+      // Odd and even lanes exchange, so that a lane stores two columns of h: of rows r and r + 1 the
+      // even lane takes the first.
+#pragma unroll
+      for (int i = 0; i < 2; i++)
+#pragma unroll
+        for (int x = 0; x < XH; x++)
+#pragma unroll
+          for (int b = 0; b < YH; b++) {
+            const int row = rm + (i * XH + x) * 16 + 4 * lq, col = rn + 16 * b + l16;
+            const floatx4 g = acc[i][x][0][b], u = acc[i][x][1][b];
+            float2 *pre = p.pre + static_cast<int64_t>(row) * p.n + col;
+            const int odd = lane & 1;
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+              if (row + r < p.m && col < p.n) pre[static_cast<int64_t>(r) * p.n] = make_float2(g[r], u[r]);
+#pragma unroll
+            for (int r = 0; r < 4; r += 2) {
+              const uint32_t v0 = N::save(act(p.act, g[r]) * u[r]);
+              const uint32_t v1 = N::save(act(p.act, g[r + 1]) * u[r + 1]);
+              const uint32_t give = odd ? v0 : v1;
+              const uint32_t take = __builtin_amdgcn_update_dpp(0u, give, 0xb1, 0xf, 0xf, true);
+              const uint32_t w = odd ? take | v1 << 16 : v0 | take << 16;
+              if (row + r + odd >= p.m) continue;
+              uint16_t *out = p.c + static_cast<int64_t>(row + r + odd) * p.n + (col - odd);
+              if (col - odd + 1 < p.n) __builtin_memcpy(out, &w, 4);
+              else if (col - odd < p.n) *out = static_cast<uint16_t>(w);
+            }
+          }
+      if (tile >= work.tiles) return;
+      continue;
+    }
     // Results: rows of 16-bit values, two neighbouring 16-column blocks exchanged between odd and
     // even lane groups where there are two, so a lane stores 16 bytes.
     constexpr int NB = C::GATED ? YH : 2 * YH;
@@ -400,7 +436,7 @@ __global__ __launch_bounds__(512) void tile_kernel(Work work) {
     for (int i = 0; i < 2; i++)
 #pragma unroll
       for (int x = 0; x < XH; x++) {
-        const int row = rm + (i * XH + x) * 16;
+        const int row = rm + (i * XH + x) * 16 + l16;
         uint32_t w[NB][2];
 #pragma unroll
         for (int b = 0; b < NB; b++) {
@@ -412,18 +448,6 @@ __global__ __launch_bounds__(512) void tile_kernel(Work work) {
           }
           w[b][0] = N::save(v[0]) | static_cast<uint32_t>(N::save(v[1])) << 16;
           w[b][1] = N::save(v[2]) | static_cast<uint32_t>(N::save(v[3])) << 16;
-          if constexpr (C::GATED)
-            if (p.pre && row < p.m) {
-              const int col = rn + 16 * b + 4 * lq;
-              float2 *dst = p.pre + static_cast<int64_t>(row) * p.n + col;
-#pragma unroll
-              for (int r = 0; r < 4; r += 2) {
-                const float4 gu = {acc[i][x][0][b][r], acc[i][x][1][b][r], acc[i][x][0][b][r + 1],
-                                   acc[i][x][1][b][r + 1]};
-                if (col + r + 1 < p.n) __builtin_memcpy(dst + r, &gu, 16);
-                else if (col + r < p.n) dst[r] = make_float2(gu.x, gu.y);
-              }
-            }
         }
         if (row >= p.m) continue;
         uint16_t *out = p.c + static_cast<int64_t>(row) * p.n;
@@ -841,11 +865,11 @@ double estimate(const Args *q, int count) {
   return count == 1 ? t : std::max(longest, total);
 }
 
-template <class N, bool GATED>
+template <class N, bool GATED, bool SAVE>
 vs_status product(const Args *q, int count, hipStream_t s) {
-  using Large = Cfg<4, 2, GATED>;
-  using Wide = Cfg<2, 2, GATED>;
-  using Small = Cfg<2, 1, GATED>;
+  using Large = Cfg<4, 2, GATED, SAVE>;
+  using Wide = Cfg<2, 2, GATED, SAVE>;
+  using Small = Cfg<2, 1, GATED, SAVE>;
   const double l = estimate<Large>(q, count), w = estimate<Wide>(q, count), sm = estimate<Small>(q, count);
   if (l <= w && l <= sm) return launch_tile<N, Large>(q, count, s);
   if (w <= sm) return launch_tile<N, Wide>(q, count, s);
@@ -973,7 +997,7 @@ vs_status forward(Args p, void *workspace, size_t bytes, hipStream_t s) {
     VS_HIP(hipGetLastError());
   }
   p.k = kp;  // (the same where nothing was copied: a direct operand has whole pieces)
-  return product<N, true>(&p, 1, s);
+  return p.pre ? product<N, true, true>(&p, 1, s) : product<N, true, false>(&p, 1, s);
 }
 
 size_t backward_need(int64_t m, int64_t f, int64_t k, bool dx, bool dw) {
@@ -1053,7 +1077,7 @@ vs_status backward(const uint16_t *x, int64_t ldx, const uint16_t *wg, int64_t l
     VS_HIP(hipGetLastError());
   }
   if (count == 2 && q[1].k > q[0].k) std::swap(q[0], q[1]);
-  return count ? product<N, false>(q, count, s) : VS_OK;
+  return count ? product<N, false, false>(q, count, s) : VS_OK;
 }
 
 }  // namespace
