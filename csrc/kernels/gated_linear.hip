@@ -97,6 +97,10 @@ struct Args {
   uint16_t *c;            // [m][n], row stride n
   float2 *pre;            // [m][n] (g, u), or null
   int act;
+  // k in `parts` parts of `k_part` (a multiple of 64) when `parts` > 1: part i's sums, fp32 (pairs of
+  // the gated product), go to sums + i m n and the join kernel adds them
+  int parts, k_part;
+  float *sums;
 };
 
 // One or two products in a launch: tiles [0, first) belong to q[0], the rest to q[1].
@@ -107,7 +111,7 @@ struct Work {
 
 // A tile of 2 (rows) x 4 (columns) waves, each with 2 x 2 quadrants of 16 XH x 16 YH products.
 // GATED: the column quadrants are Wg and Wu of the same outputs.
-// SAVE: of the gated product, (g, u) are results too.
+// SAVE: of the gated product, (g, u) are results too (or the only ones: parts of the sums).
 template <int XH_, int YH_, bool GATED_, bool SAVE_ = false>
 struct Cfg {
   static constexpr int XH = XH_, YH = YH_, BK = 64;
@@ -207,16 +211,20 @@ __global__ __launch_bounds__(512) void tile_kernel(Work work) {
   const int wm = wid / 4, wn = wid % 4;
   const int l16 = lane & 15, lq = lane >> 4;
 
-  int m0, n0;
+  int m0, n0, part, k;  // of the tile: first row and column, part and length of k
   __amdgpu_buffer_rsrc_t ra, rb0, rb1;
   const auto place = [&](unsigned tile) {
     unsigned tm, tn;
-    dev::grouped_tile(dev::xcd_remap(tile - begin, tiles_m * tiles_n), tiles_m, tiles_n, tm, tn);
+    const unsigned at = dev::xcd_remap(tile - begin, tiles_m * tiles_n * p.parts);
+    part = at / (tiles_m * tiles_n);
+    dev::grouped_tile(at - part * (tiles_m * tiles_n), tiles_m, tiles_n, tm, tn);
     m0 = tm * C::BM;
     n0 = tn * C::BO;
-    ra = rows_of(p.a, p.lda, m0, p.m, C::BM, p.k);
-    rb0 = rows_of(p.b[0], p.ldb[0], n0, p.n, C::BO, p.k);
-    rb1 = C::GATED ? rows_of(p.b[1], p.ldb[1], n0, p.n, C::BO, p.k) : rb0;
+    const int k0 = part * p.k_part;
+    k = p.k - k0 < p.k_part ? p.k - k0 : p.k_part;
+    ra = rows_of(p.a + k0, p.lda, m0, p.m, C::BM, k);
+    rb0 = rows_of(p.b[0] + k0, p.ldb[0], n0, p.n, C::BO, k);
+    rb1 = C::GATED ? rows_of(p.b[1] + k0, p.ldb[1], n0, p.n, C::BO, k) : rb0;
   };
   // Image row r of A half h is row 32 XH (r / 16 XH) + 16 XH h + r % 16 XH of the tile; of B half
   // h it is the same with YH and four waves (GATED: row r of operand h).  Piece i of a wave: image rows
@@ -246,19 +254,19 @@ __global__ __launch_bounds__(512) void tile_kernel(Work work) {
   const auto start_a = [&](auto half, auto buf, int tile) {
     constexpr int h = decltype(half)::value;
     uint8_t *dst = lds + decltype(buf)::value * C::kBuf + h * C::kHalfA + wid * (C::PA * 1024);
-    const int k0 = tile * C::BK, at = k0 < p.k ? 2 * k0 : 0;  // (at stays inside the range)
+    const int k0 = tile * C::BK, at = k0 < k ? 2 * k0 : 0;  // (at stays inside the range)
 #pragma unroll
     for (int i = 0; i < C::PA; i++)
-      dma16(ra, dst + i * 1024, ka[i] < p.k - k0 ? offa[h][i] : kOut, at);
+      dma16(ra, dst + i * 1024, ka[i] < k - k0 ? offa[h][i] : kOut, at);
   };
   const auto start_b = [&](auto half, auto buf, int tile) {
     constexpr int h = decltype(half)::value;
     uint8_t *dst = lds + decltype(buf)::value * C::kBuf + 2 * C::kHalfA + h * C::kHalfB +
                    wid * (C::PB * 1024);
-    const int k0 = tile * C::BK, at = k0 < p.k ? 2 * k0 : 0;
+    const int k0 = tile * C::BK, at = k0 < k ? 2 * k0 : 0;
 #pragma unroll
     for (int i = 0; i < C::PB; i++)
-      dma16(h ? rb1 : rb0, dst + i * 1024, kb[i] < p.k - k0 ? offb[h][i] : kOut, at);
+      dma16(h ? rb1 : rb0, dst + i * 1024, kb[i] < k - k0 ? offb[h][i] : kOut, at);
   };
   // LDS addresses of this lane's fragments [buffer][32-deep step]
   uint32_t ata[2][2], atb[2][2];
@@ -354,7 +362,6 @@ __global__ __launch_bounds__(512) void tile_kernel(Work work) {
     start_b(c0, c1, 1);
     start_a(c1, c1, 1);
   };
-  const int nk = (p.k + C::BK - 1) / C::BK;
   place(blockIdx.x);
   start_tile();
   for (unsigned tile = blockIdx.x;;) {
@@ -372,7 +379,7 @@ __global__ __launch_bounds__(512) void tile_kernel(Work work) {
     settle<YH>(fb[0]);
     meet();
     if (wid >= 4) meet();
-    for (int t = 0; t < nk; t += 2) {
+    for (int t = 0; t * C::BK < k; t += 2) {
       phases(c0, c1, c0, c1, t);
       phases(c1, c0, c1, c0, t + 1);
     }
@@ -380,6 +387,7 @@ __global__ __launch_bounds__(512) void tile_kernel(Work work) {
     wait_vmcnt<0>();  // the pieces started past the end of k have written their zeros
     meet();
     const int rm = m0 + wm * (32 * XH), rn = n0 + wn * (C::GATED ? 16 * YH : 32 * YH);
+    const int64_t skip = static_cast<int64_t>(part) * p.m * p.n;  // where the sums of this part begin
     tile += gridDim.x;
     if (tile < work.tiles) {
       place(tile);
@@ -397,11 +405,13 @@ __global__ __launch_bounds__(512) void tile_kernel(Work work) {
           for (int b = 0; b < YH; b++) {
             const int row = rm + (i * XH + x) * 16 + 4 * lq, col = rn + 16 * b + l16;
             const floatx4 g = acc[i][x][0][b], u = acc[i][x][1][b];
-            float2 *pre = p.pre + static_cast<int64_t>(row) * p.n + col;
+            float2 *pre = (p.parts > 1 ? reinterpret_cast<float2 *>(p.sums) + skip : p.pre) +
+                          static_cast<int64_t>(row) * p.n + col;
             const int odd = lane & 1;
 #pragma unroll
             for (int r = 0; r < 4; r++)
               if (row + r < p.m && col < p.n) pre[static_cast<int64_t>(r) * p.n] = make_float2(g[r], u[r]);
+            if (p.parts > 1) continue;
 #pragma unroll
             for (int r = 0; r < 4; r += 2) {
               const uint32_t v0 = N::save(act(p.act, g[r]) * u[r]);
@@ -418,6 +428,29 @@ __global__ __launch_bounds__(512) void tile_kernel(Work work) {
       if (tile >= work.tiles) return;
       continue;
     }
+    if constexpr (!C::GATED)
+      if (p.parts > 1) {
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+#pragma unroll
+          for (int x = 0; x < XH; x++)
+#pragma unroll
+            for (int b = 0; b < 2 * YH; b++) {
+              const int row = rm + (i * XH + x) * 16 + l16, col = rn + 16 * b + 4 * lq;
+              float *dst = p.sums + skip + static_cast<int64_t>(row) * p.n + col;
+              const floatx4 v = acc[i][x][b / YH][b % YH];
+              if (row >= p.m) continue;
+              if (col + 4 <= p.n) {
+                __builtin_memcpy(dst, &v, 16);
+              } else {
+#pragma unroll
+                for (int r = 0; r < 3; r++)
+                  if (col + r < p.n) dst[r] = v[r];
+              }
+            }
+        if (tile >= work.tiles) return;
+        continue;
+      }
     // Results: rows of 16-bit values, two neighbouring 16-column blocks exchanged between odd and
     // even lane groups where there are two, so a lane stores 16 bytes.
     constexpr int NB = C::GATED ? YH : 2 * YH;
@@ -466,6 +499,47 @@ __global__ __launch_bounds__(512) void tile_kernel(Work work) {
         }
       }
     if (tile >= work.tiles) return;
+  }
+}
+
+// Adds the parts of up to two products, in order.  One thread per four results.
+struct Join {
+  Args q[2];
+  int64_t fours[2];
+};
+template <class N, bool GATED>
+__global__ __launch_bounds__(256) void join_kernel(Join j) {
+  for (int64_t at = blockIdx.x * 256ll + threadIdx.x; at < j.fours[0] + j.fours[1];
+       at += gridDim.x * 256ll) {
+    const int w = at < j.fours[0] ? 0 : 1;
+    const Args &p = j.q[w];
+    const int64_t size = static_cast<int64_t>(p.m) * p.n, i = 4 * (w ? at - j.fours[0] : at);
+    constexpr int V = GATED ? 2 : 1;
+    float sum[4 * V] = {};
+    const int have = size - i < 4 ? static_cast<int>(size - i) : 4;
+    const float *src = p.sums + V * i;
+    for (int s = 0; s < p.parts; s++, src += V * size) {
+      if (have == 4) {
+        float v[4 * V];
+        __builtin_memcpy(v, src, sizeof(v));
+#pragma unroll
+        for (int e = 0; e < 4 * V; e++) sum[e] += v[e];
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4 * V; e++)
+          if (e < V * have) sum[e] += src[e];
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      if (e >= have) continue;
+      if constexpr (GATED) {
+        p.c[i + e] = N::save(act(p.act, sum[2 * e]) * sum[2 * e + 1]);
+        if (p.pre) p.pre[i + e] = make_float2(sum[2 * e], sum[2 * e + 1]);
+      } else {
+        p.c[i + e] = N::save(sum[e]);
+      }
+    }
   }
 }
 
@@ -812,9 +886,11 @@ bool direct(const void *p, int64_t ld, int64_t k) {
   return k % 8 == 0 && ld % 8 == 0 && reinterpret_cast<uintptr_t>(p) % 16 == 0;
 }
 
+int k_tiles(const Args &p) { return (std::min(p.k, p.k_part) + 63) / 64; }
+
 template <class C>
 int64_t tiles_of(const Args &p) {
-  return static_cast<int64_t>((p.m + C::BM - 1) / C::BM) * ((p.n + C::BO - 1) / C::BO);
+  return static_cast<int64_t>((p.m + C::BM - 1) / C::BM) * ((p.n + C::BO - 1) / C::BO) * p.parts;
 }
 
 template <class N, class C>
@@ -854,7 +930,7 @@ double estimate(const Args *q, int count) {
   const double slots = device_cu_count() * (160 * 1024 / C::kLds);
   double total = 0, longest = 0, t = 0;
   for (int i = 0; i < count; i++) {
-    const double nk = (q[i].k + C::BK - 1) / C::BK, n = static_cast<double>(tiles_of<C>(q[i]));
+    const double nk = k_tiles(q[i]), n = static_cast<double>(tiles_of<C>(q[i]));
     const int64_t rounds = static_cast<int64_t>(n / slots);
     const double rest = n - static_cast<double>(rounds) * slots;
     t = static_cast<double>(rounds) * (fixed + step * nk) +
@@ -865,15 +941,80 @@ double estimate(const Args *q, int count) {
   return count == 1 ? t : std::max(longest, total);
 }
 
+// Few tiles and a long k leave most of the chip idle: then k is cut, the parts' sums go through memory
+// in fp32, and another launch adds them, which takes about 4 us and reads what was written at
+// about 4 TB/s.  Parts are doubled for the product with the longest tiles as long as the estimate
+// falls.  us in one part and as chosen, bf16: 300 x 8192 to 200 outputs 65 and 20, the backward pass of
+// 64 x 2048 with 16384 outputs 333 and 142, of 8192 x 256 with 256 outputs 79 and 30.
+size_t sums_bytes(const Args &p, bool gated) {
+  return p.parts > 1 ? up256(static_cast<size_t>(gated ? 8 : 4) * p.parts * p.m * p.n) : 0;
+}
+template <class C>
+double cut(Args *q, int count) {
+  const auto cost = [&] {
+    const double bytes = static_cast<double>(sums_bytes(q[0], C::GATED) + (count > 1 ? sums_bytes(q[1], C::GATED) : 0));
+    double memory = 0;  // the operands once
+    for (int i = 0; i < count; i++) memory += 2.0 * q[i].k * (q[i].m + (C::GATED ? 2.0 : 1.0) * q[i].n) / 5e6;
+    const double time = estimate<C>(q, count);
+    return std::max(time, memory) + 0.01 * time + (bytes > 0 ? 4 + bytes / 2e6 : 0);
+  };
+  for (int i = 0; i < count; i++) q[i].parts = 1, q[i].k_part = std::max(q[i].k, 1);
+  double best = cost();
+  for (;;) {
+    const int i = count == 2 && k_tiles(q[1]) > k_tiles(q[0]) ? 1 : 0;
+    const Args before = q[i];
+    if (k_tiles(before) < 8 || before.parts >= 32) return best;
+    q[i].k_part = (k_tiles(before) + 1) / 2 * 64;
+    q[i].parts = (q[i].k + q[i].k_part - 1) / q[i].k_part;
+    const double now = cost();
+    if (now >= best) {
+      q[i] = before;
+      return best;
+    }
+    best = now;
+  }
+}
+
+// Tile shape (0: 256 x 256, 1: 128 x 256, 2: 128 x 128) and the parts of each product.
+template <bool GATED>
+int plan(Args *q, int count) {
+  Args w[2], s[2];
+  for (int i = 0; i < count; i++) w[i] = s[i] = q[i];
+  const double large = cut<Cfg<4, 2, GATED>>(q, count), wide = cut<Cfg<2, 2, GATED>>(w, count),
+               small = cut<Cfg<2, 1, GATED>>(s, count);
+  if (large <= wide && large <= small) return 0;
+  for (int i = 0; i < count; i++) q[i] = wide <= small ? w[i] : s[i];
+  return wide <= small ? 1 : 2;
+}
+
 template <class N, bool GATED, bool SAVE>
-vs_status product(const Args *q, int count, hipStream_t s) {
-  using Large = Cfg<4, 2, GATED, SAVE>;
-  using Wide = Cfg<2, 2, GATED, SAVE>;
-  using Small = Cfg<2, 1, GATED, SAVE>;
-  const double l = estimate<Large>(q, count), w = estimate<Wide>(q, count), sm = estimate<Small>(q, count);
-  if (l <= w && l <= sm) return launch_tile<N, Large>(q, count, s);
-  if (w <= sm) return launch_tile<N, Wide>(q, count, s);
-  return launch_tile<N, Small>(q, count, s);
+vs_status launch_shape(int shape, const Args *q, int count, hipStream_t s) {
+  if (shape == 0) return launch_tile<N, Cfg<4, 2, GATED, SAVE>>(q, count, s);
+  if (shape == 1) return launch_tile<N, Cfg<2, 2, GATED, SAVE>>(q, count, s);
+  return launch_tile<N, Cfg<2, 1, GATED, SAVE>>(q, count, s);
+}
+
+template <class N, bool GATED>
+vs_status product(int shape, const Args *q, int count, hipStream_t s) {
+  if constexpr (GATED) {
+    if (q->pre || q->parts > 1) VS_TRY((launch_shape<N, true, true>(shape, q, count, s)));
+    else VS_TRY((launch_shape<N, true, false>(shape, q, count, s)));
+  } else {
+    VS_TRY((launch_shape<N, false, false>(shape, q, count, s)));
+  }
+  Join j{};
+  int n = 0;
+  for (int i = 0; i < count; i++)
+    if (q[i].parts > 1) {
+      j.fours[n] = (static_cast<int64_t>(q[i].m) * q[i].n + 3) / 4;
+      j.q[n++] = q[i];
+    }
+  if (const int64_t all = j.fours[0] + j.fours[1]) {
+    const unsigned grid = static_cast<unsigned>(std::min<int64_t>((all + 255) / 256, 1 << 20));
+    hipLaunchKernelGGL((join_kernel<N, GATED>), dim3(grid), dim3(256), 0, s, j);
+    VS_HIP(hipGetLastError());
+  }
+  return VS_OK;
 }
 
 // Bump allocator over the caller's workspace or the library's pool.
@@ -885,6 +1026,7 @@ struct Space {
     used += up256(2 * elems);
     return reinterpret_cast<uint16_t *>(p);
   }
+  float *take_sums(size_t bytes) { return reinterpret_cast<float *>(take(bytes / 2)); }
 };
 
 vs_status open_space(Space &sp, DeviceBuffer &own, void *workspace, size_t bytes, size_t need,
@@ -913,16 +1055,19 @@ vs_status check(const char *who, int dtype, int act, int64_t m, int64_t f, int64
 
 struct ForwardNeed {
   bool px, pg, pu;  // copies to rows that the DMA can read
-  size_t bytes;
+  int shape;
+  size_t sums, bytes;
 };
-ForwardNeed forward_need(int64_t m, int64_t f, int64_t k, bool dx, bool dg, bool du) {
+// Sets p's parts as well.
+ForwardNeed forward_need(Args &p, bool dx, bool dg, bool du) {
   ForwardNeed q{};
-  if (m <= kFewRows) return q;
   q.px = !dx;
   q.pg = !dg;
   q.pu = !du;
-  const size_t kp = up8(k);
-  q.bytes = (q.px ? up256(2 * m * kp) : 0) + ((q.pg ? 1 : 0) + (q.pu ? 1 : 0)) * up256(2 * f * kp);
+  const size_t kp = up8(p.k);
+  q.shape = plan<true>(&p, 1);
+  q.sums = sums_bytes(p, true);
+  q.bytes = q.sums + (q.px ? up256(2 * p.m * kp) : 0) + ((q.pg ? 1 : 0) + (q.pu ? 1 : 0)) * up256(2 * p.n * kp);
   return q;
 }
 
@@ -947,7 +1092,10 @@ int few_columns(const Args &p, bool all_direct) {
     return 3 + std::max(memory, rounds * (64.0 * ct + 32.0 * rt) * p.k / 40e3);
   };
   const double one = few(1), two = few(2);
-  const double tile = 5 + std::max(estimate<Cfg<2, 1, true>>(&p, 1), 4.0 * p.n * p.k / 4.6e6);
+  Args one_part = p;
+  one_part.parts = 1;
+  one_part.k_part = std::max(p.k, 1);
+  const double tile = 5 + std::max(estimate<Cfg<2, 1, true>>(&one_part, 1), 4.0 * p.n * p.k / 4.6e6);
   if (all_direct && tile < std::min(one, two)) return 0;
   return one <= two ? 1 : 2;
 }
@@ -971,7 +1119,7 @@ vs_status forward(Args p, void *workspace, size_t bytes, hipStream_t s) {
       return VS_OK;
     }
   }
-  const ForwardNeed q = forward_need(p.m, p.n, p.k, da, dg, du);
+  const ForwardNeed q = forward_need(p, da, dg, du);
   DeviceBuffer own;
   Space sp;
   VS_TRY(open_space(sp, own, workspace, bytes, q.bytes, s));
@@ -996,14 +1144,39 @@ vs_status forward(Args p, void *workspace, size_t bytes, hipStream_t s) {
     hipLaunchKernelGGL(pad_kernel, dim3(grid), dim3(256), 0, s, pd);
     VS_HIP(hipGetLastError());
   }
+  if (q.sums) p.sums = sp.take_sums(q.sums);
   p.k = kp;  // (the same where nothing was copied: a direct operand has whole pieces)
-  return p.pre ? product<N, true, true>(&p, 1, s) : product<N, true, false>(&p, 1, s);
+  if (p.parts == 1) p.k_part = kp;
+  return product<N, true>(q.shape, &p, 1, s);
 }
 
-size_t backward_need(int64_t m, int64_t f, int64_t k, bool dx, bool dw) {
+// The backward products' sizes, the longer k first: dx = [dg du] [Wg; Wu] and dw = [dg du]^T x.
+struct BackwardNeed {
+  Args q[2];
+  int count, shape;
+  int dx, dw;  // which of q each is, or -1
+  size_t bytes;
+};
+BackwardNeed backward_need(int64_t m, int64_t f, int64_t k, bool dx, bool dw) {
+  BackwardNeed b{};
   const size_t fp = up8(f), mp = up8(m);
-  return (dx ? up256(2 * m * 2 * fp) + up256(2 * k * 2 * fp) : 0) +
-         (dw ? up256(2 * 2 * f * mp) + up256(2 * k * mp) : 0);
+  const auto add = [&](int64_t rows, int64_t inner) {
+    Args &p = b.q[b.count];
+    p.m = static_cast<int>(rows);
+    p.n = static_cast<int>(k);
+    p.k = static_cast<int>(inner);
+    return b.count++;
+  };
+  b.dx = b.dw = -1;
+  const bool first = 2 * fp >= mp;
+  if (dx && m && first) b.dx = add(m, 2 * fp);
+  if (dw && f) b.dw = add(2 * f, mp);
+  if (dx && m && !first) b.dx = add(m, 2 * fp);
+  b.bytes = (dx ? up256(2 * m * 2 * fp) + up256(2 * k * 2 * fp) : 0) +
+            (dw ? up256(2 * 2 * f * mp) + up256(2 * k * mp) : 0);
+  if (b.count) b.shape = plan<false>(b.q, b.count);
+  for (int i = 0; i < b.count; i++) b.bytes += sums_bytes(b.q[i], false);
+  return b;
 }
 
 template <class N>
@@ -1013,7 +1186,8 @@ vs_status backward(const uint16_t *x, int64_t ldx, const uint16_t *wg, int64_t l
                    void *workspace, size_t bytes, hipStream_t s) {
   DeviceBuffer own;
   Space sp;
-  VS_TRY(open_space(sp, own, workspace, bytes, backward_need(m, f, k, dx, dw), s));
+  BackwardNeed need = backward_need(m, f, k, dx, dw);
+  VS_TRY(open_space(sp, own, workspace, bytes, need.bytes, s));
   const int fp = up8(f), mp = up8(m);
   uint16_t *rows = dx ? sp.take(static_cast<size_t>(m) * 2 * fp) : nullptr;
   uint16_t *wt = dx ? sp.take(static_cast<size_t>(k) * 2 * fp) : nullptr;
@@ -1042,42 +1216,28 @@ vs_status backward(const uint16_t *x, int64_t ldx, const uint16_t *wg, int64_t l
     t.tiles = static_cast<unsigned>(std::min<int64_t>(n, 1ll << 23));
     blocks += n;
   };
-  Args q[2] = {};
-  int count = 0;
   if (dx) {
     turn(wg, ldg, f, k, wt, 2 * fp, fp);
     turn(wu, ldu, f, k, wt + fp, 2 * fp, fp);
-    if (m) {
-      Args &p = q[count++];
-      p.a = rows;
-      p.b[0] = wt;
-      p.lda = p.ldb[0] = 2 * fp;
-      p.m = m;
-      p.n = k;
-      p.k = 2 * fp;
-      p.c = dx;
-    }
   }
-  if (dw) {
-    turn(x, ldx, m, k, xt, mp, mp);
-    if (f) {
-      Args &p = q[count++];
-      p.a = cols;
-      p.b[0] = xt;
-      p.lda = p.ldb[0] = mp;
-      p.m = 2 * f;
-      p.n = k;
-      p.k = mp;
-      p.c = dw;
-    }
-  }
+  if (dw) turn(x, ldx, m, k, xt, mp, mp);
+  const auto set = [&](int i, const uint16_t *a, const uint16_t *b, uint16_t *c) {
+    if (i < 0) return;
+    Args &p = need.q[i];
+    p.a = a;
+    p.b[0] = b;
+    p.lda = p.ldb[0] = p.k;
+    p.c = c;
+    if (const size_t sums = sums_bytes(p, false)) p.sums = sp.take_sums(sums);
+  };
+  set(need.dx, rows, wt, dx);
+  set(need.dw, cols, xt, dw);
   VS_REQUIRE(blocks < (1ll << 23), "gated_linear: too many tiles");
   if (blocks) {
     hipLaunchKernelGGL((prepare_kernel<N>), dim3(static_cast<unsigned>(blocks)), dim3(256), 0, s, pr);
     VS_HIP(hipGetLastError());
   }
-  if (count == 2 && q[1].k > q[0].k) std::swap(q[0], q[1]);
-  return count ? product<N, false, false>(q, count, s) : VS_OK;
+  return need.count ? product<N, false>(need.shape, need.q, need.count, s) : VS_OK;
 }
 
 }  // namespace
@@ -1088,9 +1248,14 @@ using namespace vs;
 
 extern "C" {
 
-size_t vs_gated_linear_workspace(int64_t m, int64_t f, int64_t k) {
-  if (glin::check("", VS_BF16, 0, m, f, k) != VS_OK) return 0;
-  return glin::forward_need(m, f, k, false, false, false).bytes;
+size_t vs_gated_linear_workspace(int64_t m, int64_t f, int64_t k, int aligned) {
+  if (glin::check("", VS_BF16, 0, m, f, k) != VS_OK || m == 0 || f == 0) return 0;
+  glin::Args p{};
+  p.m = static_cast<int>(m);
+  p.n = static_cast<int>(f);
+  p.k = static_cast<int>(k);
+  if (m <= glin::kFewRows && glin::few_columns(p, aligned != 0)) return 0;
+  return glin::forward_need(p, aligned != 0, aligned != 0, aligned != 0).bytes;
 }
 
 vs_status vs_gated_linear(int dtype, int act, const void *x, int64_t ldx, const void *w_gate,
@@ -1125,7 +1290,7 @@ vs_status vs_gated_linear(int dtype, int act, const void *x, int64_t ldx, const 
 
 size_t vs_gated_linear_backward_workspace(int64_t m, int64_t f, int64_t k, int want_dx, int want_dw) {
   if (glin::check("", VS_BF16, 0, m, f, k) != VS_OK) return 0;
-  return glin::backward_need(m, f, k, want_dx != 0, want_dw != 0);
+  return k ? glin::backward_need(m, f, k, want_dx != 0, want_dw != 0).bytes : 0;
 }
 
 vs_status vs_gated_linear_backward(int dtype, int act, const void *x, int64_t ldx,

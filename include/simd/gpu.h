@@ -387,14 +387,15 @@ vs_status vs_matvec_int4(int dtype, const void *x, int64_t ldx, const uint8_t *q
 /// x [m][k], w_gate and w_up [f][k] with row strides ldx, ld_gate, ld_up in
 /// elements; h [m][f] contiguous.  pre: NULL, or fp32 [m][f][2], the pairs
 /// (x w_gate^T, x w_up^T) that the backward pass reads.  workspace: device
-/// memory of vs_gated_linear_workspace(m, f, k) bytes, or NULL for the library's
-/// pool; it is used where rows are not 16-byte aligned.
+/// memory of vs_gated_linear_workspace(m, f, k, aligned) bytes, or NULL for the
+/// library's pool; it is used where k is summed in parts (few outputs, long k)
+/// and where rows of an operand are not whole 16-byte pieces (aligned = 0).
 typedef enum { VS_ACT_SILU = 0, VS_ACT_GELU = 1, VS_ACT_RELU = 2, VS_ACT_SIGMOID = 3 } vs_activation;
 vs_status vs_gated_linear(int dtype, int act, const void *x, int64_t ldx, const void *w_gate,
                           int64_t ld_gate, const void *w_up, int64_t ld_up, int64_t m, int64_t f,
                           int64_t k, void *h, float *pre, void *workspace, size_t workspace_bytes,
                           vs_stream_t stream);
-size_t vs_gated_linear_workspace(int64_t m, int64_t f, int64_t k);
+size_t vs_gated_linear_workspace(int64_t m, int64_t f, int64_t k, int aligned);
 /// Gradients of vs_gated_linear from dh [m][f] (row stride ld_dh) and pre:
 /// dx [m][k] and dw [2 f][k] (w_gate's rows, then w_up's); NULL skips one.
 /// dw takes fewer than 2^22 - 8 rows.

@@ -110,6 +110,25 @@ def test_large_tiles(shape, dtype):
     _all(*_inputs(*shape, dtype, "cuda", seed=3), "silu")
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(300, 8192, 200), (70, 5003, 33), (130, 1500, 1), (66, 130, 9001), (9000, 40, 72),
+                                   (9001, 513, 65), (64, 128, 16384)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_sums_in_parts(shape, dtype):
+    """Few outputs and a long reduction, forward, in dx or in dw: summed in parts, which changes no result between calls."""
+    args = _inputs(*shape, dtype, "cuda", seed=8)
+    first = _all(*args, "gelu")
+    for a, b in zip(first, _all(*args, "gelu")):
+        assert torch.equal(a, b)
+
+
+def test_workspace_sizes():
+    size = _lib.lib().vs_gated_linear_workspace
+    assert size(4096, 2048, 2048, 1) == 0 and size(8, 64, 64, 0) == 0
+    assert size(4096, 2048, 2048, 0) >= 2 * 2048 * (4096 + 2 * 2048)
+    assert 0 < size(300, 200, 8192, 1) < size(300, 200, 8192, 0)
+
+
 @pytest.mark.parametrize("dev", DEVICES)
 @pytest.mark.parametrize("m", [6, 90])
 def test_shapes_strides_and_alignment(dev, m):
@@ -262,7 +281,7 @@ def test_native_refusals():
         assert call(**kw) == 1 and b"gated_linear" in lib.vs_last_error()
     assert call(m=100, f=100, k=65, ldx=65, ldw=65, ws=p, size=16) == 1 and b"workspace" in lib.vs_last_error()
     assert lib.vs_gated_linear_backward(5, 0, p, 8, p, 8, p, 8, None, p, 8, 1, 1, 8, p, p, None, 0, None) == 1
-    assert lib.vs_gated_linear_workspace(-1, 1, 1) == 0
+    assert lib.vs_gated_linear_workspace(-1, 1, 1, 0) == 0
     assert lib.vs_gated_linear_backward(5, 0, p, 8, p, 8, p, 8, p, p, 1, 1 << 22, 1, 8, None, p, p, 16, None) == 1
     assert b"too many rows" in lib.vs_last_error()
 

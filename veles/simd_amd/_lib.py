@@ -112,7 +112,7 @@ _SIGNATURES = {
     "vs_gated_recurrence_step": (_i, [_i, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _vp, _vp]),
     "vs_matvec_int4": (_i, [_i, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _vp]),
     "vs_gated_linear": (_i, [_i, _i, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _sz, _vp]),
-    "vs_gated_linear_workspace": (_sz, [_i64, _i64, _i64]),
+    "vs_gated_linear_workspace": (_sz, [_i64, _i64, _i64, _i]),
     "vs_gated_linear_backward": (_i, [_i, _i, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _i64,
                                       _vp, _vp, _vp, _sz, _vp]),
     "vs_gated_linear_backward_workspace": (_sz, [_i64, _i64, _i64, _i, _i]),

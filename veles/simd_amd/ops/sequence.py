@@ -482,8 +482,8 @@ def _gated_impl(x, w_gate, w_up, activation, save):
     h = _new(x, *x.shape[:-1], f)
     pre = torch.empty((m, f, 2), dtype=torch.float32, device=x.device) if save else None
     size, ws = 0, None
-    if not _aligned(rows, w_gate, w_up):
-        size = int(_lib.lib().vs_gated_linear_workspace(m, f, k))
+    if m > 16:      # fewer rows need none
+        size = int(_lib.lib().vs_gated_linear_workspace(m, f, k, _aligned(rows, w_gate, w_up)))
         ws = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
     launch(x, "vs_gated_linear", DTYPES[x.dtype], ACTIVATIONS[activation], rows.data_ptr(), rows.stride(0),
            w_gate.data_ptr(), w_gate.stride(0), w_up.data_ptr(), w_up.stride(0), m, f, k, h.data_ptr(),
