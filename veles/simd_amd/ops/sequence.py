@@ -29,7 +29,7 @@ def _same_device(name, first, **others):
 
 
 def _new(x: torch.Tensor, *shape) -> torch.Tensor:
-    return torch.empty(shape, dtype=x.dtype, device=x.device)
+    return x.new_empty(shape)
 
 
 # ------------------------------------------------------- gated recurrence
@@ -277,10 +277,14 @@ def _step_impl(x, gate, state):
     if not x.is_cuda:
         state += torch.sigmoid(-gate.double()) * (x.double() - state)
         return state.to(x.dtype, copy=True)
-    x, gate = _rows_last(x), _rows_last(gate)
-    y = _new(x, *x.shape)
-    launch(x, "vs_gated_recurrence_step", DTYPES[x.dtype], x.data_ptr(), x.stride(0), gate.data_ptr(),
-           gate.stride(0), state.data_ptr(), x.shape[0], x.shape[1], y.data_ptr())
+    b, d = x.shape
+    if x.is_contiguous() and gate.is_contiguous():
+        y, ldx, ldg = torch.empty_like(x), d, d
+    else:
+        x, gate = _rows_last(x), _rows_last(gate)
+        y, ldx, ldg = _new(x, b, d), x.stride(0), gate.stride(0)
+    launch(x, "vs_gated_recurrence_step", DTYPES[x.dtype], x.data_ptr(), ldx, gate.data_ptr(), ldg,
+           state.data_ptr(), b, d, y.data_ptr())
     return y
 
 
@@ -310,6 +314,9 @@ def _check_group(name, group_size):
         raise ValueError(f"{name}: group size {group_size}; 32, 64 or a multiple of 128 expected")
 
 
+_HALF = (torch.float16, torch.bfloat16)
+
+
 def _check_matvec(name, x, qweight, scales, zeros, group_size):
     if x.dtype not in (torch.bfloat16, torch.float16):
         raise TypeError(f"{name}: x is {x.dtype}; float16 or bfloat16 expected")
@@ -333,6 +340,20 @@ def _check_matvec(name, x, qweight, scales, zeros, group_size):
 
 def _matvec_impl(x, qweight, scales, zeros, group_size):
     name = "veles::matvec_int4"
+    # the usual case in one expression; _check_matvec names what is wrong otherwise
+    dev, dtype = x.get_device(), x.dtype
+    if (dev >= 0 and x.dim() == 2 and qweight.dim() == 2 and dtype in _HALF and scales.dtype is dtype
+            and qweight.dtype is torch.uint8 and (group_size in (32, 64) or (group_size > 0 and group_size % 128 == 0))
+            and x.is_contiguous() and qweight.is_contiguous() and scales.is_contiguous()
+            and dev == qweight.get_device() == scales.get_device()
+            and (zeros is None or (zeros.dtype is torch.uint8 and zeros.is_contiguous()
+                                   and zeros.shape == scales.shape and dev == zeros.get_device()))):
+        (m, k), (n, half) = x.shape, qweight.shape
+        if half == (k + 1) // 2 and scales.shape == (n, -(-k // group_size)):
+            y = x.new_empty((m, n))
+            launch(x, "vs_matvec_int4", DTYPES[dtype], x.data_ptr(), k, qweight.data_ptr(), half, scales.data_ptr(),
+                   _opt(zeros), group_size, m, n, k, y.data_ptr())
+            return y
     _check_matvec(name, x, qweight, scales, zeros, group_size)
     n, k = qweight.shape[0], x.shape[-1]
     if not x.is_cuda:
@@ -340,7 +361,7 @@ def _matvec_impl(x, qweight, scales, zeros, group_size):
         at = torch.arange(k) // group_size
         z = 8.0 if zeros is None else zeros.double()[:, at]
         return (x.double() @ ((q - z) * scales.double()[:, at]).t()).to(x.dtype)
-    rows = x if x.dim() == 2 and x.is_contiguous() else _near_rows(_as_rows(x), True)
+    rows = _near_rows(_as_rows(x), True)
     y = _new(x, *x.shape[:-1], n)
     scales = scales.contiguous()
     zeros = None if zeros is None else zeros.contiguous()
@@ -470,6 +491,18 @@ def _slope_cpu(kind, g):
 
 def _gated_impl(x, w_gate, w_up, activation, save):
     name = "veles::gated_linear"
+    # few rows, as a generating model has them, in one expression; _check_gated names what is wrong otherwise
+    dev, dtype = x.get_device(), x.dtype
+    if (dev >= 0 and not save and x.dim() == 2 and w_gate.dim() == 2 and dtype in _HALF
+            and w_gate.dtype is dtype and w_up.dtype is dtype and activation in ACTIVATIONS
+            and x.is_contiguous() and w_gate.is_contiguous() and w_up.is_contiguous()
+            and dev == w_gate.get_device() == w_up.get_device()):
+        (m, k), (f, kw) = x.shape, w_gate.shape
+        if m <= 16 and k == kw < _LD_MAX and w_up.shape == w_gate.shape:
+            h = x.new_empty((m, f))
+            launch(x, "vs_gated_linear", DTYPES[dtype], ACTIVATIONS[activation], x.data_ptr(), k, w_gate.data_ptr(), k,
+                   w_up.data_ptr(), k, m, f, k, h.data_ptr(), None, None, 0)
+            return h, None
     _check_gated(name, x, w_gate, w_up, activation)
     f, k = w_gate.shape
     rows = _near_rows(_as_rows(x), True)
