@@ -86,7 +86,7 @@ struct Shape {
 
   // The L steps of this wave from `t` on, at lane offset c: row addresses are the same for the
   // whole wave, so they live in scalar registers.  Steps in the padding load the last step that
-  // is none (memory of the tensor; the value is replaced by blank() below).
+  // is none (memory of the tensor; what comes of it is not used).
   __device__ __forceinline__ static void load(P (&r)[L], const void *base, int64_t off,
                                               int64_t stride, int c, int64_t t, int64_t len) {
     const E *row = static_cast<const E *>(base) + off;
@@ -103,16 +103,6 @@ struct Shape {
   __device__ __forceinline__ static void store(void *base, int64_t row, int d, int c, const P &v) {
     *reinterpret_cast<P *>(static_cast<E *>(base) + row * d + c) = v;
   }
-  // Padding steps become `v`: a gate of +inf lets nothing in (share() is exactly 0), so they
-  // keep the state and pass gradients through whatever the tensor holds there.
-  __device__ __forceinline__ static void blank(P (&r)[L], int64_t t, int64_t len, float f) {
-    P z;
-#pragma unroll
-    for (int v = 0; v < V; v++) z.set(v, f);
-#pragma unroll
-    for (int s = 0; s < L; s++)
-      if (t + s >= len) r[s] = z;
-  }
   __device__ __forceinline__ static P zero() {
     P z;
 #pragma unroll
@@ -120,13 +110,10 @@ struct Shape {
     return z;
   }
 
-  // Shares of the wave's steps and their map: product a, end e from a zero state.
-  __device__ __forceinline__ static void forward_map(P (&x)[L], P (&g)[L], int64_t t, int64_t len,
+  // Shares of the wave's steps and their map: product a, end e from a zero state.  `on` steps are
+  // none of padding; the others are left out (a share of 0 would turn an infinite state into NaN).
+  __device__ __forceinline__ static void forward_map(const P (&x)[L], const P (&g)[L], int on,
                                                      float (&i)[L][V], float (&a)[V], float (&e)[V]) {
-    if (t + L > len) {
-      blank(x, t, len, 0.f);
-      blank(g, t, len, __builtin_inff());
-    }
 #pragma unroll
     for (int v = 0; v < V; v++) {
       a[v] = 1.f;
@@ -135,47 +122,58 @@ struct Shape {
 #pragma unroll
     for (int s = 0; s < L; s++)
 #pragma unroll
+      for (int v = 0; v < V; v++) i[s][v] = share(g[s][v]);
+    steps(on, [&](int s, bool use) {
+#pragma unroll
       for (int v = 0; v < V; v++) {
-        i[s][v] = share(g[s][v]);
-        e[v] = fmaf(i[s][v], x[s][v] - e[v], e[v]);
-        a[v] = fmaf(-i[s][v], a[v], a[v]);
+        const float en = fmaf(i[s][v], x[s][v] - e[v], e[v]), an = fmaf(-i[s][v], a[v], a[v]);
+        e[v] = use ? en : e[v];
+        a[v] = use ? an : a[v];
       }
+    });
+  }
+  // f(s, whether step s is none of padding) for s = 0 .. L - 1, or down from L - 1.
+  template <bool DOWN = false, class F>
+  __device__ __forceinline__ static void steps(int on, const F &f) {
+    if (on >= L) {
+#pragma unroll
+      for (int s = 0; s < L; s++) f(DOWN ? L - 1 - s : s, true);
+    } else {
+#pragma unroll
+      for (int s = 0; s < L; s++) f(DOWN ? L - 1 - s : s, (DOWN ? L - 1 - s : s) < on);
+    }
   }
   // Runs the steps from state h and stores y.
-  __device__ __forceinline__ static void forward_steps(const Args &p, int64_t b, int c, bool in, bool full,
-                                                       int64_t t, int64_t len, const P (&x)[L],
-                                                       const float (&i)[L][V], float (&h)[V]) {
-#pragma unroll
-    for (int s = 0; s < L; s++) {
+  __device__ __forceinline__ static void forward_steps(const Args &p, int64_t b, int c, bool in, int64_t t,
+                                                       int on, const P (&x)[L], const float (&i)[L][V],
+                                                       float (&h)[V]) {
+    steps(on, [&](int s, bool use) {
       P y;
 #pragma unroll
       for (int v = 0; v < V; v++) {
         h[v] = fmaf(i[s][v], x[s][v] - h[v], h[v]);
         y.set(v, h[v]);
       }
-      if (full ? in : in && t + s < p.t)
-        store(p.y, b * p.t + t + s, p.d, c, full || t + s < len ? y : zero());
-    }
+      if (in && (use || t + s < p.t)) store(p.y, b * p.t + t + s, p.d, c, use ? y : zero());
+    });
   }
   // End q of the wave's steps backward from a zero m (the product is the forward one).
-  __device__ __forceinline__ static void backward_map(const Args &p, P (&dy)[L], int64_t t, int64_t len,
-                                                      const float (&i)[L][V], float (&q)[V]) {
-    if (!p.dy) blank(dy, 0, 0, 0.f);
-    else if (t + L > len) blank(dy, t, len, 0.f);
+  __device__ __forceinline__ static void backward_map(const P (&dy)[L], int on, const float (&i)[L][V],
+                                                      float (&q)[V]) {
 #pragma unroll
     for (int v = 0; v < V; v++) q[v] = 0.f;
-#pragma unroll
-    for (int s = L - 1; s >= 0; s--)
+    steps<true>(on, [&](int s, bool use) {
 #pragma unroll
       for (int v = 0; v < V; v++) {
-        const float l = q[v] + dy[s][v];
-        q[v] = fmaf(-i[s][v], l, l);
+        const float l = q[v] + dy[s][v], qn = fmaf(-i[s][v], l, l);
+        q[v] = use ? qn : q[v];
       }
+    });
   }
   // Runs the steps forward from state h, then backward from m, and stores dx and dg.
   __device__ __forceinline__ static void backward_steps(const Args &p, int64_t b, int c, bool in,
-                                                        bool full, int64_t t, int64_t len,
-                                                        const P (&x)[L], const P (&dy)[L],
+                                                        int64_t t, int on, const P (&x)[L],
+                                                        const P (&dy)[L],
                                                         const float (&i)[L][V], float (&h)[V],
                                                         float (&m)[V]) {
     float before[L][V];  // h_{t-1} - x_t
@@ -186,23 +184,21 @@ struct Shape {
         before[s][v] = h[v] - x[s][v];
         h[v] = fmaf(-i[s][v], before[s][v], h[v]);
       }
-#pragma unroll
-    for (int s = L - 1; s >= 0; s--) {
+    steps<true>(on, [&](int s, bool use) {
       P ox, og;
 #pragma unroll
       for (int v = 0; v < V; v++) {
         const float l = m[v] + dy[s][v];
         const float il = i[s][v] * l;
-        m[v] = l - il;
+        m[v] = use ? l - il : m[v];
         ox.set(v, il);
         og.set(v, (1.f - i[s][v]) * il * before[s][v]);
       }
-      if (full ? in : in && t + s < p.t) {
-        const bool on = full || t + s < len;
-        store(p.dx, b * p.t + t + s, p.d, c, on ? ox : zero());
-        store(p.dg, b * p.t + t + s, p.d, c, on ? og : zero());
+      if (in && (use || t + s < p.t)) {
+        store(p.dx, b * p.t + t + s, p.d, c, use ? ox : zero());
+        store(p.dg, b * p.t + t + s, p.d, c, use ? og : zero());
       }
-    }
+    });
   }
   __device__ __forceinline__ static void zero_gradients(const Args &p, int64_t b, int c, bool in,
                                                         int64_t t) {
@@ -353,7 +349,8 @@ __global__ __launch_bounds__(64 * W) void forward_kernel(Args p) {
   const bool in = c0 < p.d;
   const int c = in ? c0 : 0;
   const int64_t len = steps_of(p, b), t0 = pos * S::kTile + wave * L;
-  const bool live = pos * S::kTile < len, full = t0 + L <= len;
+  const bool live = pos * S::kTile < len;
+  const int on = static_cast<int>(len - t0 < 0 ? 0 : len - t0 < L ? len - t0 : L);  // steps that are no padding
   P x[L], g[L];
   float i[L][V], ta[V], te[V], s[V];
 #pragma unroll
@@ -365,7 +362,7 @@ __global__ __launch_bounds__(64 * W) void forward_kernel(Args p) {
     float a[V], e[V];
     S::load(x, p.x, b * p.xb, p.xt, c, t0, len);
     S::load(g, p.g, b * p.gb, p.gt, c, t0, len);
-    S::forward_map(x, g, t0, len, i, a, e);
+    S::forward_map(x, g, on, i, a, e);
 #pragma unroll
     for (int v = 0; v < V; v++) {
       maps[0][wave][lane * V + v] = a[v];
@@ -401,7 +398,7 @@ __global__ __launch_bounds__(64 * W) void forward_kernel(Args p) {
   for (int w = 0; w < wave; w++)
 #pragma unroll
     for (int v = 0; v < V; v++) s[v] = fmaf(maps[0][w][lane * V + v], s[v], maps[1][w][lane * V + v]);
-  S::forward_steps(p, b, c, in, full, t0, len, x, i, s);
+  S::forward_steps(p, b, c, in, t0, on, x, i, s);
 }
 
 template <class N, int V, int W, int L>
@@ -417,7 +414,8 @@ __global__ __launch_bounds__(64 * W) void backward_kernel(Args p) {
   const bool in = c0 < p.d;
   const int c = in ? c0 : 0;
   const int64_t len = steps_of(p, b), t0 = tile * S::kTile + wave * L;
-  const bool live = tile * S::kTile < len, full = t0 + L <= len;
+  const bool live = tile * S::kTile < len;
+  const int on = static_cast<int>(len - t0 < 0 ? 0 : len - t0 < L ? len - t0 : L);
   P x[L], g[L], dy[L];
   float i[L][V], h[V], ta[V], te[V], m[V];
 #pragma unroll
@@ -431,9 +429,14 @@ __global__ __launch_bounds__(64 * W) void backward_kernel(Args p) {
     for (int v = 0; v < V; v++) h[v] = p.starts[(b * p.tiles + tile) * p.d + c + v];
     S::load(x, p.x, b * p.xb, p.xt, c, t0, len);
     S::load(g, p.g, b * p.gb, p.gt, c, t0, len);
-    if (p.dy) S::load(dy, p.dy, b * p.yb, p.yt, c, t0, len);
-    S::forward_map(x, g, t0, len, i, a, e);
-    S::backward_map(p, dy, t0, len, i, q);
+    if (p.dy) {
+      S::load(dy, p.dy, b * p.yb, p.yt, c, t0, len);
+    } else {
+#pragma unroll
+      for (int k = 0; k < L; k++) dy[k] = S::zero();
+    }
+    S::forward_map(x, g, on, i, a, e);
+    S::backward_map(dy, on, i, q);
 #pragma unroll
     for (int v = 0; v < V; v++) {
       maps[0][wave][lane * V + v] = a[v];
@@ -466,7 +469,7 @@ __global__ __launch_bounds__(64 * W) void backward_kernel(Args p) {
   for (int w = W - 1; w > wave; w--)
 #pragma unroll
     for (int v = 0; v < V; v++) m[v] = fmaf(maps[0][w][lane * V + v], m[v], maps[2][w][lane * V + v]);
-  S::backward_steps(p, b, c, in, full, t0, len, x, dy, i, h, m);
+  S::backward_steps(p, b, c, in, t0, on, x, dy, i, h, m);
 }
 
 // ------------------------------------------------------------ single step

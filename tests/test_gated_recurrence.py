@@ -296,6 +296,24 @@ def test_step_continues_a_prefill(dev, dtype, b, d):
 
 
 @pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("t", [9, 30, 300])
+def test_infinite_states_pass_through_padding(dev, t):
+    """An infinite initial state of an empty sequence, and a value that is infinite at the last step before the padding."""
+    n = torch.tensor([0, 5, t - 1, 1], device=dev)
+    x, gate, h0, _ = _inputs(4, t, 6, torch.float32, dev, seed=9)
+    h0, x = h0.clone(), x.clone()
+    h0[0, 2] = float("inf")
+    for b in (1, 2, 3):
+        x[b, int(n[b]) - 1, 2] = -float("inf")
+    y, final = ops.gated_recurrence(x, gate, h0, n)
+    assert final[0, 2] == float("inf") and (final[1:, 2] == -float("inf")).all()
+    other = [0, 1, 3, 4, 5]
+    assert torch.isfinite(final[:, other]).all() and torch.isfinite(y[:, :, other]).all()
+    for b in range(4):
+        assert (y[b, int(n[b]):] == 0).all()
+
+
+@pytest.mark.parametrize("dev", DEVICES)
 def test_step_counts_as_a_write(dev):
     """A backward pass that needs the state as it was before the step refuses, as for any tensor written in place."""
     x, gate, h0, _ = _inputs(2, 3, 4, torch.float32, dev)

@@ -247,8 +247,8 @@ def gated_recurrence(x: torch.Tensor, gate: torch.Tensor, state: torch.Tensor | 
     lengths: int32 / int64 [batch] on x's device: steps from lengths[b] on are padding (not read,
     y = 0, the state passes through; values outside 0..time are clamped).
     The state is held in float32.  Differentiable in x, gate and state; in the padding the
-    gradients are 0 and dy is not read.  Where the update meets an infinite state or value inside
-    a sequence it follows the formula above (inf - inf is NaN)."""
+    gradients are 0 and dy is not read.  From an infinite state or value on, a channel is infinite or
+    NaN to its end (the formula above has inf - inf)."""
     save = records(x, gate, state)
     if plain_tensors(x, gate, state, lengths):
         if save:
