@@ -122,6 +122,18 @@ def test_sums_in_parts(shape, dtype):
         assert torch.equal(a, b)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,k,f", [(5, 2104, 1 << 20), (70, 2104, 1 << 20), ((1 << 20) + 300, 2104, 40)])
+def test_operands_past_32_bit_offsets(m, k, f):
+    """The last rows and features where x, the weights or the pairs have more than 2^31 elements."""
+    gen = torch.Generator("cuda").manual_seed(4)
+    x = torch.randn(m, k, device="cuda", dtype=torch.bfloat16, generator=gen)
+    wg, wu = (torch.randn(f, k, device="cuda", dtype=torch.bfloat16, generator=gen).mul_(k ** -0.5) for _ in range(2))
+    h = ops.gated_linear(x, wg, wu)
+    x, wg, wu, h = x[-64:], wg[-64:], wu[-64:], h[-64:, -64:]
+    _close("h", h, _oracle(x, wg, wu, torch.zeros_like(h), "silu")["h"])
+
+
 def test_workspace_sizes():
     size = _lib.lib().vs_gated_linear_workspace
     assert size(4096, 2048, 2048, 1) == 0 and size(8, 64, 64, 0) == 0

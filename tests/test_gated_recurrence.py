@@ -295,6 +295,39 @@ def test_step_continues_a_prefill(dev, dtype, b, d):
         _close("state", state, (want_y[idx], ey[idx]))
 
 
+@pytest.mark.gpu
+def test_arrays_past_32_bit_offsets():
+    """2.2e9 values in one sequence: its last steps, and the gradients there, are those of a sequence of its own that begins
+    2000 steps earlier (what came before has decayed: the shares are 1/2)."""
+    t, d, k = (1 << 21) + 130, 1040, 2000
+    x = torch.randn(1, t, d, device="cuda", dtype=torch.bfloat16, generator=torch.Generator("cuda").manual_seed(5))
+    gate = torch.zeros(1, t, d, device="cuda", dtype=torch.bfloat16)
+    leaves = [v.requires_grad_() for v in (x, gate)]
+    y, final = ops.gated_recurrence(*leaves)
+    got = [y.detach()[:, -200:].clone(), final.detach()] + [g[:, -200:].clone() for g in torch.autograd.grad(final.sum(), leaves)]
+    del y
+    own = [v.detach()[:, -k:].clone().requires_grad_() for v in (x, gate)]
+    y, final = ops.gated_recurrence(*own)
+    want = [y.detach()[:, -200:], final.detach()] + [g[:, -200:] for g in torch.autograd.grad(final.sum(), own)]
+    # the same steps in other tiles: a step's 3 roundings of at most u max|h| halve with every step, so 6 u max|h| on each
+    # side with max|h| < 5; then a step of the result's type where the rounding falls on different sides
+    for a, b in zip(got, want):
+        eps = torch.finfo(a.dtype).eps
+        assert ((a.double() - b.double()).abs() <= eps * b.double().abs() + 64 * U).all()
+
+
+@pytest.mark.gpu
+def test_more_groups_than_one_launch():
+    """2^21 + 5 sequences of two tiles take two launches; the sequences around the cut have the bits of a small call."""
+    b, t = (1 << 21) + 5, 130
+    gen = torch.Generator("cuda").manual_seed(6)
+    x, gate = (torch.randn(b, t, 1, device="cuda", dtype=torch.bfloat16, generator=gen) for _ in range(2))
+    y, final = ops.gated_recurrence(x, gate)
+    for at in (0, (1 << 21) - 3, b - 6):
+        ys, fs = ops.gated_recurrence(x[at:at + 6], gate[at:at + 6])
+        assert torch.equal(y[at:at + 6], ys) and torch.equal(final[at:at + 6], fs)
+
+
 @pytest.mark.parametrize("dev", DEVICES)
 @pytest.mark.parametrize("t", [9, 30, 300])
 def test_infinite_states_pass_through_padding(dev, t):

@@ -129,6 +129,18 @@ def test_quantize(dev, symmetric, k):
 
 
 @pytest.mark.gpu
+def test_weight_past_32_bit_offsets():
+    """The last rows of 4.3 GB of weights."""
+    n, k = (1 << 20) + 40, 8192
+    gen = torch.Generator("cuda").manual_seed(3)
+    x = torch.randn(2, k, device="cuda", generator=gen).bfloat16()
+    q = torch.randint(0, 256, (n, k // 2), device="cuda", dtype=torch.uint8, generator=gen)
+    s = (torch.rand(n, k // 128, device="cuda", generator=gen) * 0.02).bfloat16()
+    y = ops.matvec_int4(x, q, s)
+    _check(y[:, -100:], x, q[-100:], s[-100:], None, 128)
+
+
+@pytest.mark.gpu
 def test_more_rows_than_one_grid():
     """16 x 65535 rows fill a grid dimension; the rows behind them get the bits of a small call."""
     m = 16 * 65535 + 3
