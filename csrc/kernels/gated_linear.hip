@@ -8,18 +8,22 @@
 // are rows of Wg and Wu for the same outputs, so a wave ends with g and u of the same outputs in
 // its accumulators and h is formed in registers.  Operand tiles go global -> LDS by DMA into two
 // stages, eight waves take a k tile in four phases with one half of them a barrier behind the other
-// (see tile_kernel).  Rows past the end and the ragged end of k read zeros through the buffer
-// descriptor's range check.  The backward products are the same kernel with one B operand: one
-// launch forms the gradients of g and u, side by side, as they are and transposed, and transposes x
-// and the weights, so both products have their operands contiguous in the reduction dimension; a
-// second launch computes both.  bf16, x [m][k], f outputs: 8192 x 4096 x 12288 takes 1120-1180 us
-// (1400-1470 TFLOP/s; a plain library product of this size 1081 us); forward and backward of
-// 4096 x 2048 x 6144 590-610 us, of which the three products' work is 426 us at that rate.
+// (see take_tiles).  Rows past the end and the ragged end of k read zeros through the buffer
+// descriptor's range check.  bf16, x [m][k], f outputs: 8192 x 4096 x 12288 takes 1090-1180 us
+// (1400-1510 TFLOP/s; a plain library product of this size 1081 us).
+//
+// Backward: one launch forms dg and du side by side, another computes the three products with the same
+// loop.  Where an operand has the reduction as its rows (the weights in dx, everything in dWg
+// and dWu), its tile goes to LDS as it lies in memory and the fragments are read across (see
+// take_tiles), so nothing is transposed in memory.  Forward and backward of 4096 x 2048 x 6144 take
+// 530-570 us, of which the products' work is 412 us at 1500 TFLOP/s (with transposed copies of
+// dg, du, x and the weights it was 580-600, and the backward pass of 1000 x 4096 x 4096 181 instead of
+// 146).
 //
 // Few rows (up to 16, and up to 64 where it is faster): bound by reading the weights.  The waves of
 // a workgroup cut k; each loads whole 128-byte stretches of the rows of Wg, Wu and x, forms
 // fragments through a small LDS image of its own, and the waves' sums meet in LDS in a fixed order.
-// bf16: 1 x 2048 x 6144 10.9 us (4.6 TB/s of weights), 33 x 4096 x 10240 41 us (4.1 TB/s).
+// bf16: 1 x 2048 x 6144 10 us (5 TB/s of weights), 33 x 4096 x 10240 41 us (4.1 TB/s).
 //
 // Roundings: h once; for training, g and u are kept in fp32 (a 16-bit copy would add its own
 // rounding to every gradient, 1.7 instead of 1.4 times the error of the result's own rounding);
@@ -90,10 +94,13 @@ __device__ __forceinline__ float act_slope(int kind, float g) {
 
 // ------------------------------------------------------------------- tiles
 struct Args {
-  const uint16_t *a;      // [m][k], row stride lda
-  const uint16_t *b[2];   // [n][k], row stride ldb[.]; b[1] only for the gated product
+  // Forward: a [m][k], b[0] and b[1] [n][k].  Backward: a [m][k] or, with `across`, [k][m]; b [k][n],
+  // of which the first `fold` rows are b[0] and those behind b[1], `have` rows of each (zeros behind).
+  const uint16_t *a;
+  const uint16_t *b[2];
   int64_t lda, ldb[2];
   int m, n, k;            // n: outputs (columns of h, or of c)
+  int across, fold, have;
   uint16_t *c;            // [m][n], row stride n
   float2 *pre;            // [m][n] (g, u), or null
   int act;
@@ -103,10 +110,11 @@ struct Args {
   float *sums;
 };
 
-// One or two products in a launch: tiles [0, first) belong to q[0], the rest to q[1].
+// Up to three products in a launch: tiles up to end[0] belong to q[0], up to end[1] to q[1], ...
+constexpr int kProducts = 3;
 struct Work {
-  Args q[2];
-  unsigned first, tiles;
+  Args q[kProducts];
+  unsigned end[kProducts];
 };
 
 // A tile of 2 (rows) x 4 (columns) waves, each with 2 x 2 quadrants of 16 XH x 16 YH products.
@@ -150,12 +158,45 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_of(const uint16_t *p, int
       0x00020000);
 }
 
+// Rows [row0, row0 + rows) of a [.][n] operand from column c0 on, 64 of them at most.  (Rows hold
+// whole 16-byte pieces.)
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t columns_of(const uint16_t *p, int64_t ld, int row0,
+                                                             int rows, int c0, int n) {
+  const int have = rows < 64 ? rows : 64;
+  const uint32_t bytes = (static_cast<uint32_t>(have - 1) * static_cast<uint32_t>(ld) + (n + 7) / 8 * 8 - c0) * 2;
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t *>(p + row0 * ld + c0), 0,
+                                           have > 0 ? bytes : 0u, 0x00020000);  // (0: nothing is read)
+}
+
+// Where the 32 bytes of 16 columns lie in an image row of ROW bytes that is read across: piece p of
+// row r at p ^ turn(r), so the 8 rows of two 16-lane groups are in different banks.
+template <int ROW>
+__device__ __forceinline__ int turn(int r) {
+  return ROW == 256 ? (r & 3) | (r >> 1 & 4) : (r >> 1 & 1) | (r >> 2 & 2);
+}
+
+// A fragment, in one piece or as two reads bring it.
+struct Halves {
+  u32x2 lo, hi;
+};
+template <bool T>
+using Frag = std::conditional_t<T, Halves, u32x4>;
+__device__ __forceinline__ const u32x4 &whole(const u32x4 &f) { return f; }
+__device__ __forceinline__ u32x4 whole(const Halves &f) {
+  return __builtin_shufflevector(f.lo, f.hi, 0, 1, 2, 3);
+}
+
 // Fragment reads are inline asm: the compiler would wait for every DMA in flight before a read of
 // LDS that it sees.  `settle` is the wait, and the registers pass through it, so no product can
 // move above it.
 template <int OFF>
 __device__ __forceinline__ void read_frag(u32x4 &f, uint32_t at) {
   asm volatile("ds_read_b128 %0, %1 offset:%2" : "=v"(f) : "v"(at), "i"(OFF) : "memory");
+}
+template <int OFF, int ROW>
+__device__ __forceinline__ void read_across(Halves &f, uint32_t at) {
+  asm volatile("ds_read_b64_tr_b16 %0, %1 offset:%2" : "=v"(f.lo) : "v"(at), "i"(OFF) : "memory");
+  asm volatile("ds_read_b64_tr_b16 %0, %1 offset:%2" : "=v"(f.hi) : "v"(at), "i"(OFF + 4 * ROW) : "memory");
 }
 template <int XH>
 __device__ __forceinline__ void settle(u32x4 (&f)[XH][2]) {
@@ -168,6 +209,17 @@ __device__ __forceinline__ void settle(u32x4 (&f)[XH][2]) {
                  : "+v"(f[0][0]), "+v"(f[1][0]), "+v"(f[0][1]), "+v"(f[1][1])::"memory");
   else
     asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(f[0][0]), "+v"(f[0][1])::"memory");
+}
+template <int XH>
+__device__ __forceinline__ void settle(Halves (&f)[XH][2]) {
+  asm volatile("s_waitcnt lgkmcnt(0)"
+               : "+v"(f[0][0].lo), "+v"(f[0][0].hi), "+v"(f[0][1].lo), "+v"(f[0][1].hi)::"memory");
+  if constexpr (XH > 1)  // (no instruction: nothing may move above the wait)
+    asm volatile("" : "+v"(f[1][0].lo), "+v"(f[1][0].hi), "+v"(f[1][1].lo), "+v"(f[1][1].hi)::"memory");
+  if constexpr (XH > 2) {
+    asm volatile("" : "+v"(f[2][0].lo), "+v"(f[2][0].hi), "+v"(f[2][1].lo), "+v"(f[2][1].hi)::"memory");
+    asm volatile("" : "+v"(f[3][0].lo), "+v"(f[3][0].hi), "+v"(f[3][1].lo), "+v"(f[3][1].hi)::"memory");
+  }
 }
 template <int N>
 __device__ __forceinline__ void wait_vmcnt() {
@@ -200,18 +252,23 @@ __device__ __forceinline__ void meet() {
 //
 // A workgroup takes tiles blockIdx.x, + gridDim.x, ...; the next tile's first eight halves are
 // started before the results of the last one are stored.
-template <class N, class C>
-__global__ __launch_bounds__(512) void tile_kernel(Work work) {
-  extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+// TA, TB: the operand has k as its rows.  Its image halves are 64 k of neighbouring columns then, and
+// fragments are read across: ds_read_b64_tr_b16 gives lane i of 16 the i-th of 16 columns of four
+// rows, whose 8-byte pieces lanes 4 r .. 4 r + 3 point at.  Columns past the end read what lies there
+// (inside the operand) and are not stored.
+template <class N, class C, bool TA, bool TB>
+__device__ __forceinline__ void take_tiles(const Args &p, unsigned begin, unsigned end, uint8_t *lds) {
   constexpr int XH = C::XH, YH = C::YH;
-  const Args &p = work.q[blockIdx.x < work.first ? 0 : 1];
-  const unsigned begin = blockIdx.x < work.first ? 0 : work.first;
+  constexpr int RA = TA ? 64 * XH : C::RB, RT = TB ? 128 * YH : C::RB;  // bytes of an image row
   const unsigned tiles_m = (p.m + C::BM - 1) / C::BM, tiles_n = (p.n + C::BO - 1) / C::BO;
+  const uint16_t *pa = p.a, *pb0 = p.b[0], *pb1 = p.b[1];
+  const int64_t lda = p.lda, ldb = p.ldb[0];
+  const int pm = p.m, pn = p.n, fold = p.fold, have = p.have;
   const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wid / 4, wn = wid % 4;
   const int l16 = lane & 15, lq = lane >> 4;
 
-  int m0, n0, part, k;  // of the tile: first row and column, part and length of k
+  int m0, n0, part, k, ks0;  // of the tile: first row and column, part, length and start of k
   __amdgpu_buffer_rsrc_t ra, rb0, rb1;
   const auto place = [&](unsigned tile) {
     unsigned tm, tn;
@@ -220,19 +277,30 @@ __global__ __launch_bounds__(512) void tile_kernel(Work work) {
     dev::grouped_tile(at - part * (tiles_m * tiles_n), tiles_m, tiles_n, tm, tn);
     m0 = tm * C::BM;
     n0 = tn * C::BO;
-    const int k0 = part * p.k_part;
-    k = p.k - k0 < p.k_part ? p.k - k0 : p.k_part;
-    ra = rows_of(p.a + k0, p.lda, m0, p.m, C::BM, k);
-    rb0 = rows_of(p.b[0] + k0, p.ldb[0], n0, p.n, C::BO, k);
-    rb1 = C::GATED ? rows_of(p.b[1] + k0, p.ldb[1], n0, p.n, C::BO, k) : rb0;
+    ks0 = part * p.k_part;
+    k = p.k - ks0 < p.k_part ? p.k - ks0 : p.k_part;
+    if constexpr (!TA) ra = rows_of(p.a + ks0, p.lda, m0, p.m, C::BM, k);
+    if constexpr (!TB) {
+      rb0 = rows_of(p.b[0] + ks0, p.ldb[0], n0, p.n, C::BO, k);
+      rb1 = C::GATED ? rows_of(p.b[1] + ks0, p.ldb[1], n0, p.n, C::BO, k) : rb0;
+    }
   };
   // Image row r of A half h is row 32 XH (r / 16 XH) + 16 XH h + r % 16 XH of the tile; of B half
   // h it is the same with YH and four waves (GATED: row r of operand h).  Piece i of a wave: image rows
   // 8 (P wid + i) + lane / 8, chunk lane % 8.
+  // TA, TB: column c of half h is column (half the tile) h + c of the tile.  Piece i of a wave: bytes
+  // 1024 (P wid + i) on, rows of RA (RT) bytes.
   uint32_t offa[2][C::PA], offb[2][C::PB];
   int ka[C::PA], kb[C::PB];
 #pragma unroll
   for (int i = 0; i < C::PA; i++) {
+    if constexpr (TA) {
+      const int o = (wid * C::PA + i) * 1024 + lane * 16, r = o / RA, c = o % RA / 16;
+#pragma unroll
+      for (int h = 0; h < 2; h++)
+        offa[h][i] = static_cast<uint32_t>((r * p.lda + h * (RA / 2) + 8 * (c ^ 2 * turn<RA>(r))) * 2);
+      continue;
+    }
     const int r = (wid * C::PA + i) * 8 + lane / 8;
     ka[i] = 8 * swz(r, lane % 8);
 #pragma unroll
@@ -243,6 +311,13 @@ __global__ __launch_bounds__(512) void tile_kernel(Work work) {
   }
 #pragma unroll
   for (int i = 0; i < C::PB; i++) {
+    if constexpr (TB) {
+      const int o = (wid * C::PB + i) * 1024 + lane * 16, r = o / RT, c = o % RT / 16;
+#pragma unroll
+      for (int h = 0; h < 2; h++)  // both operands of a fold have one row stride
+        offb[h][i] = static_cast<uint32_t>((r * p.ldb[0] + h * (RT / 2) + 8 * (c ^ 2 * turn<RT>(r))) * 2);
+      continue;
+    }
     const int r = (wid * C::PB + i) * 8 + lane / 8;
     kb[i] = 8 * swz(r, lane % 8);
 #pragma unroll
@@ -255,6 +330,12 @@ __global__ __launch_bounds__(512) void tile_kernel(Work work) {
     constexpr int h = decltype(half)::value;
     uint8_t *dst = lds + decltype(buf)::value * C::kBuf + h * C::kHalfA + wid * (C::PA * 1024);
     const int k0 = tile * C::BK, at = k0 < k ? 2 * k0 : 0;  // (at stays inside the range)
+    if constexpr (TA) {
+      const auto r = columns_of(pa, lda, ks0 + k0, k - k0, m0, pm);
+#pragma unroll
+      for (int i = 0; i < C::PA; i++) dma16(r, dst + i * 1024, offa[h][i], 0);
+      return;
+    }
 #pragma unroll
     for (int i = 0; i < C::PA; i++)
       dma16(ra, dst + i * 1024, ka[i] < k - k0 ? offa[h][i] : kOut, at);
@@ -264,26 +345,50 @@ __global__ __launch_bounds__(512) void tile_kernel(Work work) {
     uint8_t *dst = lds + decltype(buf)::value * C::kBuf + 2 * C::kHalfA + h * C::kHalfB +
                    wid * (C::PB * 1024);
     const int k0 = tile * C::BK, at = k0 < k ? 2 * k0 : 0;
+    if constexpr (TB) {
+      const bool second = ks0 + k0 >= fold;
+      const int row = ks0 + k0 - (second ? fold : 0), left = have - row < k - k0 ? have - row : k - k0;
+      const auto r = columns_of(second ? pb1 : pb0, ldb, row, left, n0, pn);
+#pragma unroll
+      for (int i = 0; i < C::PB; i++) dma16(r, dst + i * 1024, offb[h][i], 0);
+      return;
+    }
 #pragma unroll
     for (int i = 0; i < C::PB; i++)
       dma16(h ? rb1 : rb0, dst + i * 1024, kb[i] < k - k0 ? offb[h][i] : kOut, at);
   };
-  // LDS addresses of this lane's fragments [buffer][32-deep step]
-  uint32_t ata[2][2], atb[2][2];
+  // LDS addresses of this lane's fragments: [buffer][32-deep step], TA, TB: [buffer][16 columns]
+  uint32_t ata[2][TA ? XH : 2], atb[2][TB ? YH : 2];
   {
     const uint32_t base = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_void *)lds));
     const int arow = wm * (16 * XH) + l16, brow = wn * (16 * YH) + l16;
+    const int trow = 8 * lq + l16 / 4, tcol = 8 * (l16 % 4);
 #pragma unroll
-    for (int b = 0; b < 2; b++)
+    for (int b = 0; b < 2; b++) {
 #pragma unroll
-      for (int ks = 0; ks < 2; ks++) {
-        ata[b][ks] = base + b * C::kBuf + arow * C::RB + 16 * swz(arow, 4 * ks + lq);
-        atb[b][ks] = base + b * C::kBuf + 2 * C::kHalfA + brow * C::RB + 16 * swz(brow, 4 * ks + lq);
-      }
+      for (int x = 0; x < (TA ? XH : 2); x++)
+        ata[b][x] = base + b * C::kBuf +
+                    (TA ? trow * RA + 32 * ((wm * XH + x) ^ turn<RA>(trow)) + tcol
+                        : arow * C::RB + 16 * swz(arow, 4 * x + lq));
+#pragma unroll
+      for (int y = 0; y < (TB ? YH : 2); y++)
+        atb[b][y] = base + b * C::kBuf + 2 * C::kHalfA +
+                    (TB ? trow * RT + 32 * ((wn * YH + y) ^ turn<RT>(trow)) + tcol
+                        : brow * C::RB + 16 * swz(brow, 4 * y + lq));
+    }
   }
-  u32x4 fa[XH][2], fb[2][YH][2];
+  Frag<TA> fa[XH][2];
+  Frag<TB> fb[2][YH][2];
   const auto read_a = [&](auto half, auto buf) {
     constexpr int O = decltype(half)::value * C::kHalfA, b = decltype(buf)::value;
+    if constexpr (TA) {
+#pragma unroll
+      for (int x = 0; x < XH; x++) {
+        read_across<O, RA>(fa[x][0], ata[b][x]);
+        read_across<O + 32 * RA, RA>(fa[x][1], ata[b][x]);
+      }
+      return;
+    } else
 #pragma unroll
     for (int ks = 0; ks < 2; ks++) {
       read_frag<O>(fa[0][ks], ata[b][ks]);
@@ -294,6 +399,14 @@ __global__ __launch_bounds__(512) void tile_kernel(Work work) {
   };
   const auto read_b = [&](auto half, auto buf) {
     constexpr int h = decltype(half)::value, O = h * C::kHalfB, b = decltype(buf)::value;
+    if constexpr (TB) {
+#pragma unroll
+      for (int y = 0; y < YH; y++) {
+        read_across<O, RT>(fb[h][y][0], atb[b][y]);
+        read_across<O + 32 * RT, RT>(fb[h][y][1], atb[b][y]);
+      }
+      return;
+    } else
 #pragma unroll
     for (int ks = 0; ks < 2; ks++) {
       read_frag<O>(fb[h][0][ks], atb[b][ks]);
@@ -314,8 +427,8 @@ __global__ __launch_bounds__(512) void tile_kernel(Work work) {
       for (int x = 0; x < XH; x++)
 #pragma unroll
         for (int y = 0; y < YH; y++)
-          acc[i][x][j][y] = C::SAVE ? mma<N>(fa[x][ks], fb[j][y][ks], acc[i][x][j][y])
-                                    : mma<N>(fb[j][y][ks], fa[x][ks], acc[i][x][j][y]);
+          acc[i][x][j][y] = C::SAVE ? mma<N>(whole(fa[x][ks]), whole(fb[j][y][ks]), acc[i][x][j][y])
+                                    : mma<N>(whole(fb[j][y][ks]), whole(fa[x][ks]), acc[i][x][j][y]);
     __builtin_amdgcn_s_setprio(0);
   };
   constexpr std::integral_constant<int, 0> c0{};
@@ -326,28 +439,28 @@ __global__ __launch_bounds__(512) void tile_kernel(Work work) {
     read_a(c0, buf);
     start_b(first, buf, t + 2);
     wait_vmcnt<kFlight>();
-    settle<XH>(fa);
+    settle(fa);
     meet();
     multiply(c0, first);
     meet();
     read_b(second, buf);
     start_a(c0, buf, t + 2);
     wait_vmcnt<kFlight>();
-    settle<YH>(fb[S]);
+    settle(fb[S]);
     meet();
     multiply(c0, second);
     meet();
     read_a(c1, buf);
     start_b(second, buf, t + 2);
     wait_vmcnt<kFlight>();
-    settle<XH>(fa);
+    settle(fa);
     meet();
     multiply(c1, second);
     meet();
     read_b(second, other);  // the next tile's first half
     start_a(c1, buf, t + 2);
     wait_vmcnt<kFlight>();
-    settle<YH>(fb[S]);
+    settle(fb[S]);
     meet();
     multiply(c1, first);
     meet();
@@ -376,7 +489,7 @@ __global__ __launch_bounds__(512) void tile_kernel(Work work) {
     wait_vmcnt<kFlight>();
     meet();
     read_b(c0, c0);
-    settle<YH>(fb[0]);
+    settle(fb[0]);
     meet();
     if (wid >= 4) meet();
     for (int t = 0; t * C::BK < k; t += 2) {
@@ -386,10 +499,13 @@ __global__ __launch_bounds__(512) void tile_kernel(Work work) {
     if (wid < 4) meet();
     wait_vmcnt<0>();  // the pieces started past the end of k have written their zeros
     meet();
-    const int rm = m0 + wm * (32 * XH), rn = n0 + wn * (C::GATED ? 16 * YH : 32 * YH);
+    // first row of accumulator rows i, first column of column block b (of 2 YH; GATED: of YH)
+    const int rm = m0 + wm * (TA ? 16 * XH : 32 * XH), rn = n0 + wn * (C::GATED || TB ? 16 * YH : 32 * YH);
+    const auto row_of = [&](int i, int x) { return rm + i * (TA ? 32 * XH : 16 * XH) + 16 * x; };
+    const auto col_of = [&](int b) { return rn + (TB ? b / YH * (64 * YH) + 16 * (b % YH) : 16 * b); };
     const int64_t skip = static_cast<int64_t>(part) * p.m * p.n;  // where the sums of this part begin
     tile += gridDim.x;
-    if (tile < work.tiles) {
+    if (tile < end) {
       place(tile);
       start_tile();
     }
@@ -403,7 +519,7 @@ __global__ __launch_bounds__(512) void tile_kernel(Work work) {
         for (int x = 0; x < XH; x++)
 #pragma unroll
           for (int b = 0; b < YH; b++) {
-            const int row = rm + (i * XH + x) * 16 + 4 * lq, col = rn + 16 * b + l16;
+            const int row = row_of(i, x) + 4 * lq, col = col_of(b) + l16;
             const floatx4 g = acc[i][x][0][b], u = acc[i][x][1][b];
             float2 *pre = (p.parts > 1 ? reinterpret_cast<float2 *>(p.sums) + skip : p.pre) +
                           static_cast<int64_t>(row) * p.n + col;
@@ -425,7 +541,7 @@ __global__ __launch_bounds__(512) void tile_kernel(Work work) {
               else if (col - odd < p.n) *out = static_cast<uint16_t>(w);
             }
           }
-      if (tile >= work.tiles) return;
+      if (tile >= end) return;
       continue;
     }
     if constexpr (!C::GATED)
@@ -436,7 +552,7 @@ __global__ __launch_bounds__(512) void tile_kernel(Work work) {
           for (int x = 0; x < XH; x++)
 #pragma unroll
             for (int b = 0; b < 2 * YH; b++) {
-              const int row = rm + (i * XH + x) * 16 + l16, col = rn + 16 * b + 4 * lq;
+              const int row = row_of(i, x) + l16, col = col_of(b) + 4 * lq;
               float *dst = p.sums + skip + static_cast<int64_t>(row) * p.n + col;
               const floatx4 v = acc[i][x][b / YH][b % YH];
               if (row >= p.m) continue;
@@ -448,7 +564,7 @@ __global__ __launch_bounds__(512) void tile_kernel(Work work) {
                   if (col + r < p.n) dst[r] = v[r];
               }
             }
-        if (tile >= work.tiles) return;
+        if (tile >= end) return;
         continue;
       }
     // Results: rows of 16-bit values, two neighbouring 16-column blocks exchanged between odd and
@@ -469,7 +585,7 @@ __global__ __launch_bounds__(512) void tile_kernel(Work work) {
     for (int i = 0; i < 2; i++)
 #pragma unroll
       for (int x = 0; x < XH; x++) {
-        const int row = rm + (i * XH + x) * 16 + l16;
+        const int row = row_of(i, x) + l16;
         uint32_t w[NB][2];
 #pragma unroll
         for (int b = 0; b < NB; b++) {
@@ -490,30 +606,50 @@ __global__ __launch_bounds__(512) void tile_kernel(Work work) {
           for (int b = 0; b + 1 < NB; b += 2) {
             const u32x2 lo = __builtin_amdgcn_permlane16_swap(w[b][0], w[b + 1][0], false, false);
             const u32x2 hi = __builtin_amdgcn_permlane16_swap(w[b][1], w[b + 1][1], false, false);
-            put(out, rn + 16 * (b + (lq & 1)) + 8 * (lq >> 1), u32x4{lo.x, hi.x, lo.y, hi.y});
+            put(out, (lq & 1 ? col_of(b + 1) : col_of(b)) + 8 * (lq >> 1), u32x4{lo.x, hi.x, lo.y, hi.y});
           }
 #endif
         } else {
 #pragma unroll
-          for (int b = 0; b < NB; b++) put(out, rn + 16 * b + 4 * lq, u32x2{w[b][0], w[b][1]});
+          for (int b = 0; b < NB; b++) put(out, col_of(b) + 4 * lq, u32x2{w[b][0], w[b][1]});
         }
       }
-    if (tile >= work.tiles) return;
+    if (tile >= end) return;
   }
 }
 
-// Adds the parts of up to two products, in order.  One thread per four results.
+// The forward product: workgroups walk its tiles.
+template <class N, class C>
+__global__ __launch_bounds__(512) void tile_kernel(Work w) {
+  extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+  take_tiles<N, C, false, false>(w.q[0], 0, w.end[0], lds);
+}
+// The backward products: a workgroup per tile.
+template <class N, class C>
+__global__ __launch_bounds__(512) void backward_kernel(Work w) {
+  extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+  int i = 0;
+  while (blockIdx.x >= w.end[i]) i++;
+  const unsigned begin = i ? w.end[i - 1] : 0;
+  if (w.q[i].across) take_tiles<N, C, true, true>(w.q[i], begin, 0, lds);
+  else take_tiles<N, C, false, true>(w.q[i], begin, 0, lds);
+}
+
+// Adds the parts of up to three products, in order.  One thread per four results.
 struct Join {
-  Args q[2];
-  int64_t fours[2];
+  Args q[kProducts];
+  int64_t fours[kProducts];
 };
 template <class N, bool GATED>
 __global__ __launch_bounds__(256) void join_kernel(Join j) {
-  for (int64_t at = blockIdx.x * 256ll + threadIdx.x; at < j.fours[0] + j.fours[1];
+  for (int64_t at = blockIdx.x * 256ll + threadIdx.x; at < j.fours[0] + j.fours[1] + j.fours[2];
        at += gridDim.x * 256ll) {
-    const int w = at < j.fours[0] ? 0 : 1;
+    int64_t i = at;
+    int w = 0;
+    while (i >= j.fours[w]) i -= j.fours[w++];
     const Args &p = j.q[w];
-    const int64_t size = static_cast<int64_t>(p.m) * p.n, i = 4 * (w ? at - j.fours[0] : at);
+    const int64_t size = static_cast<int64_t>(p.m) * p.n;
+    i *= 4;
     constexpr int V = GATED ? 2 : 1;
     float sum[4 * V] = {};
     const int have = size - i < 4 ? static_cast<int>(size - i) : 4;
@@ -738,146 +874,54 @@ __global__ __launch_bounds__(256) void pad_kernel(Pad p) {
   }
 }
 
-// What the backward products read, written by one launch: blocks [0, slope) form dg and du,
-// the rest transpose up to three matrices.
-struct Turn {
-  const uint16_t *src;  // [rows][cols], row stride ld
-  int64_t ld;
-  int rows, cols;
-  uint16_t *dst;        // [cols][rows_p], row stride ld_d; rows_p a multiple of 8, zeros behind rows
-  int64_t ld_d;
-  int rows_p;
-  unsigned tiles_c, tiles;
-};
-struct Prepare {
+// The gradients of g and u as the backward products read them: [m][2 fp], dg's columns, then du's, zeros
+// behind each.
+struct Slopes {
   const uint16_t *dh;
   int64_t ld;
   const float2 *pre;
-  int act, m, f, fp, mp;
-  uint16_t *rows, *cols;  // dg, du as [m][2 fp] (dg, then du) and transposed [2 f][mp]; either may be null
-  unsigned tiles_c, tiles;
-  Turn turn[3];
+  int act, m, f, fp;
+  uint16_t *rows;
 };
 
-constexpr int kLd = 72;  // elements of an LDS row of 64: 16-byte aligned
-
-// Eight values of column c of an LDS tile from row r on.
-__device__ __forceinline__ uint4 column(const uint16_t (&tile)[64][kLd], int r, int c) {
-  uint32_t e[4];
-#pragma unroll
-  for (int j = 0; j < 4; j++)
-    e[j] = tile[r + 2 * j][c] | (static_cast<uint32_t>(tile[r + 2 * j + 1][c]) << 16);
-  return uint4{e[0], e[1], e[2], e[3]};
-}
-
-// 64 x 64 tile: rows in 16-byte pieces into LDS, columns in 16-byte pieces out of it.
-__device__ __forceinline__ void turn_tile(const Turn &t, unsigned block, uint16_t (&tile)[64][kLd]) {
-  const int c0 = static_cast<int>(block % t.tiles_c) * 64, r0 = static_cast<int>(block / t.tiles_c) * 64;
-  const int a = threadIdx.x >> 3, b = (threadIdx.x & 7) * 8;
-  uint4 v[2];
-#pragma unroll
-  for (int i = 0; i < 2; i++) {
-    const int r = r0 + a + 32 * i;
-    v[i] = uint4{0, 0, 0, 0};
-    if (r >= t.rows || c0 + b >= t.cols) continue;
-    const uint16_t *s = t.src + r * t.ld + c0 + b;
-    if (c0 + b + 8 <= t.cols) {
-      __builtin_memcpy(&v[i], s, 16);
+// Four columns of a row a thread: 32 bytes of pairs, 8 of dh and of each result.
+template <class N>
+__global__ __launch_bounds__(256) void slope_kernel(Slopes p) {
+  const int64_t all = static_cast<int64_t>(p.m) * (p.fp / 4);
+  for (int64_t at = blockIdx.x * 256ll + threadIdx.x; at < all; at += gridDim.x * 256ll) {
+    const int64_t r = at / (p.fp / 4);
+    const int c = static_cast<int>(at - r * (p.fp / 4)) * 4;
+    const float2 *s = p.pre + r * p.f + c;
+    const uint16_t *q = p.dh + r * p.ld + c;
+    float2 gu[4] = {};
+    uint16_t d[4] = {};
+    if (c + 4 <= p.f) {
+      __builtin_memcpy(gu, s, 32);
+      __builtin_memcpy(d, q, 8);
     } else {
-      uint32_t e[4] = {0, 0, 0, 0};
-      for (int j = 0; j < 8; j++)
-        if (c0 + b + j < t.cols) e[j / 2] |= static_cast<uint32_t>(s[j]) << (16 * (j & 1));
-      v[i] = uint4{e[0], e[1], e[2], e[3]};
+#pragma unroll
+      for (int e = 0; e < 4; e++)
+        if (c + e < p.f) {
+          gu[e] = s[e];
+          d[e] = q[e];
+        }
     }
-  }
+    uint16_t dg[4], du[4];
 #pragma unroll
-  for (int i = 0; i < 2; i++) *reinterpret_cast<uint4 *>(&tile[a + 32 * i][b]) = v[i];
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < 2; i++) {
-    const int c = c0 + a + 32 * i, r = r0 + b;
-    if (c < t.cols && r < t.rows_p)
-      *reinterpret_cast<uint4 *>(t.dst + c * t.ld_d + r) = column(tile, b, a + 32 * i);
-  }
-}
-
-// (dh, g, u) -> dg, du of a 64 x 64 tile, zeros in the padding: a wave reads two rows of 64 pairs
-// (16 bytes, two columns, a lane), the results meet in LDS and leave 16 bytes a lane both ways.
-template <class N>
-__device__ __forceinline__ void slope_tile(const Prepare &p, uint16_t (&tile)[2][64][kLd]) {
-  const int c0 = static_cast<int>(blockIdx.x % p.tiles_c) * 64;
-  const int r0 = static_cast<int>(blockIdx.x / p.tiles_c) * 64;
-  {
-    const int r1 = threadIdx.x / 32, c = (threadIdx.x % 32) * 2;
-    float4 gu[8];
-    uint32_t d[8];
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-      const int r = r0 + r1 + 8 * i;
-      gu[i] = float4{0.f, 0.f, 0.f, 0.f};
-      d[i] = 0;
-      if (r >= p.m || c0 + c >= p.f) continue;
-      const float2 *s = p.pre + static_cast<int64_t>(r) * p.f + c0 + c;
-      const uint16_t *q = p.dh + r * p.ld + c0 + c;
-      if (c0 + c + 2 <= p.f) {
-        __builtin_memcpy(&gu[i], s, 16);
-        __builtin_memcpy(&d[i], q, 4);
-      } else {
-        gu[i].x = s->x;
-        gu[i].y = s->y;
-        d[i] = *q;
-      }
+    for (int e = 0; e < 4; e++) {  // 0 behind the row: d, g and u are
+      const float v = N::load(d[e]);
+      dg[e] = N::save(v * gu[e].y * act_slope(p.act, gu[e].x));
+      du[e] = N::save(v * act(p.act, gu[e].x));
     }
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-      const float d0 = N::load(static_cast<uint16_t>(d[i])), d1 = N::load(static_cast<uint16_t>(d[i] >> 16));
-      const uint32_t dg = N::save(d0 * gu[i].y * act_slope(p.act, gu[i].x)) |
-                          static_cast<uint32_t>(N::save(d1 * gu[i].w * act_slope(p.act, gu[i].z))) << 16;
-      const uint32_t du = N::save(d0 * act(p.act, gu[i].x)) |
-                          static_cast<uint32_t>(N::save(d1 * act(p.act, gu[i].z))) << 16;
-      // a pair past the end of its row or of the rows is 0: d, g and u are
-      *reinterpret_cast<uint32_t *>(&tile[0][r1 + 8 * i][c]) = dg;
-      *reinterpret_cast<uint32_t *>(&tile[1][r1 + 8 * i][c]) = du;
-    }
+    uint16_t *dst = p.rows + r * (2 * p.fp) + c;
+    __builtin_memcpy(dst, dg, 8);
+    __builtin_memcpy(dst + p.fp, du, 8);
   }
-  __syncthreads();
-  const int a = threadIdx.x >> 3, b = (threadIdx.x & 7) * 8;
-#pragma unroll
-  for (int i = 0; i < 2; i++) {
-    const int lr = a + 32 * i;
-    if (p.rows && c0 + b < p.fp && r0 + lr < p.m) {
-      uint16_t *dst = p.rows + static_cast<int64_t>(r0 + lr) * (2 * p.fp) + c0 + b;
-      *reinterpret_cast<uint4 *>(dst) = *reinterpret_cast<const uint4 *>(&tile[0][lr][b]);
-      *reinterpret_cast<uint4 *>(dst + p.fp) = *reinterpret_cast<const uint4 *>(&tile[1][lr][b]);
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < 2; i++) {
-    const int c = c0 + a + 32 * i, r = r0 + b;
-    if (!p.cols || c >= p.f || r >= p.mp) continue;
-#pragma unroll
-    for (int k = 0; k < 2; k++)
-      *reinterpret_cast<uint4 *>(p.cols + (static_cast<int64_t>(k) * p.f + c) * p.mp + r) =
-          column(tile[k], b, a + 32 * i);
-  }
-}
-
-template <class N>
-__global__ __launch_bounds__(256) void prepare_kernel(Prepare p) {
-  __shared__ __attribute__((aligned(16))) uint16_t tile[2][64][kLd];
-  unsigned block = blockIdx.x;
-  if (block < p.tiles) {
-    slope_tile<N>(p, tile);
-    return;
-  }
-  block -= p.tiles;
-  int i = 0;
-  while (i < 2 && block >= p.turn[i].tiles) block -= p.turn[i++].tiles;
-  turn_tile(p.turn[i], block, tile[0]);
 }
 
 // -------------------------------------------------------------------- host
 constexpr int kFewRows = 64;
+constexpr int64_t kMostLd = 1 << 21;  // 32-bit offsets over 256 rows
 int up8(int64_t v) { return static_cast<int>((v + 7) / 8 * 8); }
 size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 
@@ -895,24 +939,28 @@ int64_t tiles_of(const Args &p) {
 
 template <class N, class C>
 vs_status launch_tile(const Args *q, int count, hipStream_t s) {
-  static const hipError_t attr =
-      hipFuncSetAttribute(reinterpret_cast<const void *>(&tile_kernel<N, C>),
-                          hipFuncAttributeMaxDynamicSharedMemorySize, C::kLds);
+  constexpr auto kernel = [] {
+    if constexpr (C::GATED) return &tile_kernel<N, C>;
+    else return &backward_kernel<N, C>;
+  }();
+  static const hipError_t attr = hipFuncSetAttribute(
+      reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, C::kLds);
   VS_HIP(attr);
   Work w{};
   int64_t tiles = 0;
-  for (int i = 0; i < count; i++) {
-    w.q[i] = q[i];
-    tiles += tiles_of<C>(q[i]);
-    if (i == 0) w.first = static_cast<unsigned>(tiles);
+  for (int i = 0; i < kProducts; i++) {
+    if (i < count) {
+      w.q[i] = q[i];
+      tiles += tiles_of<C>(q[i]);
+    }
+    VS_REQUIRE(tiles < (1ll << 23), "gated_linear: too many output tiles");
+    w.end[i] = static_cast<unsigned>(tiles);
   }
-  VS_REQUIRE(tiles < (1ll << 23), "gated_linear: too many output tiles");
-  w.tiles = static_cast<unsigned>(tiles);
-  // one product: as many workgroups as fit the chip walk its tiles; two: a workgroup per tile,
-  // the longer product's first, so whichever CU is free takes the next
+  // forward: as many workgroups as fit the chip walk the tiles; backward: a workgroup per tile, the
+  // longer products' first, so whichever CU is free takes the next
   const int64_t fit = static_cast<int64_t>(device_cu_count()) * (160 * 1024 / C::kLds);
-  const unsigned grid = static_cast<unsigned>(count == 1 ? std::min(tiles, fit) : tiles);
-  hipLaunchKernelGGL((tile_kernel<N, C>), dim3(grid), dim3(C::kThreads), C::kLds, s, w);
+  const unsigned grid = static_cast<unsigned>(C::GATED ? std::min(tiles, fit) : tiles);
+  hipLaunchKernelGGL(kernel, dim3(grid), dim3(C::kThreads), C::kLds, s, w);
   VS_HIP(hipGetLastError());
   return VS_OK;
 }
@@ -943,17 +991,17 @@ double estimate(const Args *q, int count) {
 
 // Few tiles and a long k leave most of the chip idle: then k is cut, the parts' sums go through memory
 // in fp32, and another launch adds them, which takes about 4 us and reads what was written at
-// about 4 TB/s.  Parts are doubled for the product with the longest tiles as long as the estimate
-// falls.  us in one part and as chosen, bf16: 300 x 8192 to 200 outputs 65 and 20, the backward pass of
-// 64 x 2048 with 16384 outputs 333 and 142, of 8192 x 256 with 256 outputs 79 and 30.
+// about 4 TB/s.  Parts are doubled for the products with the longest tiles as long as the
+// estimate falls.  us in one part and as chosen, bf16: 300 x 8192 to 200 outputs 65 and 20, the backward pass of
+// 64 x 2048 with 16384 outputs 333 and 95, of 8192 x 256 with 256 outputs 79 and 26.
 size_t sums_bytes(const Args &p, bool gated) {
   return p.parts > 1 ? up256(static_cast<size_t>(gated ? 8 : 4) * p.parts * p.m * p.n) : 0;
 }
 template <class C>
 double cut(Args *q, int count) {
   const auto cost = [&] {
-    const double bytes = static_cast<double>(sums_bytes(q[0], C::GATED) + (count > 1 ? sums_bytes(q[1], C::GATED) : 0));
-    double memory = 0;  // the operands once
+    double bytes = 0, memory = 0;  // the parts' sums; the operands once
+    for (int i = 0; i < count; i++) bytes += static_cast<double>(sums_bytes(q[i], C::GATED));
     for (int i = 0; i < count; i++) memory += 2.0 * q[i].k * (q[i].m + (C::GATED ? 2.0 : 1.0) * q[i].n) / 5e6;
     const double time = estimate<C>(q, count);
     return std::max(time, memory) + 0.01 * time + (bytes > 0 ? 4 + bytes / 2e6 : 0);
@@ -961,14 +1009,23 @@ double cut(Args *q, int count) {
   for (int i = 0; i < count; i++) q[i].parts = 1, q[i].k_part = std::max(q[i].k, 1);
   double best = cost();
   for (;;) {
-    const int i = count == 2 && k_tiles(q[1]) > k_tiles(q[0]) ? 1 : 0;
-    const Args before = q[i];
-    if (k_tiles(before) < 8 || before.parts >= 32) return best;
-    q[i].k_part = (k_tiles(before) + 1) / 2 * 64;
-    q[i].parts = (q[i].k + q[i].k_part - 1) / q[i].k_part;
+    Args before[kProducts];
+    int longest = 0;
+    for (int i = 0; i < count; i++) {
+      before[i] = q[i];
+      longest = std::max(longest, k_tiles(q[i]));
+    }
+    if (longest < 8) return best;
+    for (int i = 0; i < count; i++)
+      if (k_tiles(q[i]) == longest && q[i].parts >= 32) return best;
+    for (int i = 0; i < count; i++) {
+      if (k_tiles(before[i]) < longest) continue;
+      q[i].k_part = (longest + 1) / 2 * 64;
+      q[i].parts = (q[i].k + q[i].k_part - 1) / q[i].k_part;
+    }
     const double now = cost();
     if (now >= best) {
-      q[i] = before;
+      std::copy(before, before + count, q);
       return best;
     }
     best = now;
@@ -978,7 +1035,7 @@ double cut(Args *q, int count) {
 // Tile shape (0: 256 x 256, 1: 128 x 256, 2: 128 x 128) and the parts of each product.
 template <bool GATED>
 int plan(Args *q, int count) {
-  Args w[2], s[2];
+  Args w[kProducts], s[kProducts];
   for (int i = 0; i < count; i++) w[i] = s[i] = q[i];
   const double large = cut<Cfg<4, 2, GATED>>(q, count), wide = cut<Cfg<2, 2, GATED>>(w, count),
                small = cut<Cfg<2, 1, GATED>>(s, count);
@@ -1009,7 +1066,7 @@ vs_status product(int shape, const Args *q, int count, hipStream_t s) {
       j.fours[n] = (static_cast<int64_t>(q[i].m) * q[i].n + 3) / 4;
       j.q[n++] = q[i];
     }
-  if (const int64_t all = j.fours[0] + j.fours[1]) {
+  if (const int64_t all = j.fours[0] + j.fours[1] + j.fours[2]) {
     const unsigned grid = static_cast<unsigned>(std::min<int64_t>((all + 255) / 256, 1 << 20));
     hipLaunchKernelGGL((join_kernel<N, GATED>), dim3(grid), dim3(256), 0, s, j);
     VS_HIP(hipGetLastError());
@@ -1042,6 +1099,33 @@ vs_status open_space(Space &sp, DeviceBuffer &own, void *workspace, size_t bytes
   }
   return VS_OK;
 }
+
+// Copies of operands whose rows the DMA cannot read, to rows of whole 16-byte pieces.
+struct Copies {
+  Space &sp;
+  Pad pd{};
+  int n = 0;
+  Copies(Space &space, int cols) : sp(space) {
+    pd.cols = cols;
+    pd.cols_p = up8(cols);
+  }
+  void add(const uint16_t *&src, int64_t &ld, int64_t rows) {
+    pd.src[n] = src;
+    pd.ld[n] = ld;
+    pd.dst[n] = sp.take(static_cast<size_t>(rows) * pd.cols_p);
+    pd.pieces[n] = rows * (pd.cols_p / 8);
+    src = pd.dst[n++];
+    ld = pd.cols_p;
+  }
+  vs_status launch(hipStream_t s) {
+    if (const int64_t all = pd.pieces[0] + pd.pieces[1] + pd.pieces[2]) {
+      const unsigned grid = static_cast<unsigned>(std::min<int64_t>((all + 255) / 256, 1 << 20));
+      hipLaunchKernelGGL(pad_kernel, dim3(grid), dim3(256), 0, s, pd);
+      VS_HIP(hipGetLastError());
+    }
+    return VS_OK;
+  }
+};
 
 vs_status check(const char *who, int dtype, int act, int64_t m, int64_t f, int64_t k) {
   VS_REQUIRE(dtype == VS_F16 || dtype == VS_BF16, "%s: unsupported dtype %d (fp16, bf16)", who, dtype);
@@ -1124,56 +1208,42 @@ vs_status forward(Args p, void *workspace, size_t bytes, hipStream_t s) {
   Space sp;
   VS_TRY(open_space(sp, own, workspace, bytes, q.bytes, s));
   const int kp = up8(p.k);
-  Pad pd{};
-  pd.cols = p.k;
-  pd.cols_p = kp;
-  int n = 0;
-  const auto copy = [&](const uint16_t *&src, int64_t &ld, int64_t rows) {
-    pd.src[n] = src;
-    pd.ld[n] = ld;
-    pd.dst[n] = sp.take(static_cast<size_t>(rows) * kp);
-    pd.pieces[n] = rows * (kp / 8);
-    src = pd.dst[n++];
-    ld = kp;
-  };
-  if (q.px) copy(p.a, p.lda, p.m);
-  if (q.pg) copy(p.b[0], p.ldb[0], p.n);
-  if (q.pu) copy(p.b[1], p.ldb[1], p.n);
-  if (const int64_t all = pd.pieces[0] + pd.pieces[1] + pd.pieces[2]) {
-    const unsigned grid = static_cast<unsigned>(std::min<int64_t>((all + 255) / 256, 1 << 20));
-    hipLaunchKernelGGL(pad_kernel, dim3(grid), dim3(256), 0, s, pd);
-    VS_HIP(hipGetLastError());
-  }
+  Copies copies(sp, p.k);
+  if (q.px) copies.add(p.a, p.lda, p.m);
+  if (q.pg) copies.add(p.b[0], p.ldb[0], p.n);
+  if (q.pu) copies.add(p.b[1], p.ldb[1], p.n);
+  VS_TRY(copies.launch(s));
   if (q.sums) p.sums = sp.take_sums(q.sums);
   p.k = kp;  // (the same where nothing was copied: a direct operand has whole pieces)
   if (p.parts == 1) p.k_part = kp;
   return product<N, true>(q.shape, &p, 1, s);
 }
 
-// The backward products' sizes, the longer k first: dx = [dg du] [Wg; Wu] and dw = [dg du]^T x.
+// The backward products, the longer k first: dx = [dg du] [Wg; Wu], dWg = dg^T x and dWu = du^T x.
 struct BackwardNeed {
-  Args q[2];
+  Args q[kProducts];
   int count, shape;
-  int dx, dw;  // which of q each is, or -1
+  int dx, dw;  // the first of q that each is, or -1
   size_t bytes;
 };
-BackwardNeed backward_need(int64_t m, int64_t f, int64_t k, bool dx, bool dw) {
+BackwardNeed backward_need(int64_t m, int64_t f, int64_t k, bool dx, bool dw, bool ax, bool aw) {
   BackwardNeed b{};
-  const size_t fp = up8(f), mp = up8(m);
-  const auto add = [&](int64_t rows, int64_t inner) {
+  const int fp = static_cast<int>((f + 63) / 64 * 64);
+  const auto add = [&](int64_t rows, int64_t inner, int across) {
     Args &p = b.q[b.count];
     p.m = static_cast<int>(rows);
     p.n = static_cast<int>(k);
-    p.k = static_cast<int>(inner);
+    p.k = p.fold = p.have = static_cast<int>(inner);
+    p.across = across;
     return b.count++;
   };
   b.dx = b.dw = -1;
-  const bool first = 2 * fp >= mp;
-  if (dx && m && first) b.dx = add(m, 2 * fp);
-  if (dw && f) b.dw = add(2 * f, mp);
-  if (dx && m && !first) b.dx = add(m, 2 * fp);
-  b.bytes = (dx ? up256(2 * m * 2 * fp) + up256(2 * k * 2 * fp) : 0) +
-            (dw ? up256(2 * 2 * f * mp) + up256(2 * k * mp) : 0);
+  const bool first = 2 * fp >= m;
+  if (dx && m && first) b.dx = add(m, 2 * fp, 0);
+  if (dw && f) b.dw = add(f, m, 1), add(f, m, 1);
+  if (dx && m && !first) b.dx = add(m, 2 * fp, 0);
+  const size_t kp = up8(k);
+  b.bytes = up256(2 * m * 2 * fp) + (dw && !ax ? up256(2 * m * kp) : 0) + (dx && !aw ? 2 * up256(2 * f * kp) : 0);
   if (b.count) b.shape = plan<false>(b.q, b.count);
   for (int i = 0; i < b.count; i++) b.bytes += sums_bytes(b.q[i], false);
   return b;
@@ -1186,57 +1256,56 @@ vs_status backward(const uint16_t *x, int64_t ldx, const uint16_t *wg, int64_t l
                    void *workspace, size_t bytes, hipStream_t s) {
   DeviceBuffer own;
   Space sp;
-  BackwardNeed need = backward_need(m, f, k, dx, dw);
+  // read as they are: rows apart (what lies behind the last one has to be out of range), and both weights
+  // with one row stride
+  const bool ax = direct(x, ldx, k) && ldx >= k && ldx < kMostLd,
+             aw = direct(wg, ldg, k) && direct(wu, ldu, k) && ldg == ldu && ldg >= k && ldg < kMostLd;
+  BackwardNeed need = backward_need(m, f, k, dx, dw, ax, aw);
   VS_TRY(open_space(sp, own, workspace, bytes, need.bytes, s));
-  const int fp = up8(f), mp = up8(m);
-  uint16_t *rows = dx ? sp.take(static_cast<size_t>(m) * 2 * fp) : nullptr;
-  uint16_t *wt = dx ? sp.take(static_cast<size_t>(k) * 2 * fp) : nullptr;
-  uint16_t *cols = dw ? sp.take(static_cast<size_t>(2) * f * mp) : nullptr;
-  uint16_t *xt = dw ? sp.take(static_cast<size_t>(k) * mp) : nullptr;
-  Prepare pr{};
-  pr.dh = dh;
-  pr.ld = ldh;
-  pr.pre = pre;
-  pr.act = act;
-  pr.m = m;
-  pr.f = f;
-  pr.fp = fp;
-  pr.mp = mp;
-  pr.rows = rows;
-  pr.cols = cols;
-  pr.tiles_c = (fp + 63) / 64;
-  int64_t blocks = static_cast<int64_t>(pr.tiles_c) * ((mp + 63) / 64);
-  VS_REQUIRE(blocks < (1ll << 23), "gated_linear: too many tiles");
-  pr.tiles = static_cast<unsigned>(blocks);
-  int turns = 0;
-  const auto turn = [&](const uint16_t *src, int64_t ld, int r, int c, uint16_t *dst, int64_t ld_d, int rp) {
-    Turn &t = pr.turn[turns++];
-    t = Turn{src, ld, r, c, dst, ld_d, rp, static_cast<unsigned>((c + 63) / 64), 0};
-    const int64_t n = static_cast<int64_t>(t.tiles_c) * ((rp + 63) / 64);
-    t.tiles = static_cast<unsigned>(std::min<int64_t>(n, 1ll << 23));
-    blocks += n;
-  };
-  if (dx) {
-    turn(wg, ldg, f, k, wt, 2 * fp, fp);
-    turn(wu, ldu, f, k, wt + fp, 2 * fp, fp);
-  }
-  if (dw) turn(x, ldx, m, k, xt, mp, mp);
-  const auto set = [&](int i, const uint16_t *a, const uint16_t *b, uint16_t *c) {
-    if (i < 0) return;
-    Args &p = need.q[i];
-    p.a = a;
-    p.b[0] = b;
-    p.lda = p.ldb[0] = p.k;
-    p.c = c;
-    if (const size_t sums = sums_bytes(p, false)) p.sums = sp.take_sums(sums);
-  };
-  set(need.dx, rows, wt, dx);
-  set(need.dw, cols, xt, dw);
-  VS_REQUIRE(blocks < (1ll << 23), "gated_linear: too many tiles");
-  if (blocks) {
-    hipLaunchKernelGGL((prepare_kernel<N>), dim3(static_cast<unsigned>(blocks)), dim3(256), 0, s, pr);
+  const int fp = (f + 63) / 64 * 64;
+  Slopes sl{};
+  sl.dh = dh;
+  sl.ld = ldh;
+  sl.pre = pre;
+  sl.act = act;
+  sl.m = m;
+  sl.f = f;
+  sl.fp = fp;
+  sl.rows = sp.take(static_cast<size_t>(m) * 2 * fp);
+  if (const int64_t n = static_cast<int64_t>(m) * (fp / 4)) {
+    const unsigned grid = static_cast<unsigned>(std::min<int64_t>((n + 255) / 256, 1 << 20));
+    hipLaunchKernelGGL((slope_kernel<N>), dim3(grid), dim3(256), 0, s, sl);
     VS_HIP(hipGetLastError());
   }
+  Copies copies(sp, k);
+  if (dw && !ax) copies.add(x, ldx, m);
+  if (dx && !aw) {
+    copies.add(wg, ldg, f);
+    copies.add(wu, ldu, f);
+  }
+  VS_TRY(copies.launch(s));
+  if (need.dx >= 0) {
+    Args &p = need.q[need.dx];
+    p.a = sl.rows;
+    p.lda = 2 * fp;
+    p.b[0] = wg;
+    p.b[1] = wu;
+    p.ldb[0] = ldg;
+    p.fold = fp;
+    p.have = f;
+    p.c = dx;
+  }
+  if (need.dw >= 0)
+    for (int i = 0; i < 2; i++) {
+      Args &p = need.q[need.dw + i];
+      p.a = sl.rows + i * fp;
+      p.lda = 2 * fp;
+      p.b[0] = p.b[1] = x;
+      p.ldb[0] = ldx;
+      p.c = dw + static_cast<int64_t>(i) * f * k;
+    }
+  for (int i = 0; i < need.count; i++)
+    if (const size_t sums = sums_bytes(need.q[i], false)) need.q[i].sums = sp.take_sums(sums);
   return need.count ? product<N, false>(need.shape, need.q, need.count, s) : VS_OK;
 }
 
@@ -1288,9 +1357,11 @@ vs_status vs_gated_linear(int dtype, int act, const void *x, int64_t ldx, const 
                           : glin::forward<num::F16>(p, workspace, workspace_bytes, s);
 }
 
-size_t vs_gated_linear_backward_workspace(int64_t m, int64_t f, int64_t k, int want_dx, int want_dw) {
+size_t vs_gated_linear_backward_workspace(int64_t m, int64_t f, int64_t k, int want_dx, int want_dw,
+                                          int aligned) {
   if (glin::check("", VS_BF16, 0, m, f, k) != VS_OK) return 0;
-  return k ? glin::backward_need(m, f, k, want_dx != 0, want_dw != 0).bytes : 0;
+  const bool al = aligned != 0;
+  return k ? glin::backward_need(m, f, k, want_dx != 0, want_dw != 0, al, al).bytes : 0;
 }
 
 vs_status vs_gated_linear_backward(int dtype, int act, const void *x, int64_t ldx,
@@ -1303,8 +1374,6 @@ vs_status vs_gated_linear_backward(int dtype, int act, const void *x, int64_t ld
   if (k == 0 || (!dx && !dw)) return VS_OK;
   VS_REQUIRE((m == 0 || f == 0) || (x && w_gate && w_up && pre && dh),
              "gated_linear_backward: null pointer");
-  // rows are the reduction of the weights' gradients: 256 of them, transposed, below 2^31 bytes
-  VS_REQUIRE(!dw || m < (1 << 22) - 8, "gated_linear_backward: too many rows for the weights' gradients (2^22)");
   const hipStream_t s = static_cast<hipStream_t>(stream);
   const auto u16 = [](const void *v) { return static_cast<const uint16_t *>(v); };
   const auto go = [&](auto tag) {

@@ -398,14 +398,16 @@ vs_status vs_gated_linear(int dtype, int act, const void *x, int64_t ldx, const 
 size_t vs_gated_linear_workspace(int64_t m, int64_t f, int64_t k, int aligned);
 /// Gradients of vs_gated_linear from dh [m][f] (row stride ld_dh) and pre:
 /// dx [m][k] and dw [2 f][k] (w_gate's rows, then w_up's); NULL skips one.
-/// dw takes fewer than 2^22 - 8 rows.
+/// The workspace needs fewer bytes with aligned = 1: x and the weights are rows of
+/// whole 16-byte pieces, at least k and less than 2^21 elements apart, w_gate's
+/// as far as w_up's.
 vs_status vs_gated_linear_backward(int dtype, int act, const void *x, int64_t ldx,
                                    const void *w_gate, int64_t ld_gate, const void *w_up,
                                    int64_t ld_up, const float *pre, const void *dh, int64_t ld_dh,
                                    int64_t m, int64_t f, int64_t k, void *dx, void *dw,
                                    void *workspace, size_t workspace_bytes, vs_stream_t stream);
 size_t vs_gated_linear_backward_workspace(int64_t m, int64_t f, int64_t k, int want_dx,
-                                          int want_dw);
+                                          int want_dw, int aligned);
 
 SIMD_API_END
 

@@ -549,7 +549,8 @@ def _gated_backward_impl(x, w_gate, w_up, pre, dh, activation, want_dx, want_dw)
     w_gate, w_up, pre = _near_rows(w_gate, False), _near_rows(w_up, False), pre.contiguous()
     dx = torch.empty(x.shape if want_dx else (0,), dtype=x.dtype, device=x.device)
     dw = torch.empty((2 * f, k) if want_dw else (0,), dtype=x.dtype, device=x.device)
-    size = int(_lib.lib().vs_gated_linear_backward_workspace(m, f, k, int(want_dx), int(want_dw)))
+    aligned = (w_gate.stride(0) == w_up.stride(0) >= k <= rows.stride(0)) and _aligned(rows, w_gate, w_up)
+    size = int(_lib.lib().vs_gated_linear_backward_workspace(m, f, k, want_dx, want_dw, aligned))
     ws = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
     launch(x, "vs_gated_linear_backward", DTYPES[x.dtype], ACTIVATIONS[activation], rows.data_ptr(),
            rows.stride(0), w_gate.data_ptr(), w_gate.stride(0), w_up.data_ptr(), w_up.stride(0), pre.data_ptr(),
@@ -634,7 +635,7 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor,
     function), relu or sigmoid.  Sums, activation and product are float32 and rounded once.  Differentiable
     in x and the weights; the float32 pairs (x @ w_gate.T, x @ w_up.T), 8 bytes per output, are kept for the
     backward pass, and the gradients of the two products are rounded to x's type before they are
-    multiplied (the weights' gradients take up to 2^22 - 9 rows).  Up to 64 rows (generation) stream the weights once at memory speed."""
+    multiplied.  Up to 64 rows (generation) stream the weights once at memory speed."""
     save = records(x, w_gate, w_up)
     if plain_tensors(x, w_gate, w_up):
         if save:
