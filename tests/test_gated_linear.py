@@ -239,7 +239,7 @@ def test_not_finite_rows_stay_in_their_rows(m):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("m,k", [(8, 96), (200, 96), (200, 75)])
+@pytest.mark.parametrize("m,k", [(8, 96), (200, 96), (200, 75), (200, 4800), (3000, 64)])
 def test_streams_captures_and_repeats(m, k):
     args = _inputs(m, k, 80, torch.bfloat16, "cuda", seed=8)
 
