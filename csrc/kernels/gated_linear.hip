@@ -1374,6 +1374,9 @@ vs_status vs_gated_linear_backward(int dtype, int act, const void *x, int64_t ld
   if (k == 0 || (!dx && !dw)) return VS_OK;
   VS_REQUIRE((m == 0 || f == 0) || (x && w_gate && w_up && pre && dh),
              "gated_linear_backward: null pointer");
+  VS_REQUIRE((m <= 1 || ((ldx >= k || ldx == 0) && (ld_dh >= f || ld_dh == 0))) &&
+                 (f <= 1 || (ld_gate >= k && ld_up >= k)),
+             "gated_linear_backward: leading dimension too small");
   const hipStream_t s = static_cast<hipStream_t>(stream);
   const auto u16 = [](const void *v) { return static_cast<const uint16_t *>(v); };
   const auto go = [&](auto tag) {

@@ -159,6 +159,7 @@ def test_shapes_strides_and_alignment(dev, m):
         _all(change(x), change(wg), change(wu), change(dh), "silu")
     _all(shifted(x, 8), wg, shifted(wu, 8), dh, "silu")
     _all(x, shifted(wg, 1), wu, dh, "silu")
+    _all(x, wg, wu, dh.flatten()[:5 * m + 35].as_strided((m, 40), (5, 1)), "silu")   # rows that overlap
     _all(shifted(x, 3), wg, wu, dh, "silu")
     far = torch.zeros(2 * (1 << 21) + 64, dtype=torch.bfloat16, device=dev)   # rows 2^21 elements apart
     two = far.as_strided((2, 64), (1 << 21, 1)).copy_(x[:2])
@@ -299,6 +300,9 @@ def test_native_refusals():
     assert lib.vs_gated_linear_workspace(-1, 1, 1, 0) == 0
     assert lib.vs_gated_linear_backward(5, 0, p, 8, p, 8, p, 8, p, p, 1, 9, 1, 8, None, p, p, 16, None) == 1
     assert b"workspace" in lib.vs_last_error()
+    for ldx, ldg, ldu, ldh in ((7, 8, 8, 2), (8, 7, 8, 2), (8, 8, -8, 2), (8, 8, 8, 1)):
+        assert lib.vs_gated_linear_backward(5, 0, p, ldx, p, ldg, p, ldu, p, p, ldh, 9, 2, 8, p, p, None, 0, None) == 1
+        assert b"leading dimension" in lib.vs_last_error()
 
 
 @pytest.mark.parametrize("dev", DEVICES)

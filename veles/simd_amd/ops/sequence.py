@@ -533,7 +533,7 @@ def _gated_backward_impl(x, w_gate, w_up, pre, dh, activation, want_dx, want_dw)
     name = "veles::gated_linear_backward"
     _check_gated(name, x, w_gate, w_up, activation)
     f, k = w_gate.shape
-    rows, dhr = _near_rows(_as_rows(x), True), _as_rows(dh)
+    rows, dhr = _near_rows(_as_rows(x), True), _near_rows(_as_rows(dh), True)
     m = rows.shape[0]
     if dh.dtype != x.dtype or tuple(dh.shape) != (*x.shape[:-1], f):
         raise ValueError(f"{name}: dh is {dh.dtype} {tuple(dh.shape)}, {x.dtype} {(*x.shape[:-1], f)} expected")
