@@ -27,7 +27,8 @@
 //
 // Roundings: h once; for training, g and u are kept in fp32 (a 16-bit copy would add its own
 // rounding to every gradient, 1.7 instead of 1.4 times the error of the result's own rounding);
-// dg and du are rounded to the operands' type because the matrix cores multiply 16-bit numbers.
+// dg and du are rounded to the operands' type because the matrix cores multiply 16-bit numbers, or,
+// where the caller asks for it, taken as sums of two such numbers, for twice the products.
 // Copyright 2026 veles.simd_amd authors. Apache-2.0.
 #include <hip/hip_runtime.h>
 
@@ -94,13 +95,14 @@ __device__ __forceinline__ float act_slope(int kind, float g) {
 
 // ------------------------------------------------------------------- tiles
 struct Args {
-  // Forward: a [m][k], b[0] and b[1] [n][k].  Backward: a [m][k] or, with `across`, [k][m]; b [k][n],
-  // of which the first `fold` rows are b[0] and those behind b[1], `have` rows of each (zeros behind).
+  // Forward: a [m][k], b[0] and b[1] [n][k].  Backward: a [m][k] or, with `across`, [k][m]; b [k][n].  Every
+  // `fold` rows of b are b[0] and b[1] in turn, `have` rows of each (zeros behind), up to four times; with
+  // `across` every `fold` rows of a begin `next` columns further on, from the first row again.
   const uint16_t *a;
   const uint16_t *b[2];
   int64_t lda, ldb[2];
   int m, n, k;            // n: outputs (columns of h, or of c)
-  int across, fold, have;
+  int across, fold, have, next;
   uint16_t *c;            // [m][n], row stride n
   float2 *pre;            // [m][n] (g, u), or null
   int act;
@@ -255,15 +257,27 @@ __device__ __forceinline__ void meet() {
 // TA, TB: the operand has k as its rows.  Its image halves are 64 k of neighbouring columns then, and
 // fragments are read across: ds_read_b64_tr_b16 gives lane i of 16 the i-th of 16 columns of four
 // rows, whose 8-byte pieces lanes 4 r .. 4 r + 3 point at.  Columns past the end read what lies there
-// (inside the operand) and are not stored.
-template <class N, class C, bool TA, bool TB>
+// (inside the operand) and are not stored.  SPLIT: their rows begin again, at most three times (TA once).
+template <class N, class C, bool TA, bool TB, bool SPLIT>
 __device__ __forceinline__ void take_tiles(const Args &p, unsigned begin, unsigned end, uint8_t *lds) {
   constexpr int XH = C::XH, YH = C::YH;
   constexpr int RA = TA ? 64 * XH : C::RB, RT = TB ? 128 * YH : C::RB;  // bytes of an image row
   const unsigned tiles_m = (p.m + C::BM - 1) / C::BM, tiles_n = (p.n + C::BO - 1) / C::BO;
   const uint16_t *pa = p.a, *pb0 = p.b[0], *pb1 = p.b[1];
   const int64_t lda = p.lda, ldb = p.ldb[0];
-  const int pm = p.m, pn = p.n, fold = p.fold, have = p.have;
+  const int pm = p.m, pn = p.n, fold = p.fold, have = p.have, next = p.next;
+  // Row of the operand that step `at` of k is, and how often the rows began again before it (`most` times at most).
+  const auto unfold = [&](auto most, int at, int &row) {
+    int turns = 0;
+    row = at;
+#pragma unroll
+    for (int i = 0; i < decltype(most)::value; i++)
+      if (row >= fold) {
+        row -= fold;
+        turns++;
+      }
+    return turns;
+  };
   const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wid / 4, wn = wid % 4;
   const int l16 = lane & 15, lq = lane >> 4;
@@ -331,7 +345,10 @@ __device__ __forceinline__ void take_tiles(const Args &p, unsigned begin, unsign
     uint8_t *dst = lds + decltype(buf)::value * C::kBuf + h * C::kHalfA + wid * (C::PA * 1024);
     const int k0 = tile * C::BK, at = k0 < k ? 2 * k0 : 0;  // (at stays inside the range)
     if constexpr (TA) {
-      const auto r = columns_of(pa, lda, ks0 + k0, k - k0, m0, pm);
+      int row;
+      const int turns = unfold(std::integral_constant<int, SPLIT ? 1 : 0>{}, ks0 + k0, row);
+      const int left = have - row < k - k0 ? have - row : k - k0;
+      const auto r = columns_of(pa + turns * next, lda, row, left, m0, pm);
 #pragma unroll
       for (int i = 0; i < C::PA; i++) dma16(r, dst + i * 1024, offa[h][i], 0);
       return;
@@ -346,9 +363,10 @@ __device__ __forceinline__ void take_tiles(const Args &p, unsigned begin, unsign
                    wid * (C::PB * 1024);
     const int k0 = tile * C::BK, at = k0 < k ? 2 * k0 : 0;
     if constexpr (TB) {
-      const bool second = ks0 + k0 >= fold;
-      const int row = ks0 + k0 - (second ? fold : 0), left = have - row < k - k0 ? have - row : k - k0;
-      const auto r = columns_of(second ? pb1 : pb0, ldb, row, left, n0, pn);
+      int row;
+      const int turns = unfold(std::integral_constant<int, SPLIT ? 3 : 1>{}, ks0 + k0, row);
+      const int left = have - row < k - k0 ? have - row : k - k0;
+      const auto r = columns_of(turns & 1 ? pb1 : pb0, ldb, row, left, n0, pn);
 #pragma unroll
       for (int i = 0; i < C::PB; i++) dma16(r, dst + i * 1024, offb[h][i], 0);
       return;
@@ -622,17 +640,17 @@ __device__ __forceinline__ void take_tiles(const Args &p, unsigned begin, unsign
 template <class N, class C>
 __global__ __launch_bounds__(512) void tile_kernel(Work w) {
   extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
-  take_tiles<N, C, false, false>(w.q[0], 0, w.end[0], lds);
+  take_tiles<N, C, false, false, false>(w.q[0], 0, w.end[0], lds);
 }
 // The backward products: a workgroup per tile.
-template <class N, class C>
+template <class N, class C, bool SPLIT>
 __global__ __launch_bounds__(512) void backward_kernel(Work w) {
   extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
   int i = 0;
   while (blockIdx.x >= w.end[i]) i++;
   const unsigned begin = i ? w.end[i - 1] : 0;
-  if (w.q[i].across) take_tiles<N, C, true, true>(w.q[i], begin, 0, lds);
-  else take_tiles<N, C, false, true>(w.q[i], begin, 0, lds);
+  if (w.q[i].across) take_tiles<N, C, true, true, SPLIT>(w.q[i], begin, 0, lds);
+  else take_tiles<N, C, false, true, SPLIT>(w.q[i], begin, 0, lds);
 }
 
 // Adds the parts of up to three products, in order.  One thread per four results.
@@ -875,14 +893,21 @@ __global__ __launch_bounds__(256) void pad_kernel(Pad p) {
 }
 
 // The gradients of g and u as the backward products read them: [m][2 fp], dg's columns, then du's, zeros
-// behind each.
+// behind each.  With `split` every one is the sum of two 16-bit numbers (to 2^-16 of it in bf16, 2^-22 or 2^-25
+// in fp16), and the rows are [4 fp], the second numbers in the same order behind the first.
 struct Slopes {
   const uint16_t *dh;
   int64_t ld;
   const float2 *pre;
-  int act, m, f, fp;
+  int act, m, f, fp, split;
   uint16_t *rows;
 };
+// What the rounded value `hi` leaves of v; nothing where it is infinite or no number.
+template <class N>
+__device__ __forceinline__ uint16_t rest(float v, uint16_t hi) {
+  const float r = v - N::load(hi);
+  return N::save(fabsf(r) < __builtin_inff() ? r : 0.f);
+}
 
 // Four columns of a row a thread: 32 bytes of pairs, 8 of dh and of each result.
 template <class N>
@@ -907,15 +932,27 @@ __global__ __launch_bounds__(256) void slope_kernel(Slopes p) {
         }
     }
     uint16_t dg[4], du[4];
+    float vg[4], vu[4];
 #pragma unroll
     for (int e = 0; e < 4; e++) {  // 0 behind the row: d, g and u are
       const float v = N::load(d[e]);
-      dg[e] = N::save(v * gu[e].y * act_slope(p.act, gu[e].x));
-      du[e] = N::save(v * act(p.act, gu[e].x));
+      vg[e] = v * gu[e].y * act_slope(p.act, gu[e].x);
+      vu[e] = v * act(p.act, gu[e].x);
+      dg[e] = N::save(vg[e]);
+      du[e] = N::save(vu[e]);
     }
-    uint16_t *dst = p.rows + r * (2 * p.fp) + c;
+    uint16_t *dst = p.rows + r * (p.split ? 4 : 2) * p.fp + c;
     __builtin_memcpy(dst, dg, 8);
     __builtin_memcpy(dst + p.fp, du, 8);
+    if (p.split) {
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        dg[e] = rest<N>(vg[e], dg[e]);
+        du[e] = rest<N>(vu[e], du[e]);
+      }
+      __builtin_memcpy(dst + 2 * p.fp, dg, 8);
+      __builtin_memcpy(dst + 3 * p.fp, du, 8);
+    }
   }
 }
 
@@ -937,11 +974,11 @@ int64_t tiles_of(const Args &p) {
   return static_cast<int64_t>((p.m + C::BM - 1) / C::BM) * ((p.n + C::BO - 1) / C::BO) * p.parts;
 }
 
-template <class N, class C>
+template <class N, class C, bool SPLIT>
 vs_status launch_tile(const Args *q, int count, hipStream_t s) {
   constexpr auto kernel = [] {
     if constexpr (C::GATED) return &tile_kernel<N, C>;
-    else return &backward_kernel<N, C>;
+    else return &backward_kernel<N, C, SPLIT>;
   }();
   static const hipError_t attr = hipFuncSetAttribute(
       reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, C::kLds);
@@ -1044,20 +1081,20 @@ int plan(Args *q, int count) {
   return wide <= small ? 1 : 2;
 }
 
-template <class N, bool GATED, bool SAVE>
+template <class N, bool GATED, bool SAVE, bool SPLIT>
 vs_status launch_shape(int shape, const Args *q, int count, hipStream_t s) {
-  if (shape == 0) return launch_tile<N, Cfg<4, 2, GATED, SAVE>>(q, count, s);
-  if (shape == 1) return launch_tile<N, Cfg<2, 2, GATED, SAVE>>(q, count, s);
-  return launch_tile<N, Cfg<2, 1, GATED, SAVE>>(q, count, s);
+  if (shape == 0) return launch_tile<N, Cfg<4, 2, GATED, SAVE>, SPLIT>(q, count, s);
+  if (shape == 1) return launch_tile<N, Cfg<2, 2, GATED, SAVE>, SPLIT>(q, count, s);
+  return launch_tile<N, Cfg<2, 1, GATED, SAVE>, SPLIT>(q, count, s);
 }
 
-template <class N, bool GATED>
+template <class N, bool GATED, bool SPLIT = false>
 vs_status product(int shape, const Args *q, int count, hipStream_t s) {
   if constexpr (GATED) {
-    if (q->pre || q->parts > 1) VS_TRY((launch_shape<N, true, true>(shape, q, count, s)));
-    else VS_TRY((launch_shape<N, true, false>(shape, q, count, s)));
+    if (q->pre || q->parts > 1) VS_TRY((launch_shape<N, true, true, false>(shape, q, count, s)));
+    else VS_TRY((launch_shape<N, true, false, false>(shape, q, count, s)));
   } else {
-    VS_TRY((launch_shape<N, false, false>(shape, q, count, s)));
+    VS_TRY((launch_shape<N, false, false, SPLIT>(shape, q, count, s)));
   }
   Join j{};
   int n = 0;
@@ -1219,31 +1256,39 @@ vs_status forward(Args p, void *workspace, size_t bytes, hipStream_t s) {
   return product<N, true>(q.shape, &p, 1, s);
 }
 
-// The backward products, the longer k first: dx = [dg du] [Wg; Wu], dWg = dg^T x and dWu = du^T x.
+// The backward products, the longer k first: dx = [dg du] [Wg; Wu], dWg = dg^T x and dWu = du^T x.  `split`: k
+// is twice as long, for the second numbers.
 struct BackwardNeed {
   Args q[kProducts];
   int count, shape;
-  int dx, dw;  // the first of q that each is, or -1
+  int dx, dw[2];  // which of q each is, or -1
   size_t bytes;
 };
-BackwardNeed backward_need(int64_t m, int64_t f, int64_t k, bool dx, bool dw, bool ax, bool aw) {
+BackwardNeed backward_need(int64_t m, int64_t f, int64_t k, bool dx, bool dwg, bool dwu, bool split, bool ax,
+                           bool aw) {
   BackwardNeed b{};
-  const int fp = static_cast<int>((f + 63) / 64 * 64);
-  const auto add = [&](int64_t rows, int64_t inner, int across) {
+  const int fp = static_cast<int>((f + 63) / 64 * 64), mp = static_cast<int>((m + 63) / 64 * 64);
+  const auto add = [&](int64_t rows, int inner, int fold, int64_t have, int across) {
     Args &p = b.q[b.count];
     p.m = static_cast<int>(rows);
     p.n = static_cast<int>(k);
-    p.k = p.fold = p.have = static_cast<int>(inner);
+    p.k = inner;
+    p.fold = fold;
+    p.have = static_cast<int>(have);
+    p.next = 2 * fp;
     p.across = across;
     return b.count++;
   };
-  b.dx = b.dw = -1;
+  b.dx = b.dw[0] = b.dw[1] = -1;
   const bool first = 2 * fp >= m;
-  if (dx && m && first) b.dx = add(m, 2 * fp, 0);
-  if (dw && f) b.dw = add(f, m, 1), add(f, m, 1);
-  if (dx && m && !first) b.dx = add(m, 2 * fp, 0);
+  const int s = split ? 2 : 1;
+  if (dx && m && first) b.dx = add(m, 2 * s * fp, fp, f, 0);
+  for (int i = 0; i < 2; i++)
+    if ((i ? dwu : dwg) && f) b.dw[i] = add(f, split ? 2 * mp : static_cast<int>(m), mp, m, 1);
+  if (dx && m && !first) b.dx = add(m, 2 * s * fp, fp, f, 0);
   const size_t kp = up8(k);
-  b.bytes = up256(2 * m * 2 * fp) + (dw && !ax ? up256(2 * m * kp) : 0) + (dx && !aw ? 2 * up256(2 * f * kp) : 0);
+  b.bytes = up256(2 * m * s * 2 * fp) + ((dwg || dwu) && !ax ? up256(2 * m * kp) : 0) +
+            (dx && !aw ? 2 * up256(2 * f * kp) : 0);
   if (b.count) b.shape = plan<false>(b.q, b.count);
   for (int i = 0; i < b.count; i++) b.bytes += sums_bytes(b.q[i], false);
   return b;
@@ -1252,7 +1297,7 @@ BackwardNeed backward_need(int64_t m, int64_t f, int64_t k, bool dx, bool dw, bo
 template <class N>
 vs_status backward(const uint16_t *x, int64_t ldx, const uint16_t *wg, int64_t ldg,
                    const uint16_t *wu, int64_t ldu, const float2 *pre, const uint16_t *dh,
-                   int64_t ldh, int act, int m, int f, int k, uint16_t *dx, uint16_t *dw,
+                   int64_t ldh, int act, bool split, int m, int f, int k, uint16_t *dx, uint16_t *const (&dw)[2],
                    void *workspace, size_t bytes, hipStream_t s) {
   DeviceBuffer own;
   Space sp;
@@ -1260,9 +1305,9 @@ vs_status backward(const uint16_t *x, int64_t ldx, const uint16_t *wg, int64_t l
   // with one row stride
   const bool ax = direct(x, ldx, k) && ldx >= k && ldx < kMostLd,
              aw = direct(wg, ldg, k) && direct(wu, ldu, k) && ldg == ldu && ldg >= k && ldg < kMostLd;
-  BackwardNeed need = backward_need(m, f, k, dx, dw, ax, aw);
+  BackwardNeed need = backward_need(m, f, k, dx, dw[0], dw[1], split, ax, aw);
   VS_TRY(open_space(sp, own, workspace, bytes, need.bytes, s));
-  const int fp = (f + 63) / 64 * 64;
+  const int fp = (f + 63) / 64 * 64, ld = (split ? 4 : 2) * fp;
   Slopes sl{};
   sl.dh = dh;
   sl.ld = ldh;
@@ -1271,14 +1316,15 @@ vs_status backward(const uint16_t *x, int64_t ldx, const uint16_t *wg, int64_t l
   sl.m = m;
   sl.f = f;
   sl.fp = fp;
-  sl.rows = sp.take(static_cast<size_t>(m) * 2 * fp);
+  sl.split = split;
+  sl.rows = sp.take(static_cast<size_t>(m) * ld);
   if (const int64_t n = static_cast<int64_t>(m) * (fp / 4)) {
     const unsigned grid = static_cast<unsigned>(std::min<int64_t>((n + 255) / 256, 1 << 20));
     hipLaunchKernelGGL((slope_kernel<N>), dim3(grid), dim3(256), 0, s, sl);
     VS_HIP(hipGetLastError());
   }
   Copies copies(sp, k);
-  if (dw && !ax) copies.add(x, ldx, m);
+  if ((dw[0] || dw[1]) && !ax) copies.add(x, ldx, m);
   if (dx && !aw) {
     copies.add(wg, ldg, f);
     copies.add(wu, ldu, f);
@@ -1287,26 +1333,34 @@ vs_status backward(const uint16_t *x, int64_t ldx, const uint16_t *wg, int64_t l
   if (need.dx >= 0) {
     Args &p = need.q[need.dx];
     p.a = sl.rows;
-    p.lda = 2 * fp;
+    p.lda = ld;
     p.b[0] = wg;
     p.b[1] = wu;
     p.ldb[0] = ldg;
-    p.fold = fp;
-    p.have = f;
     p.c = dx;
   }
-  if (need.dw >= 0)
-    for (int i = 0; i < 2; i++) {
-      Args &p = need.q[need.dw + i];
+  for (int i = 0; i < 2; i++)
+    if (need.dw[i] >= 0) {
+      Args &p = need.q[need.dw[i]];
       p.a = sl.rows + i * fp;
-      p.lda = 2 * fp;
+      p.lda = ld;
       p.b[0] = p.b[1] = x;
       p.ldb[0] = ldx;
-      p.c = dw + static_cast<int64_t>(i) * f * k;
+      p.c = dw[i];
     }
   for (int i = 0; i < need.count; i++)
     if (const size_t sums = sums_bytes(need.q[i], false)) need.q[i].sums = sp.take_sums(sums);
-  return need.count ? product<N, false>(need.shape, need.q, need.count, s) : VS_OK;
+  if (!need.count) return VS_OK;
+  return split ? product<N, false, true>(need.shape, need.q, need.count, s)
+               : product<N, false>(need.shape, need.q, need.count, s);
+}
+
+vs_status check_gradients(int dtype, int act, bool split, int64_t m, int64_t f, int64_t k) {
+  VS_TRY(check("gated_linear_backward", dtype, act, m, f, k));
+  // twice the reduction, and rows of four numbers a feature, have to stay inside the same offsets
+  VS_REQUIRE(!split || (m < (1ll << 30) - 256 && f <= (1 << 19)),
+             "gated_linear_backward: dimension too large for split gradients (rows < 2^30, features <= 2^19)");
+  return VS_OK;
 }
 
 }  // namespace
@@ -1357,21 +1411,22 @@ vs_status vs_gated_linear(int dtype, int act, const void *x, int64_t ldx, const 
                           : glin::forward<num::F16>(p, workspace, workspace_bytes, s);
 }
 
-size_t vs_gated_linear_backward_workspace(int64_t m, int64_t f, int64_t k, int want_dx, int want_dw,
-                                          int aligned) {
-  if (glin::check("", VS_BF16, 0, m, f, k) != VS_OK) return 0;
+size_t vs_gated_linear_gradients_workspace(int64_t m, int64_t f, int64_t k, int split, int want_dx,
+                                           int want_dw_gate, int want_dw_up, int aligned) {
+  if (glin::check_gradients(VS_BF16, 0, split != 0, m, f, k) != VS_OK || k == 0) return 0;
   const bool al = aligned != 0;
-  return k ? glin::backward_need(m, f, k, want_dx != 0, want_dw != 0, al, al).bytes : 0;
+  return glin::backward_need(m, f, k, want_dx != 0, want_dw_gate != 0, want_dw_up != 0, split != 0, al, al).bytes;
 }
 
-vs_status vs_gated_linear_backward(int dtype, int act, const void *x, int64_t ldx,
-                                   const void *w_gate, int64_t ld_gate, const void *w_up,
-                                   int64_t ld_up, const float *pre, const void *dh, int64_t ld_dh,
-                                   int64_t m, int64_t f, int64_t k, void *dx, void *dw,
-                                   void *workspace, size_t workspace_bytes, vs_stream_t stream) {
+vs_status vs_gated_linear_gradients(int dtype, int act, int split, const void *x, int64_t ldx,
+                                    const void *w_gate, int64_t ld_gate, const void *w_up,
+                                    int64_t ld_up, const float *pre, const void *dh, int64_t ld_dh,
+                                    int64_t m, int64_t f, int64_t k, void *dx, void *dw_gate,
+                                    void *dw_up, void *workspace, size_t workspace_bytes,
+                                    vs_stream_t stream) {
   clear_error();
-  VS_TRY(glin::check("gated_linear_backward", dtype, act, m, f, k));
-  if (k == 0 || (!dx && !dw)) return VS_OK;
+  VS_TRY(glin::check_gradients(dtype, act, split != 0, m, f, k));
+  if (k == 0 || (!dx && !dw_gate && !dw_up)) return VS_OK;
   VS_REQUIRE((m == 0 || f == 0) || (x && w_gate && w_up && pre && dh),
              "gated_linear_backward: null pointer");
   VS_REQUIRE((m <= 1 || ((ldx >= k || ldx == 0) && (ld_dh >= f || ld_dh == 0))) &&
@@ -1379,15 +1434,31 @@ vs_status vs_gated_linear_backward(int dtype, int act, const void *x, int64_t ld
              "gated_linear_backward: leading dimension too small");
   const hipStream_t s = static_cast<hipStream_t>(stream);
   const auto u16 = [](const void *v) { return static_cast<const uint16_t *>(v); };
+  uint16_t *const dw[2] = {static_cast<uint16_t *>(dw_gate), static_cast<uint16_t *>(dw_up)};
   const auto go = [&](auto tag) {
     using N = decltype(tag);
     return glin::backward<N>(u16(x), ldx, u16(w_gate), ld_gate, u16(w_up), ld_up,
-                             reinterpret_cast<const float2 *>(pre), u16(dh), ld_dh, act,
+                             reinterpret_cast<const float2 *>(pre), u16(dh), ld_dh, act, split != 0,
                              static_cast<int>(m), static_cast<int>(f), static_cast<int>(k),
-                             static_cast<uint16_t *>(dx), static_cast<uint16_t *>(dw), workspace,
-                             workspace_bytes, s);
+                             static_cast<uint16_t *>(dx), dw, workspace, workspace_bytes, s);
   };
   return dtype == VS_BF16 ? go(num::BF16{}) : go(num::F16{});
+}
+
+size_t vs_gated_linear_backward_workspace(int64_t m, int64_t f, int64_t k, int want_dx, int want_dw,
+                                          int aligned) {
+  return vs_gated_linear_gradients_workspace(m, f, k, 0, want_dx, want_dw, want_dw, aligned);
+}
+
+vs_status vs_gated_linear_backward(int dtype, int act, const void *x, int64_t ldx,
+                                   const void *w_gate, int64_t ld_gate, const void *w_up,
+                                   int64_t ld_up, const float *pre, const void *dh, int64_t ld_dh,
+                                   int64_t m, int64_t f, int64_t k, void *dx, void *dw,
+                                   void *workspace, size_t workspace_bytes, vs_stream_t stream) {
+  uint16_t *const gate = static_cast<uint16_t *>(dw);
+  uint16_t *const up = gate && f > 0 && k > 0 ? gate + f * k : gate;
+  return vs_gated_linear_gradients(dtype, act, 0, x, ldx, w_gate, ld_gate, w_up, ld_up, pre, dh,
+                                   ld_dh, m, f, k, dx, gate, up, workspace, workspace_bytes, stream);
 }
 
 }  // extern "C"

@@ -408,6 +408,19 @@ vs_status vs_gated_linear_backward(int dtype, int act, const void *x, int64_t ld
                                    void *workspace, size_t workspace_bytes, vs_stream_t stream);
 size_t vs_gated_linear_backward_workspace(int64_t m, int64_t f, int64_t k, int want_dx,
                                           int want_dw, int aligned);
+/// The same with each weight's gradient in an array of its own ([f][k]; NULL skips it) and the choice of how
+/// the gradients of the two products reach the matrix cores: split = 0 rounds them to the operands' type
+/// (at most 2^-8 of each in bf16, 2^-11 or 2^-25 in fp16, infinite above 65504), split = 1 takes each as the sum
+/// of two numbers of that type (2^-16 of it; 2^-22 or 2^-25), for twice the multiplications (rows < 2^30 - 256,
+/// features <= 2^19).
+vs_status vs_gated_linear_gradients(int dtype, int act, int split, const void *x, int64_t ldx,
+                                    const void *w_gate, int64_t ld_gate, const void *w_up,
+                                    int64_t ld_up, const float *pre, const void *dh, int64_t ld_dh,
+                                    int64_t m, int64_t f, int64_t k, void *dx, void *dw_gate,
+                                    void *dw_up, void *workspace, size_t workspace_bytes,
+                                    vs_stream_t stream);
+size_t vs_gated_linear_gradients_workspace(int64_t m, int64_t f, int64_t k, int split, int want_dx,
+                                           int want_dw_gate, int want_dw_up, int aligned);
 
 SIMD_API_END
 

@@ -358,3 +358,112 @@ def test_block_trains_prefills_and_generates(dev):
             tok = ops.gated_recurrence_step(v[at], a[at], state)
             out = ops.matvec_int4(ops.gated_linear(tok, wg, wu), *down, 32)
             assert (out.float() - whole[at].float()).abs().max() <= 4 * 2.0 ** -8 * whole.float().abs().max()
+
+
+def _split_oracle(x, wg, wu, dh, act):
+    """The gradients in float64 and how far they may be off before they are rounded to the result's type: dg and du carry 2^-16
+    (float16: 2^-22, or half of the smallest step) where they are split, the sums have twice as many terms, the rest is as
+    in _oracle."""
+    half = x.dtype == torch.float16
+    e, tiny = (2.0 ** -22, 2.0 ** -25) if half else (2.0 ** -16, 2.0 ** -133)
+    x, wg, wu, dh = (v.detach().double().cpu() for v in (x, wg, wu, dh))
+    (m, k), f = x.shape, wg.shape[0]
+    g, u = x @ wg.t(), x @ wu.t()
+    eg, eu = k * U * (x.abs() @ wg.abs().t()), k * U * (x.abs() @ wu.abs().t())
+    a, slope = _act(act, g)
+    ea, eslope = 1.2 * eg + 8 * U * a.abs(), 1.6 * eg + 16 * U
+    dg, du = dh * u * slope, dh * a
+    edg = dh.abs() * (eu * slope.abs() + u.abs() * eslope) + 4 * U * dg.abs()
+    edu = dh.abs() * ea + 4 * U * du.abs()
+    d, ed, w = torch.cat([dg, du], 1), torch.cat([edg, edu], 1), torch.cat([wg, wu])
+    ed = ed + e * (d.abs() + ed) + tiny
+    dw, edw = d.t() @ x, ed.t() @ x.abs() + 2 * m * U * ((d.abs() + ed).t() @ x.abs())
+    return dict(dx=(d @ w, ed @ w.abs() + 4 * f * U * ((d.abs() + ed) @ w.abs())), dw_gate=(dw[:f], edw[:f]),
+                dw_up=(dw[f:], edw[f:]))
+
+
+def _rounded_once(name, got, want):
+    """What was off by `bound` before it was rounded to nearest is off by what rounding the exact value costs, and twice that."""
+    ref, bound = want
+    off = (got.detach().double().cpu() - ref).abs()
+    tol = (ref.to(got.dtype).double() - ref).abs() + 2 * bound + 1e-12 * ref.abs()
+    assert (off <= tol).all(), (name, int((off > tol).sum()), (off / tol).max().item())
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("m,k,f", [(1, 8, 3), (33, 64, 24), (64, 72, 64), (65, 40, 130), (200, 33, 63), (300, 264, 257)])
+def test_split_gradients_are_rounded_once(dev, dtype, m, k, f):
+    """With split_gradients no rounding but the result's own is left, in rows, features and steps that end inside a tile."""
+    for act in ("silu", "gelu"):
+        x, wg, wu, dh = _inputs(m, k, f, dtype, dev, seed=m + k)
+        leaves = [v.detach().requires_grad_() for v in (x, wg, wu)]
+        h = ops.gated_linear(*leaves, act, split_gradients=True)
+        want = _split_oracle(x, wg, wu, dh, act)
+        for name, got in zip(("dx", "dw_gate", "dw_up"), torch.autograd.grad(h, leaves, dh)):
+            _rounded_once(name, got, want[name])
+        with torch.no_grad():
+            assert torch.equal(ops.gated_linear(x, wg, wu, act), h)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,k,f", [(4100, 1000, 2056), (9001, 513, 65), (64, 128, 16384), (2100, 2048, 1000), (70, 4096, 700)])
+def test_split_gradients_of_large_tiles_and_parts(m, k, f):
+    """Every tile shape and sums in parts; the two halves of the reduction may lie in one part or in several."""
+    x, wg, wu, dh = _inputs(m, k, f, torch.bfloat16, "cuda", seed=13)
+    leaves = [v.detach().requires_grad_() for v in (x, wg, wu)]
+    want = _split_oracle(x, wg, wu, dh, "silu")
+    first = torch.autograd.grad(ops.gated_linear(*leaves, split_gradients=True), leaves, dh)
+    for name, got in zip(("dx", "dw_gate", "dw_up"), first):
+        _rounded_once(name, got, want[name])
+    again = torch.autograd.grad(ops.gated_linear(*leaves, split_gradients=True), leaves, dh)
+    assert all(torch.equal(a, b) for a, b in zip(first, again))
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_split_gradients_that_are_not_finite(dev):
+    """A gradient that is infinite or NaN, or rounds to infinity in float16, spreads as far as without split_gradients."""
+    x, wg, wu, dh = _inputs(70, 40, 24, torch.float16, dev, seed=14)
+    wu = wu * 64
+    for bad in (float("nan"), float("inf"), 60000.0):
+        d = dh.clone()
+        d[3, 5] = bad
+        got = []
+        for split in (False, True):
+            leaves = [v.detach().requires_grad_() for v in (x, wg, wu)]
+            got.append(torch.autograd.grad(ops.gated_linear(*leaves, split_gradients=split), leaves, d))
+        for a, b in zip(*got):
+            assert torch.equal(torch.isfinite(a), torch.isfinite(b))
+
+
+@pytest.mark.gpu
+def test_split_gradients_captured_and_dispatched():
+    args = _inputs(130, 72, 100, torch.bfloat16, "cuda", seed=15)
+
+    def train(x, wg, wu, dh):
+        leaves = [v.detach().requires_grad_() for v in (x, wg, wu)]
+        return torch.autograd.grad(ops.gated_linear(*leaves, split_gradients=True), leaves, dh)
+    cap = CapturedCall(train, *args)
+    for seed in range(3):
+        other = _inputs(130, 72, 100, torch.bfloat16, "cuda", seed=40 + seed)
+        got = [v.clone() for v in cap(*other)]
+        want = train(*other)
+        leaves = [v.detach().requires_grad_() for v in other[:3]]
+        op = torch.autograd.grad(torch.ops.veles.gated_linear(*leaves, "silu", True, True)[0], leaves, other[3])
+        for a, b, c in zip(got, want, op):
+            assert torch.equal(a, b) and torch.equal(c, b)
+        torch.cuda.synchronize()
+
+
+def test_split_gradients_native_refusals_and_workspace():
+    lib = _lib.lib()
+    p = torch.zeros(8).data_ptr()
+
+    def call(split=1, m=1, f=1, ws=None, size=0, pre=p):
+        return lib.vs_gated_linear_gradients(5, 0, split, p, 8, p, 8, p, 8, pre, p, f, m, f, 8, p, p, None, ws, size, None)
+    for kw in (dict(m=1 << 30), dict(f=(1 << 19) + 1), dict(pre=None), dict(m=-1)):
+        assert call(**kw) == 1 and b"gated_linear" in lib.vs_last_error()
+    assert call(f=9, ws=p, size=16) == 1 and b"workspace" in lib.vs_last_error()
+    size = lib.vs_gated_linear_gradients_workspace
+    assert size(4096, 2048, 2048, 1, 1, 1, 1, 1) == 2 * size(4096, 2048, 2048, 0, 1, 1, 1, 1) == 2 * 4096 * 8192
+    assert size(1 << 30, 64, 64, 1, 1, 1, 1, 1) == 0 and size(64, 1 << 20, 64, 1, 1, 1, 1, 1) == 0

@@ -116,6 +116,9 @@ _SIGNATURES = {
     "vs_gated_linear_backward": (_i, [_i, _i, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _i64,
                                       _vp, _vp, _vp, _sz, _vp]),
     "vs_gated_linear_backward_workspace": (_sz, [_i64, _i64, _i64, _i, _i, _i]),
+    "vs_gated_linear_gradients": (_i, [_i, _i, _i, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _i64,
+                                       _vp, _vp, _vp, _vp, _sz, _vp]),
+    "vs_gated_linear_gradients_workspace": (_sz, [_i64, _i64, _i64, _i, _i, _i, _i, _i]),
     # multi-GPU layer (include/simd/dist.h)
     "vs_dist_create": (_i, [_i, _vp, _i, ctypes.POINTER(_vp)]),
     "vs_dist_destroy": (_i, [_vp]),

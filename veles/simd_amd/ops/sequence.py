@@ -489,7 +489,7 @@ def _slope_cpu(kind, g):
     return (g > 0).to(g.dtype) if kind == "relu" else s * (1.0 - s)
 
 
-def _gated_impl(x, w_gate, w_up, activation, save):
+def _gated_impl(x, w_gate, w_up, activation, save, split=False):
     name = "veles::gated_linear"
     # few rows, as a generating model has them, in one expression; _check_gated names what is wrong otherwise
     dev, dtype = x.get_device(), x.dtype
@@ -529,7 +529,7 @@ def _aligned(*tensors) -> bool:
     return all(t.shape[-1] % 8 == 0 and t.stride(0) % 8 == 0 and t.data_ptr() % 16 == 0 for t in tensors)
 
 
-def _gated_backward_impl(x, w_gate, w_up, pre, dh, activation, want_dx, want_dw):
+def _gated_backward_impl(x, w_gate, w_up, pre, dh, activation, want_dx, want_dw, split=False):
     name = "veles::gated_linear_backward"
     _check_gated(name, x, w_gate, w_up, activation)
     f, k = w_gate.shape
@@ -550,16 +550,16 @@ def _gated_backward_impl(x, w_gate, w_up, pre, dh, activation, want_dx, want_dw)
     dx = torch.empty(x.shape if want_dx else (0,), dtype=x.dtype, device=x.device)
     dw = torch.empty((2 * f, k) if want_dw else (0,), dtype=x.dtype, device=x.device)
     aligned = (w_gate.stride(0) == w_up.stride(0) >= k <= rows.stride(0)) and _aligned(rows, w_gate, w_up)
-    size = int(_lib.lib().vs_gated_linear_backward_workspace(m, f, k, want_dx, want_dw, aligned))
+    size = int(_lib.lib().vs_gated_linear_gradients_workspace(m, f, k, split, want_dx, want_dw, want_dw, aligned))
     ws = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
-    launch(x, "vs_gated_linear_backward", DTYPES[x.dtype], ACTIVATIONS[activation], rows.data_ptr(),
+    launch(x, "vs_gated_linear_gradients", DTYPES[x.dtype], ACTIVATIONS[activation], split, rows.data_ptr(),
            rows.stride(0), w_gate.data_ptr(), w_gate.stride(0), w_up.data_ptr(), w_up.stride(0), pre.data_ptr(),
            dhr.data_ptr(), dhr.stride(0), m, f, k, dx.data_ptr() if want_dx else None,
-           dw.data_ptr() if want_dw else None, _opt(ws), size)
+           dw.data_ptr() if want_dw else None, dw[f:].data_ptr() if want_dw else None, _opt(ws), size)
     return dx, dw
 
 
-def _gated_fake(x, w_gate, w_up, activation, save):
+def _gated_fake(x, w_gate, w_up, activation, save, split=False):
     _check_gated("veles::gated_linear", x, w_gate, w_up, activation)
     m, f = 1, w_gate.shape[0]
     for n in x.shape[:-1]:
@@ -568,17 +568,17 @@ def _gated_fake(x, w_gate, w_up, activation, save):
 
 
 def _gated_setup(ctx, inputs, output):
-    x, w_gate, w_up, activation, save = inputs
+    x, w_gate, w_up, activation, save, split = inputs
     if not save:
         raise RuntimeError("veles::gated_linear: gradients need the pre-activations (save=True)")
     ctx.set_materialize_grads(False)
     ctx.mark_non_differentiable(output[1])
     ctx.save_for_backward(x, w_gate, w_up, output[1])
-    ctx.activation = activation
+    ctx.activation, ctx.split = activation, split
 
 
 def _gated_grad(ctx, dh, _):
-    return *_gated_grads(ctx, torch.ops.veles.gated_linear_backward, dh), None, None
+    return *_gated_grads(ctx, torch.ops.veles.gated_linear_backward, dh), None, None, None
 
 
 def _gated_grads(ctx, backward, dh):
@@ -586,7 +586,7 @@ def _gated_grads(ctx, backward, dh):
         return None, None, None
     x, w_gate, w_up, pre = ctx.saved_tensors
     need = ctx.needs_input_grad
-    dx, dw = backward(x, w_gate, w_up, pre, dh, ctx.activation, need[0], need[1] or need[2])
+    dx, dw = backward(x, w_gate, w_up, pre, dh, ctx.activation, need[0], need[1] or need[2], ctx.split)
     f = w_gate.shape[0]
     return dx if need[0] else None, dw[:f] if need[1] else None, dw[f:] if need[2] else None
 
@@ -595,50 +595,54 @@ class _Gated(torch.autograd.Function):
     """The op's autograd without the dispatcher."""
 
     @staticmethod
-    def forward(ctx, x, w_gate, w_up, activation):
+    def forward(ctx, x, w_gate, w_up, activation, split):
         h, pre = _gated_impl(x, w_gate, w_up, activation, True)
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(x, w_gate, w_up, pre)
-        ctx.activation = activation
+        ctx.activation, ctx.split = activation, split
         return h
 
     @staticmethod
     def backward(ctx, dh):
         # a graph of the gradients asks for second derivatives, which the op refuses by name
         op = torch.ops.veles.gated_linear_backward if torch.is_grad_enabled() else _gated_backward_impl
-        return *_gated_grads(ctx, op, dh), None
+        return *_gated_grads(ctx, op, dh), None, None
 
 
 torch.library.define("veles::gated_linear",
-                     "(Tensor x, Tensor w_gate, Tensor w_up, str activation, bool save) -> (Tensor, Tensor)")
+                     "(Tensor x, Tensor w_gate, Tensor w_up, str activation, bool save, bool split=False) -> "
+                     "(Tensor, Tensor)")
 torch.library.impl("veles::gated_linear", "default", _with_empty(_gated_impl))
 torch.library.register_fake("veles::gated_linear", _gated_fake)
 torch.library.register_autograd("veles::gated_linear", _gated_grad, setup_context=_gated_setup)
 torch.library.define("veles::gated_linear_backward",
                      "(Tensor x, Tensor w_gate, Tensor w_up, Tensor pre, Tensor dh, str activation, bool want_dx, "
-                     "bool want_dw) -> (Tensor, Tensor)")
+                     "bool want_dw, bool split=False) -> (Tensor, Tensor)")
 torch.library.impl("veles::gated_linear_backward", "default", _gated_backward_impl)
 torch.library.register_fake(
     "veles::gated_linear_backward",
-    lambda x, w_gate, w_up, pre, dh, activation, want_dx, want_dw: (
+    lambda x, w_gate, w_up, pre, dh, activation, want_dx, want_dw, split=False: (
         x.new_empty(x.shape if want_dx else (0,)),
         x.new_empty((2 * w_gate.shape[0], w_gate.shape[1]) if want_dw else (0,))))
 _no_second_derivative("veles::gated_linear_backward")
 
 
 def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor,
-                 activation: str = "silu") -> torch.Tensor:
+                 activation: str = "silu", split_gradients: bool = False) -> torch.Tensor:
     """act(x @ w_gate.T) * (x @ w_up.T): both products, the activation and the product of the two in one
     kernel, the first half of a gated feed-forward block.
 
     x: [..., k], weights [features, k], all float16 or all bfloat16; activation: silu, gelu (by the error
     function), relu or sigmoid.  Sums, activation and product are float32 and rounded once.  Differentiable
     in x and the weights; the float32 pairs (x @ w_gate.T, x @ w_up.T), 8 bytes per output, are kept for the
-    backward pass, and the gradients of the two products are rounded to x's type before they are
-    multiplied.  Up to 64 rows (generation) stream the weights once at memory speed."""
+    backward pass.  There the gradients of the two products are rounded to x's type before they are multiplied,
+    which adds about 0.4 of the result's own rounding to the error; in float16 they are lost below 6e-8 and
+    infinite above 65504, so the loss has to be scaled.  split_gradients takes each as the sum of two numbers of x's
+    type (to 2^-16 of it in bfloat16, to 2^-22 or 3e-8 in float16), so the result's own rounding is all that counts,
+    for twice the multiplications of the backward pass (on a CPU they are not rounded at all).  Up to 64 rows (generation) stream the weights once at memory speed."""
     save = records(x, w_gate, w_up)
     if plain_tensors(x, w_gate, w_up):
         if save:
-            return _Gated.apply(x, w_gate, w_up, activation)
+            return _Gated.apply(x, w_gate, w_up, activation, split_gradients)
         return _gated_impl(x, w_gate, w_up, activation, False)[0]
-    return torch.ops.veles.gated_linear(x, w_gate, w_up, activation, save)[0]
+    return torch.ops.veles.gated_linear(x, w_gate, w_up, activation, save, split_gradients)[0]
