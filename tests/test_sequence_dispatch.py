@@ -55,3 +55,23 @@ def test_traced_training_calls_keep_the_operator(dev):
         a, b = (torch.autograd.grad(_flat(f(*leaves))[0].float().sum(), leaves) for f in (traced, fn))
         for u, v in zip(a, b):
             assert torch.equal(u, v)
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_meta_tensors(name):
+    """Tensors without data give results of the right shapes and types, with gradients and without."""
+    _, fn, args = next(c for c in _calls("cpu") if c[0] == name)
+    want = _flat(fn(*args))
+    if name == "matvec_int4":
+        q, s, z = (v.to("meta") for v in ops.quantize_int4(torch.randn(24, 64), 32))
+        fn = lambda x: ops.matvec_int4(x, q, s, z, 32)   # noqa: E731
+    metas = [a.to("meta") for a in args]
+    for leaves in (metas, [m.clone().requires_grad_() for m in metas]):
+        if leaves is not metas and name in ("gated_recurrence_step", "matvec_int4"):
+            continue
+        got = _flat(fn(*leaves))
+        for a, b in zip(got, want):
+            assert a.is_meta and a.shape == b.shape and a.dtype == b.dtype
+    if name in ("gated_recurrence", "gated_linear"):
+        for grad, leaf in zip(torch.autograd.grad(got[0].sum(), leaves), leaves):
+            assert grad.is_meta and grad.shape == leaf.shape and grad.dtype == leaf.dtype

@@ -45,14 +45,14 @@ _PLAIN = (torch.Tensor, torch.nn.Parameter)
 
 
 def plain_tensors(*tensors) -> bool:
-    """True when a call needs none of the dispatcher's services: ordinary tensors, nothing tracing.
+    """True when a call needs none of the dispatcher's services: ordinary tensors with data, nothing tracing.
     The implementation (or its autograd Function) is then called directly, which takes several
     microseconds of host time off a call, and about a hundred off a training pass."""
     if torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack() \
             or torch._C._get_tracing_state() is not None or torch._C._functorch.peek_interpreter_stack() is not None:
         return False
     for t in tensors:
-        if t is not None and type(t) not in _PLAIN:
+        if t is not None and (type(t) not in _PLAIN or t.is_meta):
             return False
     return True
 
