@@ -1,9 +1,15 @@
 """The operators of sequence models where something stands between the caller and the kernels: tracers, compilers, tensors
 without data, forward-mode derivatives."""
 import pytest
+import sympy
 import torch
+import torch._dynamo.testing
+from torch._dynamo.source import ConstantSource
+from torch._subclasses.fake_tensor import FakeTensorMode
+from torch.fx.experimental.symbolic_shapes import DimDynamic, ShapeEnv
 
-from veles.simd_amd import ops
+from veles.simd_amd import _lib, ops
+from veles.simd_amd.ops.sequence import _tiles
 
 DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
 
@@ -75,3 +81,65 @@ def test_meta_tensors(name):
     if name in ("gated_recurrence", "gated_linear"):
         for grad, leaf in zip(torch.autograd.grad(got[0].sum(), leaves), leaves):
             assert grad.is_meta and grad.shape == leaf.shape and grad.dtype == leaf.dtype
+
+
+def test_tile_count_is_the_librarys():
+    lib = _lib.lib()
+    for t in [*range(0, 700), 4095, 4096, 4097, 65536, (1 << 29) - 1, 1 << 29]:
+        assert _tiles(t) == lib.vs_gated_recurrence_tiles(t)
+
+
+def _symbolic_cases(length):
+    """Operators on GPU tensors of one symbolic dimension, as a compiler sees them; no GPU is needed."""
+    def e(*s, dtype=torch.bfloat16):
+        return torch.empty(*s, dtype=dtype, device="cuda")
+    op = torch.ops.veles
+    x = e(2, length, 6)
+    yield "recurrence", op.gated_recurrence(x, x, None, None, True)
+    yield "recurrence backward", op.gated_recurrence_backward(x, x, None, e(2, (length + 127) // 128, 6, dtype=torch.float32),
+                                                              x, None)
+    yield "linear", op.gated_linear(e(length, 40), e(16, 40), e(16, 40), "silu", True)
+    yield "linear, batched", op.gated_linear(e(2, length, 40), e(16, 40), e(16, 40), "silu", False)
+    yield "linear backward", op.gated_linear_backward(e(length, 40), e(16, 40), e(16, 40),
+                                                      e(length, 16, 2, dtype=torch.float32), e(length, 16), "silu", True, True)
+    yield "4 bits", (op.matvec_int4(e(length, 64), e(24, 32, dtype=torch.uint8), e(24, 2), None, 32),)
+
+
+@pytest.mark.parametrize("known", [True, False])
+def test_symbolic_lengths_stay_symbolic(known):
+    """A compiler that traces a call once for all lengths: nothing fixes the length, or asks for it where it is not known."""
+    env = ShapeEnv()
+    with FakeTensorMode(shape_env=env):
+        if known:
+            symbol = env.create_symbol(70, ConstantSource("length"), dynamic_dim=DimDynamic.DYNAMIC)
+            length = env.create_symintnode(symbol, hint=70)
+        else:
+            length = env.create_unbacked_symint()
+            torch._check(length > 1)
+        for name, out in _symbolic_cases(length):
+            assert any(not isinstance(n, int) for o in out for n in o.shape), name
+    assert not any(isinstance(g.expr, sympy.Eq) for g in env.guards), env.guards
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("train", [False, True])
+def test_other_lengths_do_not_compile_anew(train):
+    """With gradients there are two compilations: the compiler treats dimensions of one element, here a single tile of saved
+    states (up to 128 steps), apart from larger ones."""
+    def block(v, a, wg, wu, q, s):
+        return ops.matvec_int4(ops.gated_linear(ops.gated_recurrence(v, a)[0], wg, wu), q, s, None, 32) if not train else \
+            ops.gated_linear(ops.gated_recurrence(v, a)[0], wg, wu)
+    g = torch.Generator().manual_seed(0)
+    wg, wu = (torch.randn(96, 64, generator=g).bfloat16().cuda().requires_grad_(train) for _ in range(2))
+    q, s, _ = ops.quantize_int4(torch.randn(24, 96, generator=g).cuda(), 32, True)
+    torch._dynamo.reset()
+    counter = torch._dynamo.testing.CompileCounterWithBackend("aot_eager")
+    fn = torch.compile(block, backend=counter, dynamic=True)
+    for t in (70, 33, 130, 500, 257):
+        v, a = (torch.randn(2, t, 64, generator=g).bfloat16().cuda().requires_grad_(train) for _ in range(2))
+        got, want = (f(v, a, wg, wu, q, s) for f in (fn, block))
+        assert torch.equal(got, want)
+        if train:
+            for x, y in zip(*(torch.autograd.grad(o.float().sum(), (v, a, wg, wu)) for o in (got, want))):
+                assert torch.equal(x, y)
+    assert counter.frame_count == (2 if train else 1)
