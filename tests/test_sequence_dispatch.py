@@ -143,3 +143,26 @@ def test_other_lengths_do_not_compile_anew(train):
             for x, y in zip(*(torch.autograd.grad(o.float().sum(), (v, a, wg, wu)) for o in (got, want))):
                 assert torch.equal(x, y)
     assert counter.frame_count == (2 if train else 1)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("name", NAMES)
+def test_forward_mode_is_right_or_refused(dev, name):
+    """A tangent is never dropped: the CPU definitions carry it, the kernels and torch.func refuse it."""
+    _, fn, args = next(c for c in _calls(dev) if c[0] == name)
+    tangent = torch.ones_like(args[0])
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(args[0], tangent)
+        if dev == "cpu":
+            got = torch.autograd.forward_ad.unpack_dual(_flat(fn(dual, *args[1:]))[0]).tangent
+            # a hundredth of a step each way: the second difference and the results' roundings are below 5 % of the largest
+            up, down = (_flat(fn(args[0] + s * 0.01 * tangent, *args[1:]))[0].double() for s in (1, -1))
+            if args[0].dtype == torch.float32:
+                assert ((up - down) / 0.02 - got).abs().max() <= 0.05 * got.abs().max()
+            assert got is not None and got.abs().max() > 0
+        else:
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                fn(dual, *args[1:])
+        fn(*args)    # no tangent among the inputs
+    with pytest.raises(NotImplementedError, match="forward-mode"):
+        torch.func.jvp(lambda v: fn(v, *args[1:]), (args[0],), (tangent,))

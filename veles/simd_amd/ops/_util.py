@@ -5,6 +5,7 @@ import ctypes
 import contextlib
 
 import torch
+from torch.autograd import forward_ad
 
 from .. import _lib
 
@@ -48,13 +49,26 @@ def plain_tensors(*tensors) -> bool:
     """True when a call needs none of the dispatcher's services: ordinary tensors with data, nothing tracing.
     The implementation (or its autograd Function) is then called directly, which takes several
     microseconds of host time off a call, and about a hundred off a training pass."""
-    if torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack() \
-            or torch._C._get_tracing_state() is not None or torch._C._functorch.peek_interpreter_stack() is not None:
+    if torch.compiler.is_compiling():
         return False
+    plain = not torch._C._len_torch_dispatch_stack() and torch._C._get_tracing_state() is None \
+        and torch._C._functorch.peek_interpreter_stack() is None
+    if plain:
+        for t in tensors:
+            if t is not None and (type(t) not in _PLAIN or t.is_meta):
+                plain = False
+                break
+    if forward_ad._current_level >= 0:
+        _refuse_tangents(plain, tensors)
+    return plain
+
+
+def _refuse_tangents(plain, tensors) -> None:
+    """Raise for tensors with a forward-mode tangent that a kernel or the dispatcher would drop (only the CPU
+    definitions, called directly, carry it)."""
     for t in tensors:
-        if t is not None and (type(t) not in _PLAIN or t.is_meta):
-            return False
-    return True
+        if t is not None and (t.is_cuda or not plain) and forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError("this operator has no forward-mode derivative")
 
 
 def records(*tensors) -> bool:
