@@ -166,3 +166,22 @@ def test_forward_mode_is_right_or_refused(dev, name):
         fn(*args)    # no tangent among the inputs
     with pytest.raises(NotImplementedError, match="forward-mode"):
         torch.func.jvp(lambda v: fn(v, *args[1:]), (args[0],), (tangent,))
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_default_device_does_not_matter(name):
+    """CPU tensors are computed on the CPU whatever device new tensors would get."""
+    _, fn, args = next(c for c in _calls("cpu") if c[0] == name)
+    want = _flat(fn(*args))
+    with torch.device("meta"):
+        got = _flat(fn(*args))
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+    if name in ("gated_recurrence", "gated_linear"):
+        leaves = [a.requires_grad_() for a in args]
+        up = torch.ones_like(want[0])
+        want = torch.autograd.grad(_flat(fn(*leaves))[0], leaves, up)
+        with torch.device("meta"):
+            got = torch.autograd.grad(_flat(fn(*leaves))[0], leaves, up)
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)

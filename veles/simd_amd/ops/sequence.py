@@ -67,21 +67,21 @@ def _recurrence_workspace(x):
 
 
 def _valid_steps(x, lengths):
-    n = torch.full((x.shape[0],), x.shape[1]) if lengths is None else lengths.clamp(0, x.shape[1])
-    return torch.arange(x.shape[1])[:, None] < n[None, :]      # [time, batch]
+    n = torch.full((x.shape[0],), x.shape[1], device=x.device) if lengths is None else lengths.clamp(0, x.shape[1])
+    return torch.arange(x.shape[1], device=x.device)[:, None] < n[None, :]      # [time, batch]
 
 
 def _recurrence_cpu(x, gate, state, lengths, save):
     b, t, d = x.shape
     on = _valid_steps(x, lengths)
-    h = torch.zeros(b, d, dtype=torch.float64) if state is None else state.double()
+    h = x.new_zeros(b, d, dtype=torch.float64) if state is None else state.double()
     xd, i = x.double(), torch.sigmoid(-gate.double())
-    y = torch.zeros(b, t, d, dtype=torch.float64)
+    y = x.new_zeros(b, t, d, dtype=torch.float64)
     for s in range(t):
         h = torch.where(on[s][:, None], h + i[:, s] * (xd[:, s] - h), h)
         y[:, s] = torch.where(on[s][:, None], h, 0.0)
     # the CPU backward starts from the initial state: one tile
-    starts = (torch.zeros(b, d) if state is None else state)[:, None].clone() if save else None
+    starts = (x.new_zeros(b, d, dtype=torch.float32) if state is None else state)[:, None].clone() if save else None
     return y.to(x.dtype), h.float(), starts
 
 
@@ -109,12 +109,12 @@ def _recurrence_backward_cpu(x, gate, lengths, starts, dy, dfinal):
     on = _valid_steps(x, lengths)
     xd, i = x.double(), torch.sigmoid(-gate.double())
     h = starts[:, 0].double()
-    before = torch.zeros(b, t, d, dtype=torch.float64)
+    before = x.new_zeros(b, t, d, dtype=torch.float64)
     for s in range(t):
         before[:, s] = h
         h = torch.where(on[s][:, None], h + i[:, s] * (xd[:, s] - h), h)
-    m = torch.zeros(b, d, dtype=torch.float64) if dfinal is None else dfinal.double()
-    dx, dg = torch.zeros(b, t, d, dtype=torch.float64), torch.zeros(b, t, d, dtype=torch.float64)
+    m = x.new_zeros(b, d, dtype=torch.float64) if dfinal is None else dfinal.double()
+    dx, dg = (x.new_zeros(b, t, d, dtype=torch.float64) for _ in range(2))
     for s in range(t - 1, -1, -1):
         k = on[s][:, None]
         lam = m if dy is None else m + dy[:, s].double()
@@ -359,7 +359,7 @@ def _matvec_impl(x, qweight, scales, zeros, group_size):
     n, k = qweight.shape[0], x.shape[-1]
     if not x.is_cuda:
         q = torch.stack([qweight & 15, qweight >> 4], -1).flatten(1)[:, :k].double()
-        at = torch.arange(k) // group_size
+        at = torch.arange(k, device=x.device) // group_size
         z = 8.0 if zeros is None else zeros.double()[:, at]
         return (x.double() @ ((q - z) * scales.double()[:, at]).t()).to(x.dtype)
     rows = _near_rows(_as_rows(x), True)
