@@ -486,3 +486,31 @@ def test_compiled_call_traces_the_op():
     out = torch.compile(lambda a, b, c: ops.gated_recurrence(a, b, c), backend="aot_eager")(x, gate, h0)
     ref = ops.gated_recurrence(x, gate, h0)
     assert torch.equal(out[0], ref[0]) and torch.equal(out[1], ref[1])
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_step_on_inputs_that_share_the_states_memory(dev):
+    """x or the gate may be the state itself, a row of it for all sequences, or a stretch that begins elsewhere in it."""
+    g = torch.Generator().manual_seed(15)
+    buf = torch.randn(40 * 64 + 70, generator=g).to(dev)
+    other = torch.randn(40, 64, generator=g).to(dev)
+
+    def views(buf):
+        state = buf[:40 * 64].view(40, 64)
+        yield state, state
+        yield state[3:4].expand(40, 64), state
+        yield buf[65:65 + 40 * 64].view(40, 64), state
+        yield buf.as_strided((40, 64), (32, 1), 5), state
+        yield buf[:40 * 64 // 2].view(torch.bfloat16).view(40, 64), state
+    for i in range(5):
+        for swap in (False, True):
+            mine, ref = buf.clone(), buf.clone()
+            (x, state), (rx, rs) = list(views(mine))[i], list(views(ref))[i]
+            rx = rx.clone()
+            a, b = other.to(x.dtype), other.to(x.dtype)
+            y = ops.gated_recurrence_step(*((a, x) if swap else (x, a)), state)
+            want = ops.gated_recurrence_step(*((b, rx) if swap else (rx, b)), rs)
+            nan = torch.isnan(want)
+            assert torch.equal(torch.isnan(y), nan) and torch.equal(y[~nan], want[~nan])
+            ok = ~torch.isnan(rs)
+            assert torch.equal(state[ok], rs[ok]) and torch.equal(mine[40 * 64:], ref[40 * 64:])

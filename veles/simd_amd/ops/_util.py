@@ -43,21 +43,22 @@ def launch(t: torch.Tensor, name: str, *args) -> None:
 
 
 _PLAIN = (torch.Tensor, torch.nn.Parameter)
+_is_compiling = torch.compiler.is_compiling
+_dispatch_modes = torch._C._len_torch_dispatch_stack
+_tracer = torch._C._get_tracing_state
+_functorch_level = torch._C._functorch.peek_interpreter_stack
 
 
 def plain_tensors(*tensors) -> bool:
     """True when a call needs none of the dispatcher's services: ordinary tensors with data, nothing tracing.
     The implementation (or its autograd Function) is then called directly, which takes several
     microseconds of host time off a call, and about a hundred off a training pass."""
-    if torch.compiler.is_compiling():
+    if _is_compiling():
         return False
-    plain = not torch._C._len_torch_dispatch_stack() and torch._C._get_tracing_state() is None \
-        and torch._C._functorch.peek_interpreter_stack() is None
-    if plain:
-        for t in tensors:
-            if t is not None and (type(t) not in _PLAIN or t.is_meta):
-                plain = False
-                break
+    plain = not _dispatch_modes() and _tracer() is None and _functorch_level() is None and not tensors[0].is_meta
+    for t in tensors:
+        if t is not None and type(t) not in _PLAIN:
+            plain = False
     if forward_ad._current_level >= 0:
         _refuse_tangents(plain, tensors)
     return plain

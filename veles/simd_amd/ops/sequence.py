@@ -269,6 +269,14 @@ def _check_step(x, gate, state):
         raise ValueError(f"{name}: the state is updated in place and has to be contiguous")
 
 
+def _overlaps(p, ld, t, state):
+    """Whether rows t, at address p, lie in the memory of the state of their shape in another place than the state's
+    own values, so that a step would read what it writes elsewhere."""
+    b, d = t.shape
+    return p < state + 4 * b * d and p + ((b - 1) * ld + d) * t.itemsize > state \
+        and not (p == state and ld == d and t.itemsize == 4)
+
+
 def _step_impl(x, gate, state):
     # the usual case in one expression; _check_step names what is wrong otherwise
     if not (x.dim() == 2 and x.shape == gate.shape == state.shape and x.dtype is gate.dtype
@@ -284,8 +292,13 @@ def _step_impl(x, gate, state):
     else:
         x, gate = _rows_last(x), _rows_last(gate)
         y, ldx, ldg = _new(x, b, d), x.stride(0), gate.stride(0)
-    launch(x, "vs_gated_recurrence_step", DTYPES[x.dtype], x.data_ptr(), ldx, gate.data_ptr(), ldg,
-           state.data_ptr(), b, d, y.data_ptr())
+    px, pg, ps = x.data_ptr(), gate.data_ptr(), state.data_ptr()
+    size = 4 * b * d    # rows one behind the other and this far from the state cannot reach it
+    if (-size < px - ps < size or -size < pg - ps < size or ldx != d or ldg != d) \
+            and (_overlaps(px, ldx, x, ps) or _overlaps(pg, ldg, gate, ps)):
+        x, gate = x.clone(), gate.clone()   # (kept until the launch)
+        px, ldx, pg, ldg = x.data_ptr(), x.stride(0), gate.data_ptr(), gate.stride(0)
+    launch(x, "vs_gated_recurrence_step", DTYPES[x.dtype], px, ldx, pg, ldg, ps, b, d, y.data_ptr())
     return y
 
 
