@@ -2,14 +2,18 @@
 //
 //   i_t = 1 / (1 + exp(g_t)),   h_t = h_{t-1} + i_t (x_t - h_{t-1}),   y_t = h_t
 //
-// for every channel of [batch][time][channel] arrays.  i_t is the share of the new value and is
-// computed from the gate directly (1 - sigmoid(g) would lose its digits where the memory is
-// long), and the update in this form never multiplies the state by a rounded 1 - i_t.
-//
-// Backward, with m_t the gradient that step t receives from step t + 1 on:
+// for every channel of [batch][time][channel] arrays.  Backward, with m_t the gradient that step t
+// receives from step t + 1 on:
 //
 //   l_t = dy_t + m_t,  dx_t = i_t l_t,  dg_t = i_t (1 - i_t) l_t (h_{t-1} - x_t),
-//   m_{t-1} = l_t - i_t l_t
+//   m_{t-1} = (1 - i_t) l_t
+//
+// A step keeps the smaller of i and 1 - i, computed from the gate directly, and goes from the side of the
+// larger: h + i (x - h) where the state is kept, i x + (1 - i) h where it is replaced.  So a small share is
+// never the rest of a subtraction, a long memory is not multiplied by a rounded 1 - i, and a value that
+// replaces a much larger state keeps its digits.  (Against h + i (x - h) alone: 1 x 65536 x 1024 fp32 150 us
+// instead of 149, training pass 4 x 4096 x 4096 bf16 232 instead of 222, 16 x 1000 x 1536 fp16 35 instead
+// of 31.  With x + (1 - i) (h - x) it would be 228 and 33, but an infinite x would give inf - inf.)
 //
 // Every step is an affine map s -> a s + b of the state (forward) or of m (backward), so a run
 // of steps is one map too, and runs compose: (a2, b2) o (a1, b1) = (a2 a1, a2 b1 + b2).
@@ -74,9 +78,25 @@ __device__ __forceinline__ int64_t steps_of(const Args &p, int64_t b) {
   return n < 0 ? 0 : n < p.t ? n : p.t;
 }
 
+// The smaller of a step's two shares, at most 1/2, with the gate's sign: that of the new value (i) where
+// the gate is positive and the state is kept, that of the state (1 - i) where it is negative.
 __device__ __forceinline__ float share(float g) {
-  return __builtin_amdgcn_rcpf(1.f + __expf(g));
+  const float e = __expf(-fabsf(g));
+  return copysignf(e * __builtin_amdgcn_rcpf(1.f + e), g);
 }
+// q, to be used anew: the compiler would otherwise keep what it computed from the shares of all steps from
+// one pass to the next, in 26 registers that cost a workgroup of three a CU.
+__device__ __forceinline__ float anew(float q) {
+  asm volatile("" : "+v"(q));
+  return q;
+}
+__device__ __forceinline__ bool keeps(float q) { return __float_as_int(q) >= 0; }
+__device__ __forceinline__ float advance(float q, float x, float h) {
+  const float s = fabsf(q);
+  return fmaf(s, keeps(q) ? x - h : h, keeps(q) ? h : (1.f - s) * x);
+}
+// (1 - i) v
+__device__ __forceinline__ float kept(float q, float v) { return fmaf(-q, v, keeps(q) ? v : 0.f); }
 
 template <class N, int V, int W, int L>
 struct Shape {
@@ -126,7 +146,7 @@ struct Shape {
     steps(on, [&](int s, bool use) {
 #pragma unroll
       for (int v = 0; v < V; v++) {
-        const float en = fmaf(i[s][v], x[s][v] - e[v], e[v]), an = fmaf(-i[s][v], a[v], a[v]);
+        const float q = anew(i[s][v]), en = advance(q, x[s][v], e[v]), an = kept(q, a[v]);
         e[v] = use ? en : e[v];
         a[v] = use ? an : a[v];
       }
@@ -151,7 +171,7 @@ struct Shape {
       P y;
 #pragma unroll
       for (int v = 0; v < V; v++) {
-        h[v] = fmaf(i[s][v], x[s][v] - h[v], h[v]);
+        h[v] = advance(anew(i[s][v]), x[s][v], h[v]);
         y.set(v, h[v]);
       }
       if (in && (use || t + s < p.t)) store(p.y, b * p.t + t + s, p.d, c, use ? y : zero());
@@ -165,7 +185,7 @@ struct Shape {
     steps<true>(on, [&](int s, bool use) {
 #pragma unroll
       for (int v = 0; v < V; v++) {
-        const float l = q[v] + dy[s][v], qn = fmaf(-i[s][v], l, l);
+        const float l = q[v] + dy[s][v], qn = kept(i[s][v], l);
         q[v] = use ? qn : q[v];
       }
     });
@@ -182,17 +202,16 @@ struct Shape {
 #pragma unroll
       for (int v = 0; v < V; v++) {
         before[s][v] = h[v] - x[s][v];
-        h[v] = fmaf(-i[s][v], before[s][v], h[v]);
+        h[v] = advance(i[s][v], x[s][v], h[v]);
       }
     steps<true>(on, [&](int s, bool use) {
       P ox, og;
 #pragma unroll
       for (int v = 0; v < V; v++) {
-        const float l = m[v] + dy[s][v];
-        const float il = i[s][v] * l;
-        m[v] = use ? l - il : m[v];
-        ox.set(v, il);
-        og.set(v, (1.f - i[s][v]) * il * before[s][v]);
+        const float l = m[v] + dy[s][v], q = i[s][v], small = fabsf(q) * l, large = fmaf(-fabsf(q), l, l);
+        ox.set(v, keeps(q) ? small : large);
+        og.set(v, fabsf(q) * large * before[s][v]);
+        m[v] = use ? (keeps(q) ? large : small) : m[v];
       }
       if (in && (use || t + s < p.t)) {
         store(p.dx, b * p.t + t + s, p.d, c, use ? ox : zero());
@@ -484,7 +503,7 @@ __global__ __launch_bounds__(256) void step_kernel(const typename N::store *__re
   for (int64_t at = blockIdx.x * 256ll + threadIdx.x; at < n; at += gridDim.x * 256ll) {
     const int64_t b = at / d, c = at - b * d;
     const float h0 = state[at];
-    const float h = fmaf(share(N::load(g[b * gb + c])), N::load(x[b * xb + c]) - h0, h0);
+    const float h = advance(share(N::load(g[b * gb + c])), N::load(x[b * xb + c]), h0);
     state[at] = h;
     y[at] = N::save(h);
   }

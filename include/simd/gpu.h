@@ -340,7 +340,7 @@ vs_status vs_detect_peaks_batched(const float *x, size_t n, int64_t x_stride, si
 /* --------------------------------------------------- sequence operators */
 /// Gated linear recurrence over [batch][t][d] arrays (dtype VS_F32, VS_F16 or
 /// VS_BF16; channels contiguous, the other strides in elements and free):
-///   i = 1 / (1 + exp(gate)), h_t = h_{t-1} + i_t (x_t - h_{t-1}), y_t = h_t.
+///   i = 1 / (1 + exp(gate)), h_t = (1 - i_t) h_{t-1} + i_t x_t, y_t = h_t.
 /// state: h_0, fp32 [batch][d] (NULL: zeros).  lengths: int32 (lengths64 = 0)
 /// or int64 [batch] on the device (NULL: t for all), clamped to 0..t; steps
 /// from lengths[b] on are padding: they are not read, y is 0 there and the

@@ -514,3 +514,81 @@ def test_step_on_inputs_that_share_the_states_memory(dev):
             assert torch.equal(torch.isnan(y), nan) and torch.equal(y[~nan], want[~nan])
             ok = ~torch.isnan(rs)
             assert torch.equal(state[ok], rs[ok]) and torch.equal(mine[40 * 64:], ref[40 * 64:])
+
+
+def _relative_oracle(x, gate, h0, dy, dfinal):
+    """As _oracle, with bounds that are relative to the shares, however small.  A step computes the smaller share s of i and
+    1 - i to r relatively and rounds s (x - h) by 2 u and its result by u; i l, (1 - i) l and i (1 - i) l diff have relative
+    errors of r + 2 u, r + 2 u and 2 r + 6 u besides those of l and diff."""
+    x, gate, h, dy, m = (v.detach().double().cpu() for v in (x, gate, h0, dy, dfinal))
+    t = x.shape[1]
+    take, keep = 1.0 / (1.0 + torch.exp(gate)), 1.0 / (1.0 + torch.exp(-gate))
+    r = (1.5 * gate.abs() + 8.0) * U
+    e, hm = torch.zeros_like(h), h.abs()
+    y, ey, before, eb, dm, dx, edx, dg, edg = (torch.zeros_like(x) for _ in range(9))
+    for s in range(t):
+        i, k = take[:, s], keep[:, s]
+        before[:, s], eb[:, s], dm[:, s] = h, e, x[:, s].abs() + hm
+        h, hm = k * h + i * x[:, s], k * hm + i * x[:, s].abs()
+        e = k * e + U * hm + torch.minimum(i, k) * dm[:, s] * (r[:, s] + 2 * U)
+        y[:, s], ey[:, s] = h, 4 * e
+    em, mm = torch.zeros_like(m), m.abs()
+    final = (h, 4 * e + U * hm)
+    for s in range(t - 1, -1, -1):
+        i, k, rel = take[:, s], keep[:, s], r[:, s]
+        lam, lm = dy[:, s] + m, dy[:, s].abs() + mm
+        el = em + U * lm
+        diff = before[:, s] - x[:, s]
+        dx[:, s], edx[:, s] = i * lam, 4 * i * el + i * lm * (rel + 2 * U)
+        dg[:, s] = i * k * lam * diff
+        edg[:, s] = 4 * i * k * (el * diff.abs() + lam.abs() * (eb[:, s] + U * dm[:, s])) + dg[:, s].abs() * (2 * rel + 6 * U)
+        em, m, mm = k * el + k * lm * (rel + 2 * U), k * lam, k * lm
+    return dict(y=(y, ey), final=final, dx=(dx, edx), dgate=(dg, edg), dstate=(m, 4 * em + U * mm))
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("b,t,d", [(3, 1, 64), (2, 12, 66), (2, 30, 65), (2, 300, 64), (1, 1500, 66)])
+def test_replaced_states_and_small_shares(dev, dtype, b, t, d):
+    """Gates on both sides and values of very different sizes: a value that replaces a larger state, and the gradients through
+    the share that is nearly gone, have all their digits."""
+    g = torch.Generator().manual_seed(t)
+
+    def sizes(*s):
+        return torch.randn(*s, generator=g) * 10.0 ** (torch.rand(*s, generator=g) * 6 - 3)
+    x, dy = (sizes(b, t, d).to(dtype).to(dev) for _ in range(2))
+    gate = (torch.rand(b, t, d, generator=g) * 50 - 30).to(dtype).to(dev)
+    h0, df = (1e3 * sizes(b, d).to(dev) for _ in range(2))
+    leaves = [v.requires_grad_() for v in (x, gate, h0)]
+    y, final = ops.gated_recurrence(*leaves)
+    grads = torch.autograd.grad((y, final), leaves, (dy, df))
+    want = _relative_oracle(x, gate, h0, dy, df)
+
+    def close(name, got, want):
+        # what is past float16's largest number by more than its bound and half a step rounds to infinity
+        ref, bound = want
+        past = ref.abs() - bound >= torch.finfo(got.dtype).max * (1 + torch.finfo(got.dtype).eps / 2)
+        off = got.detach().double().cpu()
+        assert torch.equal(off[past], ref[past].sign() * float("inf")), name
+        near = (ref.abs() + bound >= torch.finfo(got.dtype).max) & ~past
+        _close(name, off[~past & ~near].to(got.dtype), (ref[~past & ~near], bound[~past & ~near]))
+    for name, got in zip(("y", "final", "dx", "dgate", "dstate"), (y, final, *grads)):
+        close(name, got, want[name])
+    state = h0.detach().clone()
+    with torch.no_grad():
+        y1 = ops.gated_recurrence_step(x[:, 0], gate[:, 0], state)
+    for got in (y1, state):
+        close("step", got, (want["y"][0][:, 0], want["y"][1][:, 0]))
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_reset_forgets_a_large_state(dev):
+    """A gate of -inf or -200 replaces a state of any finite size exactly, in y, in the final state and in a step."""
+    x = torch.randn(2, 140, 6, generator=torch.Generator().manual_seed(3)).to(dev) * 1e-3
+    h0 = torch.full((2, 6), 1e30, device=dev)
+    for v in (float("-inf"), -200.0):
+        gate = torch.full_like(x, v)
+        y, final = ops.gated_recurrence(x, gate, h0)
+        assert torch.equal(y, x) and torch.equal(final, x[:, -1])
+        state = h0.clone()
+        assert torch.equal(ops.gated_recurrence_step(x[:, 0], gate[:, 0], state), x[:, 0]) and torch.equal(state, x[:, 0])

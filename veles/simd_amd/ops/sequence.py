@@ -75,10 +75,10 @@ def _recurrence_cpu(x, gate, state, lengths, save):
     b, t, d = x.shape
     on = _valid_steps(x, lengths)
     h = x.new_zeros(b, d, dtype=torch.float64) if state is None else state.double()
-    xd, i = x.double(), torch.sigmoid(-gate.double())
+    xd, i, keep = x.double(), torch.sigmoid(-gate.double()), torch.sigmoid(gate.double())
     y = x.new_zeros(b, t, d, dtype=torch.float64)
     for s in range(t):
-        h = torch.where(on[s][:, None], h + i[:, s] * (xd[:, s] - h), h)
+        h = torch.where(on[s][:, None], keep[:, s] * h + i[:, s] * xd[:, s], h)
         y[:, s] = torch.where(on[s][:, None], h, 0.0)
     # the CPU backward starts from the initial state: one tile
     starts = (x.new_zeros(b, d, dtype=torch.float32) if state is None else state)[:, None].clone() if save else None
@@ -107,20 +107,20 @@ def _recurrence_impl(x, gate, state, lengths, save):
 def _recurrence_backward_cpu(x, gate, lengths, starts, dy, dfinal):
     b, t, d = x.shape
     on = _valid_steps(x, lengths)
-    xd, i = x.double(), torch.sigmoid(-gate.double())
+    xd, i, keep = x.double(), torch.sigmoid(-gate.double()), torch.sigmoid(gate.double())
     h = starts[:, 0].double()
     before = x.new_zeros(b, t, d, dtype=torch.float64)
     for s in range(t):
         before[:, s] = h
-        h = torch.where(on[s][:, None], h + i[:, s] * (xd[:, s] - h), h)
+        h = torch.where(on[s][:, None], keep[:, s] * h + i[:, s] * xd[:, s], h)
     m = x.new_zeros(b, d, dtype=torch.float64) if dfinal is None else dfinal.double()
     dx, dg = (x.new_zeros(b, t, d, dtype=torch.float64) for _ in range(2))
     for s in range(t - 1, -1, -1):
         k = on[s][:, None]
         lam = m if dy is None else m + dy[:, s].double()
         dx[:, s] = torch.where(k, i[:, s] * lam, 0.0)
-        dg[:, s] = torch.where(k, i[:, s] * (1 - i[:, s]) * lam * (before[:, s] - xd[:, s]), 0.0)
-        m = torch.where(k, (1 - i[:, s]) * lam, m)
+        dg[:, s] = torch.where(k, i[:, s] * keep[:, s] * lam * (before[:, s] - xd[:, s]), 0.0)
+        m = torch.where(k, keep[:, s] * lam, m)
     return dx.to(x.dtype), dg.to(x.dtype), m.float()
 
 
@@ -240,16 +240,16 @@ def gated_recurrence(x: torch.Tensor, gate: torch.Tensor, state: torch.Tensor | 
                      lengths: torch.Tensor | None = None):
     """Gated linear recurrence along time, (y, final_state):
 
-        i_t = sigmoid(-gate_t),  h_t = h_{t-1} + i_t (x_t - h_{t-1}),  y_t = h_t
+        i_t = sigmoid(-gate_t),  h_t = (1 - i_t) h_{t-1} + i_t x_t,  y_t = h_t
 
     x, gate: [batch, time, channels], float32, float16 or bfloat16, any batch and time strides.
     state: h_0, float32 [batch, channels] (zeros if None); final_state is the float32 state after
     the last step, so a sequence can be continued by another call or by gated_recurrence_step.
     lengths: int32 / int64 [batch] on x's device: steps from lengths[b] on are padding (not read,
     y = 0, the state passes through; values outside 0..time are clamped).
-    The state is held in float32.  Differentiable in x, gate and state; in the padding the
-    gradients are 0 and dy is not read.  From an infinite state or value on, a channel is infinite or
-    NaN to its end (the formula above has inf - inf)."""
+    The state is held in float32, and i and 1 - i have all of float32's digits for every gate.  Differentiable
+    in x, gate and state; in the padding the gradients are 0 and dy is not read.  From an infinite state or
+    value on, a channel is infinite or NaN to its end."""
     save = records(x, gate, state)
     if plain_tensors(x, gate, state, lengths):
         if save:
@@ -284,7 +284,8 @@ def _step_impl(x, gate, state):
             and x.device == gate.device == state.device):
         _check_step(x, gate, state)
     if not x.is_cuda:
-        state += torch.sigmoid(-gate.double()) * (x.double() - state)
+        g = gate.double()
+        state.copy_(torch.sigmoid(g) * state + torch.sigmoid(-g) * x)
         return state.to(x.dtype, copy=True)
     b, d = x.shape
     if x.is_contiguous() and gate.is_contiguous():
