@@ -65,13 +65,37 @@ __device__ __forceinline__ floatx4 mma(const u32x4 &a, const u32x4 &b, floatx4 c
 }
 
 // -------------------------------------------------------------- activations
+// No tail is the rest of a subtraction: it is computed and the large side is what it leaves of 1, and the
+// sigmoid's slope is e / (1 + e)^2, not s (1 - s).
+//
+// The normal distribution Phi(g) and E = exp(-g^2 / 2).  With z = |g|, Phi(-z) / E falls smoothly from 1/2 as
+// 1 / (sqrt(2 pi) z): times z + 3 it is a polynomial of degree 8 in (z - 3) / (z + 3), fitted on 0 <= z <= 14 (E
+// underflows at 13.2) to the least largest relative error, 5e-8; in fp32 3.4e-7.  (8192 x 1024, 8192 outputs, gelu:
+// 267 us, 305 with the library's erfcf, 295 with 1 + erff, whose tail has no digits from -5 on.)
+struct Normal {
+  float phi, e;
+};
+__device__ __forceinline__ Normal normal(float g) {
+  const float z = fabsf(g), e = __expf(-0.5f * z * z), r = __builtin_amdgcn_rcpf(z + 3.f), t = fmaf(-6.f, r, 1.f);
+  float p = -2.6676857e-4f;
+  p = fmaf(p, t, -9.0325432e-4f);
+  p = fmaf(p, t, 1.0760390e-3f);
+  p = fmaf(p, t, 6.9239237e-3f);
+  p = fmaf(p, t, -1.0479936e-2f);
+  p = fmaf(p, t, -4.7256101e-2f);
+  p = fmaf(p, t, 0.23001935f);
+  p = fmaf(p, t, -0.50933230f);
+  p = fmaf(p, t, 0.72908366f);
+  const float tail = p * r * e;
+  return Normal{g < 0.f ? tail : 1.f - tail, e};
+}
 __device__ __forceinline__ float sigmoid(float g) {
   return __builtin_amdgcn_rcpf(1.f + __expf(-g));
 }
 __device__ __forceinline__ float act(int kind, float g) {
   switch (kind) {
     case VS_ACT_SILU: return g * sigmoid(g);
-    case VS_ACT_GELU: return 0.5f * g * (1.f + erff(g * 0.70710678118654752f));
+    case VS_ACT_GELU: return g * normal(g).phi;
     case VS_ACT_RELU: return g > 0.f ? g : g == g ? 0.f : g;
     default: return sigmoid(g);
   }
@@ -82,13 +106,14 @@ __device__ __forceinline__ float act_slope(int kind, float g) {
       const float s = sigmoid(g);
       return s * fmaf(g, 1.f - s, 1.f);
     }
-    case VS_ACT_GELU:
-      return fmaf(g * 0.39894228040143268f, __expf(-0.5f * g * g),
-                  0.5f * (1.f + erff(g * 0.70710678118654752f)));
+    case VS_ACT_GELU: {
+      const Normal n = normal(g);
+      return fmaf(g * 0.39894228040143268f, n.e, n.phi);
+    }
     case VS_ACT_RELU: return g > 0.f ? 1.f : 0.f;
     default: {
-      const float s = sigmoid(g);
-      return s * (1.f - s);
+      const float e = __expf(-fabsf(g)), r = __builtin_amdgcn_rcpf(1.f + e);
+      return e * r * r;
     }
   }
 }

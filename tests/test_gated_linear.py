@@ -467,3 +467,46 @@ def test_split_gradients_native_refusals_and_workspace():
     size = lib.vs_gated_linear_gradients_workspace
     assert size(4096, 2048, 2048, 1, 1, 1, 1, 1) == 2 * size(4096, 2048, 2048, 0, 1, 1, 1, 1) == 2 * 4096 * 8192
     assert size(1 << 30, 64, 64, 1, 1, 1, 1, 1) == 0 and size(64, 1 << 20, 64, 1, 1, 1, 1, 1) == 0
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("m", [9, 130])
+def test_tails_of_activations(dev, act, m):
+    """k = 1 with a gate weight of 1 and an up weight of 1: g = u = x exactly.  h = act(x) x and, from dh = 1, the weights'
+    gradients of one row, act'(x) x x and act(x) x, to a few units of their own last place however small they are: functions of
+    16 u and 1.5 |g| u for the exponential's argument (g^2 / 2 for gelu; erfc's is rounded, u g^2), 4 u for the products, then
+    roundings to 16 bits: one of h, two of a gradient.  A slope's two terms are rounded apart."""
+    x = torch.cat([torch.arange(-9, 20.01, 0.125), torch.tensor([1e-3, -1e-3, 40.0, -40.0])]).to(torch.bfloat16)
+    for values in (x, x.flip(0)):
+        for v in values.split(m):
+            d = v.double()
+            rows = v[:, None].to(dev)
+            one = torch.ones(1, 1, dtype=torch.bfloat16, device=dev)
+            h = ops.gated_linear(rows, one, one, act)
+            a, slope = _act(act, d)
+            if act == "gelu":
+                arg = d * d
+                parts = 0.5 * torch.special.erfc(-d * 0.5 ** 0.5) + d.abs() * torch.exp(-0.5 * d * d) / (2 * torch.pi) ** 0.5
+            else:
+                arg, parts = 1.5 * d.abs(), slope.abs()
+                if act == "silu":
+                    s = torch.sigmoid(d)
+                    parts = s + d.abs() * s * torch.sigmoid(-d)
+                if act == "sigmoid":     # s (1 - s) loses digits in the file's oracle
+                    slope = parts = torch.sigmoid(d) * torch.sigmoid(-d)
+            rel, e = (24 + 2 * arg) * U, 2.0 ** -8
+            tiny = torch.finfo(torch.bfloat16).smallest_normal
+
+            def near(got, ref, bound, roundings):
+                tol = bound + ref.abs() * ((1 + e) ** roundings - 1) + 2 * e * bound + tiny * (1 + d.abs())
+                off = (got.detach().double().cpu().flatten() - ref).abs()
+                assert (off <= tol).all(), (act, d[off > tol], (off / tol).max().item())
+            near(h, a * d, (a * d).abs() * rel, 1)
+            # a feature for every value, one row: dw_gate = dh u act'(g) x, dw_up = dh act(g) x with x = 1
+            wg = v[:, None].to(dev).clone().requires_grad_()
+            wu = v[:, None].to(dev).clone().requires_grad_()
+            up = torch.ones(1, len(v), dtype=torch.bfloat16, device=dev)
+            dwg, dwu = torch.autograd.grad(ops.gated_linear(one, wg, wu, act), (wg, wu), up)
+            near(dwg, d * slope, d.abs() * parts * rel, 2)
+            near(dwu, a, a.abs() * rel, 2)

@@ -491,7 +491,7 @@ def _act_cpu(kind, g):
     if kind == "silu":
         return g * torch.sigmoid(g)
     if kind == "gelu":
-        return 0.5 * g * (1.0 + torch.erf(g * 0.5 ** 0.5))
+        return 0.5 * g * torch.special.erfc(g * -0.5 ** 0.5)
     return torch.relu(g) if kind == "relu" else torch.sigmoid(g)
 
 
@@ -500,8 +500,8 @@ def _slope_cpu(kind, g):
     if kind == "silu":
         return s * (1.0 + g * (1.0 - s))
     if kind == "gelu":
-        return 0.5 * (1.0 + torch.erf(g * 0.5 ** 0.5)) + g * torch.exp(-0.5 * g * g) * (0.5 / torch.pi) ** 0.5
-    return (g > 0).to(g.dtype) if kind == "relu" else s * (1.0 - s)
+        return 0.5 * torch.special.erfc(g * -0.5 ** 0.5) + g * torch.exp(-0.5 * g * g) * (0.5 / torch.pi) ** 0.5
+    return (g > 0).to(g.dtype) if kind == "relu" else s * torch.sigmoid(-g)
 
 
 def _gated_impl(x, w_gate, w_up, activation, save, split=False):
