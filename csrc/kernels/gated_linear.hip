@@ -999,6 +999,10 @@ int64_t tiles_of(const Args &p) {
   return static_cast<int64_t>((p.m + C::BM - 1) / C::BM) * ((p.n + C::BO - 1) / C::BO) * p.parts;
 }
 
+// Tiles of one launch.  Backward a grid holds fewer than 2^32 threads; forward workgroups walk the tiles.
+template <class C>
+constexpr int64_t kMostTiles = C::GATED ? 1ll << 31 : 1ll << 23;
+
 template <class N, class C, bool SPLIT>
 vs_status launch_tile(const Args *q, int count, hipStream_t s) {
   constexpr auto kernel = [] {
@@ -1015,7 +1019,7 @@ vs_status launch_tile(const Args *q, int count, hipStream_t s) {
       w.q[i] = q[i];
       tiles += tiles_of<C>(q[i]);
     }
-    VS_REQUIRE(tiles < (1ll << 23), "gated_linear: too many output tiles");
+    VS_REQUIRE(tiles < kMostTiles<C>, "gated_linear: too many output tiles");
     w.end[i] = static_cast<unsigned>(tiles);
   }
   // forward: as many workgroups as fit the chip walk the tiles; backward: a workgroup per tile, the
@@ -1026,6 +1030,8 @@ vs_status launch_tile(const Args *q, int count, hipStream_t s) {
   VS_HIP(hipGetLastError());
   return VS_OK;
 }
+
+constexpr double kNever = 1e30;  // the estimate of what does not fit a launch
 
 // Estimated time, in units of 1 us at the sizes below, of `count` products with tiles of C.  A tile
 // of nk k tiles takes `fixed` + `step` nk when the chip is full of them and `fixed` + `alone` nk
@@ -1039,6 +1045,9 @@ double estimate(const Args *q, int count) {
   constexpr double alone = C::XH == 4 ? 0.92 : C::YH == 2 ? 0.59 : 0.42;
   const double slots = device_cu_count() * (160 * 1024 / C::kLds);
   double total = 0, longest = 0, t = 0;
+  int64_t tiles = 0;
+  for (int i = 0; i < count; i++) tiles += tiles_of<C>(q[i]);
+  if (tiles >= kMostTiles<C>) return kNever;
   for (int i = 0; i < count; i++) {
     const double nk = k_tiles(q[i]), n = static_cast<double>(tiles_of<C>(q[i]));
     const int64_t rounds = static_cast<int64_t>(n / slots);
@@ -1094,13 +1103,15 @@ double cut(Args *q, int count) {
   }
 }
 
-// Tile shape (0: 256 x 256, 1: 128 x 256, 2: 128 x 128) and the parts of each product.
+// Tile shape (0: 256 x 256, 1: 128 x 256, 2: 128 x 128; -1: too many tiles of every shape) and the parts of each
+// product.
 template <bool GATED>
 int plan(Args *q, int count) {
   Args w[kProducts], s[kProducts];
   for (int i = 0; i < count; i++) w[i] = s[i] = q[i];
   const double large = cut<Cfg<4, 2, GATED>>(q, count), wide = cut<Cfg<2, 2, GATED>>(w, count),
                small = cut<Cfg<2, 1, GATED>>(s, count);
+  if (std::min({large, wide, small}) >= kNever) return -1;
   if (large <= wide && large <= small) return 0;
   for (int i = 0; i < count; i++) q[i] = wide <= small ? w[i] : s[i];
   return wide <= small ? 1 : 2;
@@ -1213,7 +1224,8 @@ ForwardNeed forward_need(Args &p, bool dx, bool dg, bool du) {
   const size_t kp = up8(p.k);
   q.shape = plan<true>(&p, 1);
   q.sums = sums_bytes(p, true);
-  q.bytes = q.sums + (q.px ? up256(2 * p.m * kp) : 0) + ((q.pg ? 1 : 0) + (q.pu ? 1 : 0)) * up256(2 * p.n * kp);
+  const size_t m = p.m, n = p.n;
+  q.bytes = q.sums + (q.px ? up256(2 * m * kp) : 0) + ((q.pg ? 1 : 0) + (q.pu ? 1 : 0)) * up256(2 * n * kp);
   return q;
 }
 
@@ -1266,6 +1278,7 @@ vs_status forward(Args p, void *workspace, size_t bytes, hipStream_t s) {
     }
   }
   const ForwardNeed q = forward_need(p, da, dg, du);
+  VS_REQUIRE(q.shape >= 0, "gated_linear: too many output tiles");
   DeviceBuffer own;
   Space sp;
   VS_TRY(open_space(sp, own, workspace, bytes, q.bytes, s));
@@ -1331,6 +1344,7 @@ vs_status backward(const uint16_t *x, int64_t ldx, const uint16_t *wg, int64_t l
   const bool ax = direct(x, ldx, k) && ldx >= k && ldx < kMostLd,
              aw = direct(wg, ldg, k) && direct(wu, ldu, k) && ldg == ldu && ldg >= k && ldg < kMostLd;
   BackwardNeed need = backward_need(m, f, k, dx, dw[0], dw[1], split, ax, aw);
+  VS_REQUIRE(need.shape >= 0, "gated_linear_backward: too many output tiles");
   VS_TRY(open_space(sp, own, workspace, bytes, need.bytes, s));
   const int fp = (f + 63) / 64 * 64, ld = (split ? 4 : 2) * fp;
   Slopes sl{};

@@ -510,3 +510,36 @@ def test_tails_of_activations(dev, act, m):
             dwg, dwu = torch.autograd.grad(ops.gated_linear(one, wg, wu, act), (wg, wu), up)
             near(dwg, d * slope, d.abs() * parts * rel, 2)
             near(dwu, a, a.abs() * rel, 2)
+
+
+def test_workspaces_of_very_many_rows():
+    """Sizes stay sizes up to the documented 2^31 rows; what no launch holds is refused, not begun."""
+    lib = _lib.lib()
+    size = lib.vs_gated_linear_workspace
+    for m in (1 << 30, (1 << 30) + 5, (1 << 31) - 300):
+        for k, f in ((1, 1), (9, 30), (1001, 500)):
+            rows = 2 * m * ((k + 7) // 8 * 8)
+            assert rows <= size(m, f, k, 0) <= 1.01 * rows + (1 << 30)
+            assert size(m, f, k + (-k) % 8, 1) == 0
+    p = torch.zeros(8).data_ptr()
+    m, f, k = (1 << 31) - 300, 64, 1 << 19
+    need = lib.vs_gated_linear_gradients_workspace(m, f, k, 0, 1, 1, 1, 1)
+    assert lib.vs_gated_linear_gradients(5, 0, 0, p, k, p, k, p, k, p, p, f, m, f, k, p, p, p, p, need, None) == 1
+    assert b"too many" in lib.vs_last_error()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("k,f", [(8, 8), (1, 1)])
+def test_2_to_the_30_rows(k, f):
+    """More small tiles than a launch of one workgroup each would hold, read in place and from copied rows."""
+    m = (1 << 30) + 5
+    rows = torch.randn(1 << 12, k, generator=torch.Generator().manual_seed(5)).bfloat16().cuda()
+    x = rows.repeat((m >> 12) + 1, 1)[:m]
+    wg, wu = (torch.randn(f, k, generator=torch.Generator().manual_seed(s)).bfloat16().cuda() for s in (6, 7))
+    h = ops.gated_linear(x, wg, wu)
+    want = ops.gated_linear(rows, wg, wu)
+    _close("h", want, _oracle(rows, wg, wu, torch.zeros_like(want), "silu")["h"])
+    assert torch.equal(h[m >> 12 << 12:], want[:m & 4095])
+    blocks = h[:m >> 12 << 12].view(-1, 1 << 12, f)
+    for part in blocks.split(1 << 14):
+        assert torch.equal(part, want.expand_as(part))
