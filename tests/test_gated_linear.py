@@ -543,3 +543,36 @@ def test_2_to_the_30_rows(k, f):
     blocks = h[:m >> 12 << 12].view(-1, 1 << 12, f)
     for part in blocks.split(1 << 14):
         assert torch.equal(part, want.expand_as(part))
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("split", [False, True])
+@pytest.mark.parametrize("m,k,f", [(33, 64, 24), (300, 40, 200), (700, 2048, 33)])
+def test_gradients_are_made_one_by_one(dev, split, m, k, f):
+    """Every set of gradients: those that are asked for have the bits of a call of their own, in memory of their own, and the
+    backward op returns nothing for the others."""
+    args = _inputs(m, k, f, torch.bfloat16, dev, seed=16)
+    x, wg, wu, dh = args
+    pre = torch.ops.veles.gated_linear(x, wg, wu, "silu", True)[1]
+    want = _oracle(x, wg, wu, dh, "silu")
+    for need in range(1, 8):
+        on = [bool(need >> i & 1) for i in range(3)]
+        leaves = [v.detach().requires_grad_(n) for v, n in zip(args[:3], on)]
+        h = ops.gated_linear(*leaves, split_gradients=split)
+        got = torch.autograd.grad(h, [v for v in leaves if v.requires_grad], dh)
+        op = torch.ops.veles.gated_linear_backward(x, wg, wu, pre, dh, "silu", *on, split)
+        assert [o.numel() for o in op] == [v.numel() if n else 0 for v, n in zip(args, on)]
+        for name, g, o in zip([n for n, a in zip(("dx", "dw_gate", "dw_up"), on) if a], got, [o for o, a in zip(op, on) if a]):
+            assert torch.equal(g, o) and g.untyped_storage().nbytes() == 2 * g.numel()
+            _close(name, g, want[name])
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_second_derivatives_are_recorded_to_be_refused(dev):
+    x, wg, wu, dh = _inputs(5, 16, 8, torch.bfloat16, dev)
+    for i in range(3):
+        leaves = [v.detach().requires_grad_(j == i) for j, v in enumerate((x, wg, wu))]
+        g, = torch.autograd.grad(ops.gated_linear(*leaves).sum(), leaves[i], create_graph=True)
+        assert g.requires_grad
+        with pytest.raises(NotImplementedError, match="second"):
+            g.float().sum().backward()

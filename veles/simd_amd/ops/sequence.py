@@ -544,7 +544,8 @@ def _aligned(*tensors) -> bool:
     return all(t.shape[-1] % 8 == 0 and t.stride(0) % 8 == 0 and t.data_ptr() % 16 == 0 for t in tensors)
 
 
-def _gated_backward_impl(x, w_gate, w_up, pre, dh, activation, want_dx, want_dw, split=False):
+def _gated_backward_impl(x, w_gate, w_up, pre, dh, activation, want_dx, want_dw_gate, want_dw_up=None, split=False):
+    want_dw_up = want_dw_gate if want_dw_up is None else want_dw_up
     name = "veles::gated_linear_backward"
     _check_gated(name, x, w_gate, w_up, activation)
     f, k = w_gate.shape
@@ -559,19 +560,21 @@ def _gated_backward_impl(x, w_gate, w_up, pre, dh, activation, want_dx, want_dw,
         g, u, d = pre[..., 0].double(), pre[..., 1].double(), dhr.double()
         dg, du = d * u * _slope_cpu(activation, g), d * _act_cpu(activation, g)
         dx = (dg @ w_gate.double() + du @ w_up.double()).to(x.dtype).view(x.shape) if want_dx else x.new_empty(0)
-        dw = torch.cat([dg.t() @ rows.double(), du.t() @ rows.double()]).to(x.dtype) if want_dw else x.new_empty(0)
-        return dx, dw
+        return dx, *((v.t() @ rows.double()).to(x.dtype) if want else x.new_empty(0)
+                     for v, want in ((dg, want_dw_gate), (du, want_dw_up)))
     w_gate, w_up, pre = _near_rows(w_gate, False), _near_rows(w_up, False), pre.contiguous()
     dx = torch.empty(x.shape if want_dx else (0,), dtype=x.dtype, device=x.device)
-    dw = torch.empty((2 * f, k) if want_dw else (0,), dtype=x.dtype, device=x.device)
+    dwg, dwu = (torch.empty((f, k) if want else (0,), dtype=x.dtype, device=x.device)
+                for want in (want_dw_gate, want_dw_up))
     aligned = (w_gate.stride(0) == w_up.stride(0) >= k <= rows.stride(0)) and _aligned(rows, w_gate, w_up)
-    size = int(_lib.lib().vs_gated_linear_gradients_workspace(m, f, k, split, want_dx, want_dw, want_dw, aligned))
+    size = int(_lib.lib().vs_gated_linear_gradients_workspace(m, f, k, split, want_dx, want_dw_gate,
+                                                                want_dw_up, aligned))
     ws = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
     launch(x, "vs_gated_linear_gradients", DTYPES[x.dtype], ACTIVATIONS[activation], split, rows.data_ptr(),
            rows.stride(0), w_gate.data_ptr(), w_gate.stride(0), w_up.data_ptr(), w_up.stride(0), pre.data_ptr(),
            dhr.data_ptr(), dhr.stride(0), m, f, k, dx.data_ptr() if want_dx else None,
-           dw.data_ptr() if want_dw else None, dw[f:].data_ptr() if want_dw else None, _opt(ws), size)
-    return dx, dw
+           dwg.data_ptr() if want_dw_gate else None, dwu.data_ptr() if want_dw_up else None, _opt(ws), size)
+    return dx, dwg, dwu
 
 
 def _gated_fake(x, w_gate, w_up, activation, save, split=False):
@@ -601,9 +604,8 @@ def _gated_grads(ctx, backward, dh):
         return None, None, None
     x, w_gate, w_up, pre = ctx.saved_tensors
     need = ctx.needs_input_grad
-    dx, dw = backward(x, w_gate, w_up, pre, dh, ctx.activation, need[0], need[1] or need[2], ctx.split)
-    f = w_gate.shape[0]
-    return dx if need[0] else None, dw[:f] if need[1] else None, dw[f:] if need[2] else None
+    grads = backward(x, w_gate, w_up, pre, dh, ctx.activation, *need[:3], ctx.split)
+    return tuple(g if n else None for g, n in zip(grads, need))
 
 
 class _Gated(torch.autograd.Function):
@@ -632,13 +634,17 @@ torch.library.register_fake("veles::gated_linear", _gated_fake)
 torch.library.register_autograd("veles::gated_linear", _gated_grad, setup_context=_gated_setup)
 torch.library.define("veles::gated_linear_backward",
                      "(Tensor x, Tensor w_gate, Tensor w_up, Tensor pre, Tensor dh, str activation, bool want_dx, "
-                     "bool want_dw, bool split=False) -> (Tensor, Tensor)")
+                     "bool want_dw_gate, bool? want_dw_up=None, bool split=False) -> (Tensor, Tensor, Tensor)")
 torch.library.impl("veles::gated_linear_backward", "default", _gated_backward_impl)
-torch.library.register_fake(
-    "veles::gated_linear_backward",
-    lambda x, w_gate, w_up, pre, dh, activation, want_dx, want_dw, split=False: (
-        x.new_empty(x.shape if want_dx else (0,)),
-        x.new_empty((2 * w_gate.shape[0], w_gate.shape[1]) if want_dw else (0,))))
+
+
+def _gated_backward_fake(x, w_gate, w_up, pre, dh, activation, want_dx, want_dw_gate, want_dw_up=None, split=False):
+    want_dw_up = want_dw_gate if want_dw_up is None else want_dw_up
+    return (x.new_empty(x.shape if want_dx else (0,)), w_gate.new_empty(w_gate.shape if want_dw_gate else (0,)),
+            w_up.new_empty(w_up.shape if want_dw_up else (0,)))
+
+
+torch.library.register_fake("veles::gated_linear_backward", _gated_backward_fake)
 _no_second_derivative("veles::gated_linear_backward")
 
 
