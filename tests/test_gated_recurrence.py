@@ -592,3 +592,16 @@ def test_reset_forgets_a_large_state(dev):
         assert torch.equal(y, x) and torch.equal(final, x[:, -1])
         state = h0.clone()
         assert torch.equal(ops.gated_recurrence_step(x[:, 0], gate[:, 0], state), x[:, 0]) and torch.equal(state, x[:, 0])
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_second_derivatives_are_recorded_to_be_refused(dev):
+    """(The gradient in the state alone of a linear loss is a constant, a product of shares: there is nothing to record.)"""
+    args = _inputs(2, 5, 4, torch.float32, dev)[:3]
+    for i, linear in ((0, True), (1, True), (0, False), (1, False), (2, False)):
+        leaves = [v.detach().requires_grad_(j == i) for j, v in enumerate(args)]
+        y = ops.gated_recurrence(*leaves)[0]
+        g, = torch.autograd.grad((y if linear else y.square()).sum(), leaves[i], create_graph=True)
+        assert g.requires_grad
+        with pytest.raises(NotImplementedError, match="second"):
+            g.sum().backward()
