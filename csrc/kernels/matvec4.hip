@@ -14,8 +14,10 @@
 //
 //   s (sum x (16 + q) - (16 + z) sum x)
 //
-// where sum x comes from one more product, with ones, in the layout it is needed in.  The factor
-// 16 costs at most 3 of fp32's 24 bits against the sum of |x (q - z)|; weights are never rounded.
+// where sum x comes from one more product, with ones, in the layout it is needed in.  Weights are never
+// rounded.  What is rounded, to 2^-24 each time, are sums of |x| (16 + q) s and |x| (16 + z) s, not of
+// |x (q - z)| s: weights near their zero point give a remainder of that size in the place of a smaller sum or
+// of 0, and a group's sum of 31 |x| (of (16 + z) |x| where z > 15) has to stay below fp32's largest number.
 //
 // A step is 128 k of 16 columns: 64 bytes of each row, which four neighbouring lanes load.  (16
 // neighbouring lanes on 16 rows, the order the matrix instruction wants, cost the cache four times

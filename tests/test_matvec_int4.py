@@ -209,3 +209,45 @@ def test_opcheck(dev):
     x, q, s, z = _inputs(2, 8, 64, 32, torch.bfloat16, dev)
     for args in ((x, q, s, z, 32), (x, q, s, None, 32)):
         torch.library.opcheck(torch.ops.veles.matvec_int4.default, args)
+
+
+def _check_offsets(y, x, q, s, z, group):
+    """The bound that holds for any weights: every rounding is of a partial sum of |x| (16 + q) s or |x| (16 + z) s."""
+    k = x.shape[-1]
+    xd, at = x.detach().double(), torch.arange(k, device=x.device) // group
+    nibbles = torch.stack([q & 15, q >> 4], -1).flatten(1)[:, :k].double()
+    zero = 8.0 if z is None else z.double()[:, at]
+    scale = s.double()[:, at]
+    ref = xd @ ((nibbles - zero) * scale).t()
+    tol = (k / 32 + 48) * U * (xd.abs() @ ((32 + nibbles + zero) * scale).t())
+    tol = tol + torch.finfo(y.dtype).eps / 2 * (ref.abs() + tol) + torch.finfo(y.dtype).smallest_normal
+    assert ((y.double() - ref).abs() <= tol).all(), ((y.double() - ref).abs() / tol).max().item()
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("m,n,k,group", [(1, 40, 256, 128), (3, 33, 301, 32), (16, 64, 1030, 64), (20, 17, 640, 384)])
+@pytest.mark.parametrize("kind", ["zero", "near", "far"])
+def test_weights_at_and_far_from_their_zero_point(dev, dtype, m, n, k, group, kind):
+    """Weights that are all 0, or one step from it, and zero points up to 255."""
+    x, q, s, z = _inputs(m, n, k, group, dtype, dev, seed=21)
+    if kind == "far":
+        z = torch.randint(0, 256, z.shape, generator=torch.Generator().manual_seed(22), dtype=torch.uint8).to(dev)
+    else:
+        at = torch.arange(2 * q.shape[1], device=dev).clamp(max=k - 1) // group
+        nibbles = z[:, at]
+        if kind == "near":
+            step = torch.randint(-1, 2, nibbles.shape, generator=torch.Generator().manual_seed(23)).to(dev)
+            nibbles = (nibbles.int() + step).clamp(0, 15).to(torch.uint8)
+        q = nibbles[:, 0::2] | (nibbles[:, 1::2] << 4)
+    _check_offsets(ops.matvec_int4(x, q, s, z, group), x, q, s, z, group)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_large_finite_values(dev):
+    """Values up to the limit that the documentation names: 31 sum |x| of a group of 128 just below 3.4e38."""
+    x, q, s, z = _inputs(4, 50, 512, 128, torch.bfloat16, dev, seed=24)
+    x = (x.double() / x.double().abs().view(4, 4, 128).sum(-1).max() * 1e37).bfloat16()
+    y = ops.matvec_int4(x, q, s, z, 128)
+    assert torch.isfinite(y).all()
+    _check_offsets(y, x, q, s, z, 128)

@@ -405,8 +405,9 @@ def matvec_int4(x: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor,
     qweight: uint8 [n, (k + 1) // 2], two numbers 0..15 to a byte, the even column in the low half.
     scales: x's type, [n, ceil(k / group_size)]; zeros: uint8 of that shape (8 everywhere if None).
     group_size: 32, 64 or a multiple of 128; the last group may end early.  Weights are exact and sums
-    are float32; the result is rounded once, to x's type.  An infinite x gives NaN (the zero point is
-    taken off the sum).  For generation: it records no gradient; more than 16 rows read the weights
+    are float32; the result is rounded once, to x's type.  On a GPU the zero points are taken off the sums, so
+    float32's rounding is relative to sum |x| (32 + q + zeros) scales, also where q is close to zeros, and x has to be
+    finite, with sums of 31 |x| (or (16 + zeros) |x|, where that is more) over a group below 3.4e38.  For generation: it records no gradient; more than 16 rows read the weights
     once for every 16.  quantize_int4 makes the operands."""
     if records(x, scales):
         raise RuntimeError("matvec_int4 records no gradient: call it under torch.no_grad()")
