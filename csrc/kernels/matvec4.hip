@@ -353,18 +353,27 @@ void launch_group(const Args &p, int group, hipStream_t s) {
   else launch<N, W, CT, 4>(p, s);
 }
 
-// Waves and column tiles of a workgroup: the most columns (x is read and rearranged once for all of
-// them), then the fewest waves (each starts and ends a pipeline), that still make about 2048 waves,
-// eight for each CU.  One row, us: 28000 x 8192 g64 33 with (4 waves, 4 tiles), 35 (4, 2), 43
-// (8, 2), 42 (8, 1); 8192 x 8192 g128 19, 14, 12, 14; 4096 x 4096 g128 10.5, 7.6, 7.3, 6.2;
-// 16384 x 2048 g128 8.6, 7.3, 9.8, 10.7.
+// Waves W and column tiles of a workgroup, by how many fall to a CU.  One workgroup of eight waves fits a CU, or two
+// of four.  While one of them a CU is enough, eight waves with as many tiles as that takes; above, four
+// waves with four tiles, which read and rearrange x once for 64 columns, unless two tiles spread so much
+// more evenly that the fullest CU has less than 7/8 of the tiles.  (The rows do not count: a row gets the
+// same bits in every batch.)  1 and 16 rows, us with (8 waves, 1 tile),
+// (8, 2), (4, 2), (4, 4):
+//   4096 x 4096 g128      6.0  7.1  7.4 10.3     6.4  7.7  7.7 11.2
+//   8192 x 8192 g128     16.1 11.8 13.7 18.4    19.0 14.2 14.7 20.2
+//   11008 x 4096 g64     18.2 17.1 11.4 12.3    19.4 19.5 13.3 13.3
+//   24000 x 8192 g64     44.9 32.9 29.6 32.9    53.0 41.4 35.5 37.9   (96 columns a CU in pairs, 128 in fours)
+//   27000 x 8192 g128    50.5 38.0 34.6 31.2    57.7 46.5 42.7 36.1   (128 both ways)
+//   50000 x 4096 g64     73.0 57.0 32.0 33.1    77.7 67.7 40.0 37.8   (224, 256)
 template <class N>
 void launch_type(const Args &p, int group, hipStream_t s) {
-  const auto waves = [&](int w, int ct) { return (p.n + 16 * ct - 1) / (16 * ct) * w; };
-  if (waves(4, 4) >= 1700) launch_group<N, 4, 4>(p, group, s);
-  else if (waves(4, 2) >= 1700) launch_group<N, 4, 2>(p, group, s);
-  else if (waves(8, 2) >= 1700) launch_group<N, 8, 2>(p, group, s);
-  else launch_group<N, 8, 1>(p, group, s);
+  const int cus = device_cu_count();
+  const auto groups = [&](int ct) { return (p.n + 16 * ct - 1) / (16 * ct); };
+  const auto fullest = [&](int ct) { return (groups(ct) + cus - 1) / cus * ct; };
+  if (groups(1) <= cus) launch_group<N, 8, 1>(p, group, s);
+  else if (groups(2) <= cus) launch_group<N, 8, 2>(p, group, s);
+  else if (groups(4) <= cus || 8 * fullest(2) < 7 * fullest(4)) launch_group<N, 4, 2>(p, group, s);
+  else launch_group<N, 4, 4>(p, group, s);
 }
 
 }  // namespace

@@ -251,3 +251,14 @@ def test_large_finite_values(dev):
     y = ops.matvec_int4(x, q, s, z, 128)
     assert torch.isfinite(y).all()
     _check_offsets(y, x, q, s, z, 128)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,k", [(1001, 1500), (5000, 600), (9001, 520), (20000, 300), (27000, 260)])
+def test_a_row_has_the_same_bits_in_every_batch(n, k):
+    """Every shape of workgroup: a row alone, among 16, and among more than 16 rows."""
+    x, q, s, z = _inputs(37, n, k, 64, torch.bfloat16, "cuda", seed=25)
+    whole = ops.matvec_int4(x, q, s, z, 64)
+    _check(whole, x, q, s, z, 64)
+    for rows in (slice(0, 1), slice(3, 7), slice(5, 21), slice(36, 37)):
+        assert torch.equal(ops.matvec_int4(x[rows], q, s, z, 64), whole[rows])
