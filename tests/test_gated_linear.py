@@ -576,3 +576,13 @@ def test_second_derivatives_are_recorded_to_be_refused(dev):
         assert g.requires_grad
         with pytest.raises(NotImplementedError, match="second"):
             g.float().sum().backward()
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_split_gradients_are_refused_before_the_forward_pass(dev):
+    x = torch.zeros(1, 1, dtype=torch.bfloat16, device=dev)
+    w = torch.zeros((1 << 19) + 1, 1, dtype=torch.bfloat16, device=dev).requires_grad_()
+    with pytest.raises(ValueError, match="split gradients"):
+        ops.gated_linear(x, w, w, split_gradients=True)
+    with torch.no_grad():
+        assert ops.gated_linear(x, w, w, split_gradients=True).shape == (1, (1 << 19) + 1)

@@ -523,6 +523,8 @@ def _gated_impl(x, w_gate, w_up, activation, save, split=False):
     f, k = w_gate.shape
     rows = _near_rows(_as_rows(x), True)
     m = rows.shape[0]
+    if save and split and (f > 1 << 19 or m >= (1 << 30) - 256):
+        raise ValueError(f"{name}: split gradients of {m} rows and {f} features; 2^30 - 257 and 2^19 at most")
     if not x.is_cuda:
         g, u = rows.double() @ w_gate.double().t(), rows.double() @ w_up.double().t()
         h = (_act_cpu(activation, g) * u).to(x.dtype).view(*x.shape[:-1], f)
@@ -614,7 +616,7 @@ class _Gated(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, w_gate, w_up, activation, split):
-        h, pre = _gated_impl(x, w_gate, w_up, activation, True)
+        h, pre = _gated_impl(x, w_gate, w_up, activation, True, split)
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(x, w_gate, w_up, pre)
         ctx.activation, ctx.split = activation, split
@@ -661,7 +663,7 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor,
     which adds about 0.4 of the result's own rounding to the error; in float16 they are lost below 6e-8 and
     infinite above 65504, so the loss has to be scaled.  split_gradients takes each as the sum of two numbers of x's
     type (to 2^-16 of it in bfloat16, to 2^-22 or 3e-8 in float16), so the result's own rounding is all that counts,
-    for twice the multiplications of the backward pass (on a CPU they are not rounded at all).  Up to 64 rows (generation) stream the weights once at memory speed."""
+    for twice the multiplications of the backward pass (up to 2^19 features; on a CPU they are not rounded at all).  Up to 64 rows (generation) stream the weights once at memory speed."""
     save = records(x, w_gate, w_up)
     if plain_tensors(x, w_gate, w_up):
         if save:
