@@ -26,7 +26,7 @@
 // 16-lane groups.  Two swaps of half and quarter waves transpose the four registers against the
 // four groups, so that one instruction sees 32 neighbouring k and any group of 32 or more can be
 // scaled.  The waves of a workgroup share its columns and cut k; their sums meet in LDS in a fixed
-// order.  28000 x 8192 with groups of 64: 33 us for one row, 39 for 16 (3.8 and 3.3 TB/s).
+// order.  28000 x 8192 with groups of 64: 35 us for one row, 40 for 16 (3.6 and 3.1 TB/s).
 // Copyright 2026 veles.simd_amd authors. Apache-2.0.
 #include <hip/hip_runtime.h>
 
@@ -156,7 +156,8 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))
 #pragma unroll
   for (int c = 0; c < CT; c++)
     qr[c] = p.q + (n0 + 16 * c + r4 < p.n ? n0 + 16 * c + r4 : p.n - 1) * p.ldq;
-  // chunk c of row r lies at 4 r + (c ^ r / 4 % 4): reads and writes without bank conflicts
+  // chunk c of row r lies at 4 r + (c ^ r / 4 % 4), which spreads both orders over the banks (16 rows of
+  // 28000 x 8192: a fifth of the LDS cycles are conflicts)
   u32x4 *turn = &lds.turn[wave][0][0];
   const int put = 4 * r4 + (c4 ^ (r4 / 4 % 4)), get = 4 * l16 + (lq ^ (l16 / 4 % 4));
   const int blocks = (p.k + kBlock - 1) / kBlock, bytes = (p.k + 1) / 2;

@@ -30,11 +30,11 @@
 // composes its initial state from the maps of the tiles before it in its run of kRun tiles and the
 // state at the start of the run, which the last tile of the run before publishes.  What is composed
 // with what does not depend on timing, so results are the same bits every time.  Measured against
-// a workgroup that walks the tiles of its channels (forward, us): 1 x 65536 x 1024 fp32 154 against
+// a workgroup that walks the tiles of its channels (forward, us): 1 x 65536 x 1024 fp32 152 against
 // 2017 (295 with time cut into segments whose maps a first kernel computes, which reads x and g
-// twice), 4 x 4096 x 4096 bf16 91 against 136, 8 x 2048 x 8192 bf16 167 against 186.  That is 5.2,
-// 4.4 and 4.8 TB/s; a large copy reaches 5.1 to 5.3 on the same card.  Backward: 245, 146 and 265 us
-// (5.5, 4.6 and 5.1 TB/s).
+// twice), 4 x 4096 x 4096 bf16 97 against 136, 8 x 2048 x 8192 bf16 169 against 186.  That is 5.3,
+// 4.2 and 4.8 TB/s; a large copy reaches 5.1 to 5.3 on the same card.  Backward: 248, 150 and 275 us
+// (5.4, 4.5 and 4.9 TB/s).
 // Copyright 2026 veles.simd_amd authors. Apache-2.0.
 #include <hip/hip_runtime.h>
 
