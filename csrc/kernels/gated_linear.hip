@@ -963,6 +963,9 @@ __global__ __launch_bounds__(256) void slope_kernel(Slopes p) {
       const float v = N::load(d[e]);
       vg[e] = v * gu[e].y * act_slope(p.act, gu[e].x);
       vu[e] = v * act(p.act, gu[e].x);
+      // one fp32 number each: the compiler would round a product to 16 bits by itself in one place and by way of
+      // fp32 in the other, and rest() would be that of the number next to the one stored
+      asm("" : "+v"(vg[e]), "+v"(vu[e]));
       dg[e] = N::save(vg[e]);
       du[e] = N::save(vu[e]);
     }

@@ -586,3 +586,23 @@ def test_split_gradients_are_refused_before_the_forward_pass(dev):
         ops.gated_linear(x, w, w, split_gradients=True)
     with torch.no_grad():
         assert ops.gated_linear(x, w, w, split_gradients=True).shape == (1, (1 << 19) + 1)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_split_gradients_next_to_a_tie(dev):
+    """Products dh (x w) whose rounding to float32 lies half way between two float16 numbers while the product does not: both
+    numbers of a split gradient have to come from one and the same rounding.  (relu, one row, k = 1: dw_up = dh g x, where g = x w
+    is exact; dh g is rounded to float32 and split, the rest is exact up to the last rounding.)"""
+    g = torch.Generator().manual_seed(17)
+    x = torch.tensor([[1.3310546875]], dtype=torch.float16)
+    w = (torch.rand(1 << 18, generator=g) + 0.5).half()
+    dh = (torch.rand(1 << 18, generator=g) + 0.5).half()
+    p = dh.double() * x.double()[0, 0] * w.double()
+    once = torch.from_numpy(p.numpy().astype("float16"))     # (torch goes by way of float32)
+    found = once != p.float().half()
+    assert 10 <= int(found.sum()) <= 400
+    w, dh, p = w[found][:, None], dh[found][None], p[found][:, None]
+    leaf = w.clone().to(dev).requires_grad_()
+    got, = torch.autograd.grad(ops.gated_linear(x.to(dev), w.to(dev), leaf, "relu", split_gradients=True), leaf, dh.to(dev))
+    ref = p * x.double()
+    _rounded_once("dw_up", got, (ref, ref.abs() * (2.0 ** -24 + 2.0 ** -22) + 2.0 ** -25 * x.double()))
