@@ -8,16 +8,17 @@
 // Bound: the bandwidth of reading q (the rows of x and y are a few KB).  So the work per weight has
 // to be small: unpacked to fp32 and multiplied on the vector units, three instructions a weight
 // would take as long as reading it.  Here a weight costs one: the four bits are masked into the
-// mantissa of a bf16 or fp16 number 16 (0x4180 | q << 3 or 0x4c00 | q << 6), which is 16 + q
+// mantissa of a bf16 or fp16 number 1 (0x3f80 | q << 3 or 0x3c00 | q << 6), which is 1 + q / 16
 // exactly, two to a register, and the matrix cores multiply (16 x 16 x 32, x as the A operand,
 // rows it does not have are zero).  Per group and column the fp32 sums then become
 //
-//   s (sum x (16 + q) - (16 + z) sum x)
+//   s (sum x (1 + q / 16) - (16 + z) sum x / 16)
 //
-// where sum x comes from one more product, with ones, in the layout it is needed in.  Weights are never
-// rounded.  What is rounded, to 2^-24 each time, are sums of |x| (16 + q) s and |x| (16 + z) s, not of
-// |x (q - z)| s: weights near their zero point give a remainder of that size in the place of a smaller sum or
-// of 0, and a group's sum of 31 |x| (of (16 + z) |x| where z > 15) has to stay below fp32's largest number.
+// where sum x / 16 comes from one more product, with sixteenths, in the layout it is needed in; the result is
+// multiplied by 16 at the end.  Weights are never rounded.  What is rounded, to 2^-24 each time, are sums of
+// |x| (16 + q) s and |x| (16 + z) s, not of |x (q - z)| s: weights near their zero point give a remainder of that
+// size in the place of a smaller sum or of 0, and a group's sum of 2 |x| (of (1 + z / 16) |x| where z > 15) has
+// to stay below fp32's largest number.
 //
 // A step is 128 k of 16 columns: 64 bytes of each row, which four neighbouring lanes load.  (16
 // neighbouring lanes on 16 rows, the order the matrix instruction wants, cost the cache four times
@@ -76,7 +77,7 @@ __device__ __forceinline__ floatx4 mma(const Frag &a, const Frag &b, floatx4 c) 
                                                   __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
-// Eight 4-bit numbers as 16 + q: pair p is (q_p, q_{p + 4}).  `base` holds 16 twice; it comes in a
+// Eight 4-bit numbers as 1 + q / 16: pair p is (q_p, q_{p + 4}).  `base` holds 1 twice; it comes in a
 // register, where the mask and it can be operands of one and-or.
 template <class N>
 __device__ __forceinline__ Frag unpack(uint32_t w, uint32_t base) {
@@ -207,10 +208,10 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))
     __builtin_amdgcn_wave_barrier();
   };
 
-  const Frag ones = std::is_same_v<N, num::BF16>
-                        ? Frag{{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u}}
-                        : Frag{{0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u}};
-  uint32_t base = std::is_same_v<N, num::BF16> ? 0x41804180u : 0x4c004c00u;
+  const Frag sixteenths = std::is_same_v<N, num::BF16>
+                              ? Frag{{0x3d803d80u, 0x3d803d80u, 0x3d803d80u, 0x3d803d80u}}
+                              : Frag{{0x2c002c00u, 0x2c002c00u, 0x2c002c00u, 0x2c002c00u}};
+  uint32_t base = std::is_same_v<N, num::BF16> ? 0x3f803f80u : 0x3c003c00u;
   asm volatile("" : "+v"(base));
   float sum[CT][RV];
 #pragma unroll
@@ -249,7 +250,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))
 #pragma unroll
       for (int j = i * GS; j < (i + 1) * GS; j++) {
         const Frag a = pairs(x[j]);
-        sx = mma<N>(a, ones, sx);
+        sx = mma<N>(a, sixteenths, sx);
 #pragma unroll
         for (int c = 0; c < CT; c++) acc[c] = mma<N>(a, unpack<N>(q[c][j], base), acc[c]);
       }
@@ -333,7 +334,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))
 #pragma unroll
     for (int w = 0; w < kWaves; w++) total += lds.part[w][c][r][l];
     const int mm = m0 + l / 16 + 4 * r, nn = n0 + 16 * c + l % 16;
-    if (mm < p.m && nn < p.n) p.y[static_cast<int64_t>(mm) * p.n + nn] = N::save(total);
+    if (mm < p.m && nn < p.n) p.y[static_cast<int64_t>(mm) * p.n + nn] = N::save(16.f * total);
   }
 }
 

@@ -378,8 +378,8 @@ vs_status vs_gated_recurrence_step(int dtype, const void *x, int64_t x_batch, co
 /// x [m][k] with row stride ldx (elements; 0: one row for all); qweight [n][(k + 1) / 2] bytes with
 /// row stride ldq, two numbers to a byte, the even k in the low half; scales (x's
 /// type) and zeros (bytes; NULL: 8) [n][ceil(k / group)]; y [m][n].  group: 32,
-/// 64 or a multiple of 128.  Sums are fp32, of x (16 + q) and x (16 + zeros), which have to be finite for every
-/// group; their rounding is relative to sum |x| (32 + q + zeros) scales.  Every 16 rows read the weights once.
+/// 64 or a multiple of 128.  Sums are fp32, of x (1 + q / 16) and x (1 + zeros / 16), which have to be finite
+/// for every group; their rounding is relative to sum |x| (32 + q + zeros) scales.  Every 16 rows read the weights once.
 vs_status vs_matvec_int4(int dtype, const void *x, int64_t ldx, const uint8_t *qweight,
                          int64_t ldq, const void *scales, const uint8_t *zeros, int64_t group,
                          int64_t m, int64_t n, int64_t k, void *y, vs_stream_t stream);

@@ -244,10 +244,11 @@ def test_weights_at_and_far_from_their_zero_point(dev, dtype, m, n, k, group, ki
 
 
 @pytest.mark.parametrize("dev", DEVICES)
-def test_large_finite_values(dev):
-    """Values up to the limit that the documentation names: 31 sum |x| of a group of 128 just below 3.4e38."""
+@pytest.mark.parametrize("most", [1e37, 1.6e38])
+def test_large_finite_values(dev, most):
+    """Values up to the limit that the documentation names: 2 sum |x| of a group of 128 just below 3.4e38."""
     x, q, s, z = _inputs(4, 50, 512, 128, torch.bfloat16, dev, seed=24)
-    x = (x.double() / x.double().abs().view(4, 4, 128).sum(-1).max() * 1e37).bfloat16()
+    x = (x.double() / x.double().abs().view(4, 4, 128).sum(-1).max() * most).bfloat16()
     y = ops.matvec_int4(x, q, s, z, 128)
     assert torch.isfinite(y).all()
     _check_offsets(y, x, q, s, z, 128)
