@@ -407,8 +407,9 @@ def matvec_int4(x: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor,
     group_size: 32, 64 or a multiple of 128; the last group may end early.  Weights are exact and sums
     are float32; the result is rounded once, to x's type.  On a GPU the zero points are taken off the sums, so
     float32's rounding is relative to sum |x| (32 + q + zeros) scales, also where q is close to zeros, and x has to be
-    finite, with sums of 2 |x| (or (1 + zeros / 16) |x|, where that is more) over a group below 3.4e38.  For generation: it records no gradient; more than 16 rows read the weights
-    once for every 16.  quantize_int4 makes the operands."""
+    finite, with sums of 2 |x| (or (1 + zeros / 16) |x|, where that is more) over a group below 3.4e38.
+    For generation: it records no gradient; more than 16 rows read the weights once for every 16.
+    quantize_int4 makes the operands."""
     if records(x, scales):
         raise RuntimeError("matvec_int4 records no gradient: call it under torch.no_grad()")
     if plain_tensors(x, qweight, scales, zeros):
